@@ -653,6 +653,105 @@ int ifh_silu_mul_bf16(const void *gate_up, void *out, int64_t rows, int ffn, int
 /* values[i] += delta where mask[i] != 0 (mask optional): per-row sequence lengths advanced between graph replays */
 int ifh_add_i32_vec(int32_t *values, const int32_t *mask, int n, int delta, ifh_stream_t stream);
 
+/* ---- the same layer for prompts laid end to end, for decode steps that share a prefix, and for drafted tokens ----
+ * Cache rows as above: bf16 [row][slot][cache_ts], k heads at 0, v heads at v_off.  Lengths and offsets live on the device and are
+ * clamped to what the descriptor's host sizes allow, so that a wrong one gives wrong rows and no access out of range. */
+/* ifh_rope_append_bf16 without padding: token i belongs to the sequence s with cu[s] <= i < cu[s+1] (cu int32 [nseqs+1],
+ * non-decreasing, cu[0] = 0), turns by the angles of position pos0[s] + i - cu[s] and is appended to cache row s at slot
+ * slot0[s] + i - cu[s] (slot0 NULL: the position; a row behind a shared prefix has slots smaller than its positions).  q goes to q_out,
+ * which may be qkv itself (q_ld = qkv_ld) and otherwise does not overlap it.  Tokens behind cu[nseqs], tokens whose position is outside
+ * the table's table_len rows, and k | v whose slot is outside 0 .. max_pos-1 are left alone. */
+typedef struct ifh_rope_packed_desc {
+    const void *qkv;
+    int64_t qkv_ld;
+    void *q_out;
+    int64_t q_ld;
+    const float *cos_sin;      /* f32 [table_len][head_dim/2][2] */
+    void *cache;
+    int64_t cache_bs, cache_ts;
+    const int32_t *cu, *pos0, *slot0;
+    int32_t ntokens, nseqs, nheads, nkv, head_dim, max_pos, table_len;
+} ifh_rope_packed_desc;
+int ifh_rope_append_packed_bf16(const ifh_rope_packed_desc *desc, ifh_stream_t stream);
+/* Causal grouped-query attention of sequences laid end to end: sequence s has the tokens cu[s] .. cu[s+1]-1 and the first key_len[s]
+ * keys of cache row s; its last token sees all of them, the one before one fewer, and so on (new tokens behind what the row already
+ * holds, themselves appended before).  A token that sees no key gets zeros; tokens behind cu[nseqs] keep what out holds.  Any number of
+ * query heads per kv head; head_dim 64 or 128.  softmax(scale q.k) v, f32 sums; the probabilities are rounded to bf16 for the second
+ * product.  V rows a token does not see, inside the 64-key tile its last key is in, are multiplied by zero: they have to be finite
+ * up to key_len.  Slots from key_len on are not used.
+ * ws: f32 workspace of ifh_attn_packed_ws_floats() elements, with which few long rows are split along their keys (NULL, or
+ * where that function says 0: they are not).  A workspace belongs to one stream / graph at a time. */
+typedef struct ifh_attn_packed_desc {
+    const void *q;
+    int64_t q_ts;
+    const void *cache;
+    int64_t cache_bs, cache_ts;
+    int32_t v_off;
+    void *out;
+    int64_t o_ts;
+    const int32_t *cu, *key_len;
+    int32_t ntokens, nseqs, nheads, nkv, head_dim, max_keys;       /* max_keys >= every key_len */
+    float scale;
+    float *ws;
+    int64_t ws_floats;
+} ifh_attn_packed_desc;
+int64_t ifh_attn_packed_ws_floats(int ntokens, int nseqs, int nheads, int nkv, int head_dim, int max_keys);
+int ifh_attn_packed_bf16(const ifh_attn_packed_desc *desc, ifh_stream_t stream);
+/* Grouped-query attention of a decode step whose rows share a prefix: token i of row b = i / tokens_per_row sees the first
+ * prefix_len[b] keys of the one row `prefix` (bf16 [prefix_keys][prefix_ts]; prefix_len NULL: all of them; 0: none) and the first
+ * key_len[i] keys of cache row b.  The prefix is read once for all rows, not once a row.  A token that sees no key gets zeros.
+ * tokens_per_row > 1: drafted tokens, each with its own key_len.  ws: ifh_attn_prefix_ws_floats() f32, of one stream / graph at a time. */
+typedef struct ifh_attn_prefix_desc {
+    const void *q;
+    int64_t q_ts;
+    const void *prefix;
+    int64_t prefix_ts;
+    const void *cache;
+    int64_t cache_bs, cache_ts;
+    int32_t v_off;
+    void *out;
+    int64_t o_ts;
+    const int32_t *prefix_len, *key_len;                            /* [nrows] or NULL, [nrows * tokens_per_row] */
+    int32_t nrows, tokens_per_row, prefix_keys, nheads, nkv, head_dim, max_keys;
+    float scale;
+    float *ws;
+    int64_t ws_floats;
+} ifh_attn_prefix_desc;
+int64_t ifh_attn_prefix_ws_floats(int nrows, int tokens_per_row, int prefix_keys, int nheads, int nkv, int head_dim, int max_keys);
+int ifh_attn_prefix_bf16(const ifh_attn_prefix_desc *desc, ifh_stream_t stream);
+/* Verification of drafted tokens (speculative decoding by rejection, which keeps the target's distribution).  Row r has ndraft drafts
+ * (lens int32 [nrows], optional: its own number, 0 .. ndraft) and ndraft + 1 target rows, r * (ndraft+1) + i: the distribution p_i of the
+ * token at draft i's place given the drafts before it.  Draft i, drawn from q_i, is kept while uniform[r][i] * q_i(x_i) < p_i(x_i);
+ * at the first refusal the token is drawn from max(p_i - q_i, 0) (from p_i where that is zero everywhere), behind the last draft from
+ * p_n: the first token, in the order of the ids (or of the candidates), whose cumulated mass exceeds uniform[r][ndraft] times the whole.
+ * out_tokens int32 [nrows][ndraft+1]: the kept drafts, the drawn token, then -1; out_count int32 [nrows]: kept + 1.  uniform f32
+ * [nrows][ndraft+1] in [0, 1).  Masses and sums are f64, so the token does not depend on how a sum is split.
+ * A draft outside the vocabulary is refused; a row of logits with nothing above -inf refuses its draft and draws -1; NaN counts as -inf. */
+/* p_i = softmax(logits / temperature), f32 logits [nrows*(ndraft+1)][ld]; temperature 0: p_i is 1 at the arg-max (the lowest id of
+ * equals).  draft_probs f32 [nrows*ndraft][q_ld], or NULL: q_i is 1 at the draft (a draft that was looked up, not drawn).
+ * ws: ifh_verify_drafts_ws_bytes() bytes, 16-byte aligned, of one stream / graph at a time. ndraft <= 63. */
+typedef struct ifh_verify_desc {
+    const float *logits;
+    int64_t ld;
+    const float *draft_probs;
+    int64_t q_ld;
+    const int32_t *drafts, *lens;
+    const float *uniform;
+    int32_t *out_tokens, *out_count;
+    int32_t vocab, nrows, ndraft;
+    float temperature;
+    void *ws;
+    int64_t ws_bytes;
+} ifh_verify_desc;
+int64_t ifh_verify_drafts_ws_bytes(int nrows, int ndraft);
+int ifh_verify_drafts_f32(const ifh_verify_desc *desc, ifh_stream_t stream);
+/* The same where both distributions are the top-k sampler's: cand / probs [nrows*(ndraft+1)][32] are out_cand / out_probs of
+ * ifh_sample_topk_f32 on the target's logits (ids of a row distinct, dropped ones with probability 0), draft_cand / draft_probs
+ * [nrows*ndraft][32] the draft's, both or neither (neither: q_i is 1 at the draft). */
+int ifh_verify_drafts_topk(const int32_t *cand, const float *probs, const int32_t *draft_cand, const float *draft_probs,
+                           const int32_t *drafts, const int32_t *lens, const float *uniform, int nrows, int ndraft,
+                           int32_t *out_tokens, int32_t *out_count, ifh_stream_t stream);
+
 /* ---- TTS streaming glue, HelloSippyRTPipe.infer (HelloSippyRTPipe.py:191-240) ---- */
 /* stop rule (:227-228) on the 2 stop logits per utterance (row stride logits_ld floats); ends_at int64[n].
  * dyn_minmax (optional, device int32[2] = {minlen, maxlen}) overrides the by-value lengths: a launch captured in a

@@ -132,6 +132,38 @@ class GqaDesc(ctypes.Structure):
                 ('scale', _f), ('rope_cos_sin', _vp)]
 
 
+class RopePackedDesc(ctypes.Structure):
+    """ifh_rope_packed_desc (include/infernos_hip.h)"""
+    _fields_ = [('qkv', _vp), ('qkv_ld', _i64), ('q_out', _vp), ('q_ld', _i64), ('cos_sin', _vp), ('cache', _vp), ('cache_bs', _i64),
+                ('cache_ts', _i64), ('cu', _vp), ('pos0', _vp), ('slot0', _vp), ('ntokens', ctypes.c_int32), ('nseqs', ctypes.c_int32),
+                ('nheads', ctypes.c_int32), ('nkv', ctypes.c_int32), ('head_dim', ctypes.c_int32), ('max_pos', ctypes.c_int32),
+                ('table_len', ctypes.c_int32)]
+
+
+class AttnPackedDesc(ctypes.Structure):
+    """ifh_attn_packed_desc (include/infernos_hip.h)"""
+    _fields_ = [('q', _vp), ('q_ts', _i64), ('cache', _vp), ('cache_bs', _i64), ('cache_ts', _i64), ('v_off', ctypes.c_int32),
+                ('out', _vp), ('o_ts', _i64), ('cu', _vp), ('key_len', _vp), ('ntokens', ctypes.c_int32), ('nseqs', ctypes.c_int32),
+                ('nheads', ctypes.c_int32), ('nkv', ctypes.c_int32), ('head_dim', ctypes.c_int32), ('max_keys', ctypes.c_int32),
+                ('scale', _f), ('ws', _vp), ('ws_floats', _i64)]
+
+
+class AttnPrefixDesc(ctypes.Structure):
+    """ifh_attn_prefix_desc (include/infernos_hip.h)"""
+    _fields_ = [('q', _vp), ('q_ts', _i64), ('prefix', _vp), ('prefix_ts', _i64), ('cache', _vp), ('cache_bs', _i64),
+                ('cache_ts', _i64), ('v_off', ctypes.c_int32), ('out', _vp), ('o_ts', _i64), ('prefix_len', _vp), ('key_len', _vp),
+                ('nrows', ctypes.c_int32), ('tokens_per_row', ctypes.c_int32), ('prefix_keys', ctypes.c_int32),
+                ('nheads', ctypes.c_int32), ('nkv', ctypes.c_int32), ('head_dim', ctypes.c_int32), ('max_keys', ctypes.c_int32),
+                ('scale', _f), ('ws', _vp), ('ws_floats', _i64)]
+
+
+class VerifyDesc(ctypes.Structure):
+    """ifh_verify_desc (include/infernos_hip.h)"""
+    _fields_ = [('logits', _vp), ('ld', _i64), ('draft_probs', _vp), ('q_ld', _i64), ('drafts', _vp), ('lens', _vp), ('uniform', _vp),
+                ('out_tokens', _vp), ('out_count', _vp), ('vocab', ctypes.c_int32), ('nrows', ctypes.c_int32),
+                ('ndraft', ctypes.c_int32), ('temperature', _f), ('ws', _vp), ('ws_bytes', _i64)]
+
+
 class RtpHdr(ctypes.Structure):
     """ifh_rtp_hdr (include/infernos_hip.h)"""
     _fields_ = [(n, ctypes.c_int32) for n in ('version', 'padding', 'extension', 'cc', 'marker', 'pt')] + \
@@ -183,6 +215,14 @@ SIGNATURES.update({
     'ifh_rmsnorm_bf16': (_i, [_vp, _vp, _vp, _i, _i, _f, _vp]),
     'ifh_rope_append_bf16': (_i, [_vp, _i64, _vp, _i, _vp, _i64, _i64, _vp, _vp, _i, _i, _i, _i, _i, _vp]),
     'ifh_attn_gqa_bf16': (_i, [ctypes.POINTER(GqaDesc), _vp]),
+    'ifh_rope_append_packed_bf16': (_i, [ctypes.POINTER(RopePackedDesc), _vp]),
+    'ifh_attn_packed_ws_floats': (_i64, [_i, _i, _i, _i, _i, _i]),
+    'ifh_attn_packed_bf16': (_i, [ctypes.POINTER(AttnPackedDesc), _vp]),
+    'ifh_attn_prefix_ws_floats': (_i64, [_i, _i, _i, _i, _i, _i, _i]),
+    'ifh_attn_prefix_bf16': (_i, [ctypes.POINTER(AttnPrefixDesc), _vp]),
+    'ifh_verify_drafts_ws_bytes': (_i64, [_i, _i]),
+    'ifh_verify_drafts_f32': (_i, [ctypes.POINTER(VerifyDesc), _vp]),
+    'ifh_verify_drafts_topk': (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _vp, _vp]),
     'ifh_silu_mul_bf16': (_i, [_vp, _vp, _i64, _i, _i, _vp]),
     'ifh_add_i32_vec': (_i, [_vp, _vp, _i, _i, _vp]),
     'ifh_repetition_penalty_f32': (_i, [_vp, _i64, _i, _i, _vp, _i64, _vp, _f, _vp]),

@@ -18,7 +18,9 @@ FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-Wall', '-Wno-u
 # per-file additions: attn.hip's one-wave kernel (k_attn_prefill_few: 48 KB of LDS per wave, so hipcc plans for one wave per SIMD and
 # 512 registers) got its MFMA results in AGPRs with a v_accvgpr copy around every vector instruction that touches them (144 in the tile
 # loop); the VGPR form of the MFMAs is selected for that file (no kernel in it keeps accumulators in AGPRs on purpose)
-EXTRA_FLAGS = {'attn.hip': ['-mllvm', '-amdgpu-mfma-vgpr-form']}
+# packed.hip, verify.hip: no packed f32 arithmetic (v_pk_add / mul / fma_f32 have given wrong results now and then on these boards)
+NO_PACKED_F32 = ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
+EXTRA_FLAGS = {'attn.hip': ['-mllvm', '-amdgpu-mfma-vgpr-form'], 'packed.hip': NO_PACKED_F32, 'verify.hip': NO_PACKED_F32}
 
 
 def flags_for(src):

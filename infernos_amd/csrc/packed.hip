@@ -1,0 +1,471 @@
+// Language-model operators for prompts laid end to end and for decode steps that share a prefix (the serving forms next to llm.hip's
+// padded batches; InfernLLMWorker, Cluster/InfernLLMWorker.py:60-119):
+//   k_rope_packed    rotary embedding of q and k and the append of k | v to the cache rows, tokens of all sequences end to end.
+//   k_attn_rows      softmax(scale q k^T) v of row blocks: a row is one (token, query head), the G heads of a kv head adjacent, so a
+//                    K / V tile serves every head of the group and a block of rows covers few tokens (little work past the diagonal).
+//   k_attn_join      joins the partial results of row blocks whose keys were split.
+#include "common.h"
+
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+namespace ifh {
+
+// index s of the sequence with cu[s] <= i < cu[s + 1] (cu non-decreasing, n + 1 entries); n where there is none
+__device__ __forceinline__ int packed_seq(const int32_t *__restrict__ cu, int n, int i)
+{
+    int lo = 0, hi = n;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (cu[mid + 1] <= i) lo = mid + 1; else hi = mid;
+    }
+    return lo < n && cu[lo] <= i ? lo : n;
+}
+
+// One thread per (token, head slot, 8 pairs j .. j + 7 of the head): the arithmetic and the roundings of k_rope_append (llm.hip).
+__global__ __launch_bounds__(256) void k_rope_packed(const uint16_t *__restrict__ qkv, int64_t qkv_ld, uint16_t *__restrict__ q_out,
+                                                     int64_t q_ld, const float *__restrict__ cs, int table_len,
+                                                     uint16_t *__restrict__ cache, int64_t cache_bs, int64_t cache_ts,
+                                                     const int32_t *__restrict__ cu, const int32_t *__restrict__ pos0,
+                                                     const int32_t *__restrict__ slot0, int nseqs, int nh, int nkv, int hd, int max_pos,
+                                                     int64_t total)
+{
+    const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (idx >= total) return;
+    const int half = hd >> 1, groups = half >> 3, slots = nh + 2 * nkv;
+    const int j = (int)(idx % groups) * 8, slot = (int)((idx / groups) % slots);
+    const int64_t i = idx / ((int64_t)groups * slots);
+    const int s = packed_seq(cu, nseqs, (int)i);
+    if (s >= nseqs) return;
+    const int t = (int)i - cu[s], pos = pos0[s] + t, at = (slot0 ? slot0[s] : pos0[s]) + t;
+    if (pos < 0 || pos >= table_len) return;
+    if (slot >= nh && (at < 0 || at >= max_pos)) return;
+    const uint16_t *src = qkv + i * qkv_ld + (int64_t)slot * hd;
+    uint16_t *dst = slot < nh ? q_out + i * q_ld + (int64_t)slot * hd
+                              : cache + (int64_t)s * cache_bs + (int64_t)at * cache_ts + (int64_t)(slot - nh) * hd;
+    const uint4 lo = *reinterpret_cast<const uint4 *>(src + j), hi = *reinterpret_cast<const uint4 *>(src + j + half);
+    if (slot >= nh + nkv) {                 // value head: plain copy
+        *reinterpret_cast<uint4 *>(dst + j) = lo;
+        *reinterpret_cast<uint4 *>(dst + j + half) = hi;
+        return;
+    }
+    const float *cp = cs + ((int64_t)pos * half + j) * 2;
+    uint4 olo, ohi;
+    const uint32_t *ul = reinterpret_cast<const uint32_t *>(&lo), *uh = reinterpret_cast<const uint32_t *>(&hi);
+    uint32_t *pl = reinterpret_cast<uint32_t *>(&olo), *ph = reinterpret_cast<uint32_t *>(&ohi);
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const float4 c4 = *reinterpret_cast<const float4 *>(cp + 4 * e);       // cos, sin of pairs 2 e, 2 e + 1
+        const float a0 = __uint_as_float(ul[e] << 16), a1 = __uint_as_float(ul[e] & 0xffff0000u);
+        const float b0 = __uint_as_float(uh[e] << 16), b1 = __uint_as_float(uh[e] & 0xffff0000u);
+        pl[e] = f32x2_to_bf16x2(a0 * c4.x - b0 * c4.y, a1 * c4.z - b1 * c4.w);
+        ph[e] = f32x2_to_bf16x2(b0 * c4.x + a0 * c4.y, b1 * c4.z + a1 * c4.w);
+    }
+    *reinterpret_cast<uint4 *>(dst + j) = olo;
+    *reinterpret_cast<uint4 *>(dst + j + half) = ohi;
+}
+
+// How the rows of a launch find their keys.
+//   PACKED   sequence s has the tokens cu[s] .. cu[s+1]-1 and the first key_len[s] keys of cache row s; its last token sees them all,
+//            each earlier one a key less (causal, aligned at the end)
+//   PREFIX   every token sees the first prefix_len[token / T] keys (all of them without a list) of one shared row
+//   OWN      token i of row b = i / T sees the first key_len[i] keys of cache row b
+enum { ROWS_PACKED, ROWS_PREFIX, ROWS_OWN };
+
+struct RowsParams {
+    const uint16_t *q;
+    int64_t q_ts;
+    const uint16_t *kv;
+    int64_t kv_bs, kv_ts;
+    int v_off;
+    uint16_t *out;
+    int64_t o_ts;
+    const int32_t *cu, *key_len;
+    int ntokens, nseqs, nh, nkv, G, T, max_keys;
+    float scale;
+    int nsplit, split0, split_tiles;       // key split: this launch writes parts split0 .. split0 + nsplit - 1 of split_tiles tiles each
+    int64_t part_rows;                     // rows of one part (ntokens * nh)
+    float *part_o, *part_ml;               // [parts][part_rows][hd] f32 unnormalised, [parts][part_rows][2] (max, sum); NULL: write out
+};
+
+// NW waves of 32 rows each.  S^T = K Q^T and O^T = V^T P^T with the 32 x 32 x 16 MFMA: a lane holds one row's scores of 16 of every 32
+// keys, so the softmax of a row is lane-local up to one exchange with lane ^ 32, and P goes from the accumulators of the first product
+// into the operand of the second without leaving the lane (its 8 keys are 8 half + {0..3, 8..11} + 4 (lane / 32): V^T is read in that
+// order, transposed by ds_read_b64_tr_b16).  P is rounded to bf16 for the second product, as a bf16 model does; sums and maxima are f32.
+template <int HD, int NW, int MODE>
+__global__ __launch_bounds__(NW * 64) void k_attn_rows(const RowsParams p)
+{
+    constexpr int KT = 64, KLD = HD + 8, NS = HD / 16, ND = HD / 32, RV = HD / 8, R = NW * 32;
+    __shared__ __attribute__((aligned(16))) uint16_t Ks[KT * KLD];
+    __shared__ __attribute__((aligned(16))) uint16_t Vs[KT * KLD];
+    const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+    const int l32 = lane & 31, h2 = lane >> 5;
+    const int kvh = blockIdx.y, G = p.G;
+
+    // the block's sequence: tokens [n0, n1), first row of the block within it, its cache row and the keys it may read
+    int n0, n1, row0, kbatch, klen;
+    if (MODE == ROWS_PACKED) {
+        // sequence s owns the block slots floor(cu[s] G / R) + s .. : at least ceil(len G / R) of them, so no table of blocks is needed
+        const int x = blockIdx.x;
+        int lo = 0, hi = p.nseqs - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if ((int)((int64_t)p.cu[mid] * G / R) + mid <= x) lo = mid; else hi = mid - 1;
+        }
+        n0 = min(max(p.cu[lo], 0), p.ntokens);
+        n1 = min(max(p.cu[lo + 1], n0), p.ntokens);
+        const int blk = x - ((int)((int64_t)n0 * G / R) + lo);
+        if (blk < 0 || (int64_t)blk * R >= (int64_t)(n1 - n0) * G) return;
+        row0 = blk * R;
+        kbatch = lo;
+        klen = min(max(p.key_len[lo], 0), p.max_keys);
+    } else if (MODE == ROWS_PREFIX) {
+        n0 = 0;
+        n1 = p.ntokens;
+        row0 = blockIdx.x * R;
+        kbatch = 0;
+        klen = p.max_keys;
+    } else {
+        const int blocks = (p.T * G + R - 1) / R;
+        kbatch = blockIdx.x / blocks;
+        n0 = kbatch * p.T;
+        n1 = n0 + p.T;
+        row0 = (blockIdx.x - kbatch * blocks) * R;
+        klen = p.max_keys;
+    }
+    const int n = n1 - n0, row = row0 + wid * 32 + l32, t = row / G, g = row - t * G;
+    const bool ok = t < n;
+    const int tok = n0 + (ok ? t : 0), head = kvh * G + g;
+    int lim = 0;                                               // keys this lane's row sees
+    if (ok) {
+        if (MODE == ROWS_PACKED) lim = klen - (n - 1 - t);
+        else if (MODE == ROWS_PREFIX) lim = p.key_len ? p.key_len[tok / p.T] : klen;
+        else lim = p.key_len[tok];
+        lim = min(max(lim, 0), klen);
+    }
+    int wmax = lim;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) wmax = max(wmax, __shfl_xor(wmax, o, 64));
+    __shared__ int smax[NW];
+    if (lane == 0) smax[wid] = wmax;
+    __syncthreads();
+    int kmax = 0;
+#pragma unroll
+    for (int w = 0; w < NW; w++) kmax = max(kmax, smax[w]);
+    int kt0 = 0, kt1 = (kmax + KT - 1) / KT;
+    if (p.part_o) {
+        kt0 = blockIdx.z * p.split_tiles;
+        kt1 = min(kt1, kt0 + p.split_tiles);
+    }
+
+    bf16x8_t qf[NS];
+#pragma unroll
+    for (int s = 0; s < NS; s++) {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (ok) v = *reinterpret_cast<const uint4 *>(p.q + (int64_t)tok * p.q_ts + (int64_t)head * HD + 16 * s + 8 * h2);
+        qf[s] = __builtin_bit_cast(bf16x8_t, v);
+    }
+    f32x16 o[ND];
+#pragma unroll
+    for (int d = 0; d < ND; d++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) o[d][e] = 0.0f;
+    float mrun = -1e30f, lrun = 0.0f;
+    const float c1 = p.scale * 1.4426950408889634f;
+    const uint16_t *kb = p.kv + (int64_t)kbatch * p.kv_bs + (int64_t)kvh * HD, *vb = kb + p.v_off;
+
+    for (int kt = kt0; kt < kt1; kt++) {
+        const int kbase = kt * KT;
+        __syncthreads();
+        for (int v = tid; v < KT * RV; v += NW * 64) {
+            const int key = v / RV, dv = (v - key * RV) * 8;
+            const int64_t off = (int64_t)min(kbase + key, kmax - 1) * p.kv_ts + dv;      // past the end: the last key, masked below
+            *reinterpret_cast<uint4 *>(&Ks[key * KLD + dv]) = *reinterpret_cast<const uint4 *>(kb + off);
+            *reinterpret_cast<uint4 *>(&Vs[key * KLD + dv]) = *reinterpret_cast<const uint4 *>(vb + off);
+        }
+        __syncthreads();
+        f32x16 s[2];
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) s[c][e] = 0.0f;
+#pragma unroll
+            for (int d = 0; d < NS; d++) {
+                const bf16x8_t kf = *reinterpret_cast<const bf16x8_t *>(&Ks[(c * 32 + l32) * KLD + d * 16 + h2 * 8]);
+                s[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[d], s[c], 0, 0, 0);
+            }
+        }
+        float mloc = mrun;
+#pragma unroll
+        for (int c = 0; c < 2; c++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const int key = kbase + c * 32 + 8 * (e >> 2) + 4 * h2 + (e & 3);
+                s[c][e] = key < lim ? s[c][e] : -INFINITY;
+                mloc = fmaxf(mloc, s[c][e]);
+            }
+        mloc = fmaxf(mloc, __shfl_xor(mloc, 32, 64));
+        const float ms = mloc * c1, alpha = __builtin_amdgcn_exp2f(mrun * c1 - ms);
+        mrun = mloc;
+        float lsum = 0.0f;
+#pragma unroll
+        for (int c = 0; c < 2; c++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                s[c][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c][e], c1, -ms));
+                lsum += s[c][e];
+            }
+        lrun = lrun * alpha + lsum;
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) o[d][e] *= alpha;
+#pragma unroll
+        for (int kk = 0; kk < 4; kk++) {
+            const int c = kk >> 1, e0 = (kk & 1) * 8;
+            uint4 pb;
+            pb.x = f32x2_to_bf16x2(s[c][e0], s[c][e0 + 1]);
+            pb.y = f32x2_to_bf16x2(s[c][e0 + 2], s[c][e0 + 3]);
+            pb.z = f32x2_to_bf16x2(s[c][e0 + 4], s[c][e0 + 5]);
+            pb.w = f32x2_to_bf16x2(s[c][e0 + 6], s[c][e0 + 7]);
+            const bf16x8_t pf = __builtin_bit_cast(bf16x8_t, pb);
+            // lane i of a 16-lane group hands in row i / 4, columns 4 (i % 4) .. + 3 of a 4-key x 16-dim block and gets column i
+            const int key = kk * 16 + 4 * h2 + ((lane & 15) >> 2), col = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+#pragma unroll
+            for (int d = 0; d < ND; d++) {
+                typedef __attribute__((address_space(3))) bf16x4_t *lds4;
+                const bf16x4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)&Vs[key * KLD + 32 * d + col]);
+                const bf16x4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)&Vs[(key + 8) * KLD + 32 * d + col]);
+                const bf16x8_t vf = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf, o[d], 0, 0, 0);
+            }
+        }
+    }
+    lrun += __shfl_xor(lrun, 32, 64);
+    if (!ok) return;
+    if (p.part_o) {
+        const int64_t pr = (int64_t)(p.split0 + blockIdx.z) * p.part_rows + (int64_t)tok * p.nh + head;
+        float *po = p.part_o + pr * HD;
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4)
+                *reinterpret_cast<float4 *>(po + 32 * d + 2 * e + 4 * h2) = make_float4(o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]);
+        if (h2 == 0) *reinterpret_cast<float2 *>(p.part_ml + pr * 2) = make_float2(mrun, lrun);
+        return;
+    }
+    const float inv = lrun > 0.0f ? 1.0f / lrun : 0.0f;
+    uint16_t *op = p.out + (int64_t)tok * p.o_ts + (int64_t)head * HD;
+#pragma unroll
+    for (int d = 0; d < ND; d++)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            uint2 w;
+            w.x = f32x2_to_bf16x2(o[d][e] * inv, o[d][e + 1] * inv);
+            w.y = f32x2_to_bf16x2(o[d][e + 2] * inv, o[d][e + 3] * inv);
+            *reinterpret_cast<uint2 *>(op + 32 * d + 2 * e + 4 * h2) = w;
+        }
+}
+
+// out = sum_j o_j 2^((m_j - m) c1) / sum_j l_j 2^((m_j - m) c1); a row is HD / 4 lanes
+template <int HD>
+__global__ __launch_bounds__(256) void k_attn_join(const float *__restrict__ part_o, const float *__restrict__ part_ml, int64_t rows,
+                                                   int parts, float c1, uint16_t *__restrict__ out, int64_t o_ts, int nh)
+{
+    constexpr int L = HD / 4;
+    const int64_t row = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+    if (row >= rows) return;
+    const int d = (threadIdx.x % L) * 4;
+    float m = -1e30f;
+    for (int j = 0; j < parts; j++) m = fmaxf(m, part_ml[((int64_t)j * rows + row) * 2]);
+    float l = 0.0f;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int j = 0; j < parts; j++) {
+        const int64_t pr = (int64_t)j * rows + row;
+        const float2 ml = *reinterpret_cast<const float2 *>(part_ml + pr * 2);
+        const float w = __builtin_amdgcn_exp2f((ml.x - m) * c1);
+        const float4 v = *reinterpret_cast<const float4 *>(part_o + pr * HD + d);
+        l += ml.y * w;
+        a.x += v.x * w; a.y += v.y * w; a.z += v.z * w; a.w += v.w * w;
+    }
+    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    uint2 w;
+    w.x = f32x2_to_bf16x2(a.x * inv, a.y * inv);
+    w.y = f32x2_to_bf16x2(a.z * inv, a.w * inv);
+    *reinterpret_cast<uint2 *>(out + (row / nh) * o_ts + (row % nh) * HD + d) = w;
+}
+
+}  // namespace ifh
+
+using namespace ifh;
+
+extern "C" int ifh_rope_append_packed_bf16(const ifh_rope_packed_desc *d, ifh_stream_t stream)
+{
+    IFH_CHECK_ARG(d && d->ntokens >= 0 && d->nseqs >= 0);
+    if (d->ntokens == 0 || d->nseqs == 0) return IFH_OK;
+    IFH_CHECK_ARG(d->qkv && d->q_out && d->cos_sin && d->cache && d->cu && d->pos0 && d->table_len >= 1 && d->max_pos >= 1);
+    IFH_CHECK_ARG(d->nheads >= 1 && d->nkv >= 1 && d->head_dim >= 16 && d->head_dim % 16 == 0);
+    const int64_t width = (int64_t)(d->nheads + 2 * (int64_t)d->nkv) * d->head_dim;
+    IFH_CHECK_ARG(width < (1ll << 24) && d->qkv_ld >= width && d->q_ld >= (int64_t)d->nheads * d->head_dim);
+    IFH_CHECK_ARG(d->cache_ts >= (int64_t)2 * d->nkv * d->head_dim && d->cache_bs / d->max_pos >= d->cache_ts);
+    IFH_CHECK_ARG(d->qkv_ld % 8 == 0 && d->q_ld % 8 == 0 && d->cache_bs % 8 == 0 && d->cache_ts % 8 == 0);
+    IFH_CHECK_ARG(((((uintptr_t)d->qkv) | ((uintptr_t)d->q_out) | ((uintptr_t)d->cache) | ((uintptr_t)d->cos_sin)) & 15) == 0);
+    const int64_t total = (int64_t)d->ntokens * (width / 16);
+    IFH_CHECK_ARG(total / 256 < (1ll << 31) - 1);
+    hipLaunchKernelGGL(k_rope_packed, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, as_stream(stream), (const uint16_t *)d->qkv,
+                       d->qkv_ld, (uint16_t *)d->q_out, d->q_ld, d->cos_sin, d->table_len, (uint16_t *)d->cache, d->cache_bs, d->cache_ts,
+                       d->cu, d->pos0, d->slot0, d->nseqs, d->nheads, d->nkv, d->head_dim, d->max_pos, total);
+    IFH_LAUNCH_CHECK("rope_append_packed");
+    return IFH_OK;
+}
+
+// tiles of 64 keys per part and the number of parts, for `blocks` row blocks over max_keys keys: enough parts to give the device two
+// workgroups per CU, none of fewer than four tiles
+static int split_parts(int64_t blocks, int max_keys, int *tiles_per_part)
+{
+    const int tiles = (max_keys + 63) / 64;
+    const int64_t want = 2 * (int64_t)device_cu_count_physical() / (blocks > 0 ? blocks : 1);
+    int parts = (int)(want < 1 ? 1 : want > 64 ? 64 : want);
+    if (parts > tiles / 4) parts = tiles / 4 > 1 ? tiles / 4 : 1;
+    const int per = (tiles + parts - 1) / parts;
+    *tiles_per_part = per;
+    return (tiles + per - 1) / per;
+}
+
+static int64_t part_floats(int64_t rows, int parts, int hd) { return rows * parts * (hd + 2); }
+
+template <int MODE>
+static void rows_launch(const RowsParams &p, int hd, int64_t blocks, hipStream_t st)
+{
+    const dim3 grid((unsigned)blocks, (unsigned)p.nkv, (unsigned)(p.part_o ? p.nsplit : 1));
+    if (hd == 128) hipLaunchKernelGGL((k_attn_rows<128, 4, MODE>), grid, dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((k_attn_rows<64, 4, MODE>), grid, dim3(256), 0, st, p);
+}
+
+static void join_launch(const RowsParams &p, int hd, int parts, hipStream_t st)
+{
+    const int64_t rows = p.part_rows, per = 256 / (hd / 4);
+    const dim3 grid((unsigned)((rows + per - 1) / per));
+    const float c1 = p.scale * 1.4426950408889634f;
+    if (hd == 128) hipLaunchKernelGGL(k_attn_join<128>, grid, dim3(256), 0, st, p.part_o, p.part_ml, rows, parts, c1, p.out, p.o_ts, p.nh);
+    else hipLaunchKernelGGL(k_attn_join<64>, grid, dim3(256), 0, st, p.part_o, p.part_ml, rows, parts, c1, p.out, p.o_ts, p.nh);
+}
+
+constexpr int kRows = 128;      // rows of a block
+
+static int64_t packed_blocks(int64_t ntokens, int64_t nseqs, int G) { return ntokens * G / kRows + nseqs; }
+
+extern "C" int64_t ifh_attn_packed_ws_floats(int ntokens, int nseqs, int nheads, int nkv, int head_dim, int max_keys)
+{
+    if (ntokens <= 0 || nseqs <= 0 || nkv <= 0 || nheads < nkv || nheads % nkv || max_keys <= 0) return 0;
+    int per;
+    const int parts = split_parts(packed_blocks(ntokens, nseqs, nheads / nkv) * nkv, max_keys, &per);
+    return parts > 1 ? part_floats((int64_t)ntokens * nheads, parts, head_dim) : 0;
+}
+
+// what the two attention descriptors share
+#define IFH_CHECK_HEADS(d)                                                                                                          \
+    IFH_CHECK_ARG((d)->nkv >= 1 && (d)->nkv < 65536 && (d)->nheads >= 1 && (d)->nheads <= 65536 && (d)->nheads % (d)->nkv == 0);     \
+    IFH_CHECK_ARG((d)->head_dim == 64 || (d)->head_dim == 128);                                                                     \
+    IFH_CHECK_ARG((d)->scale > 0.0f && (d)->scale < 1e6f);                                                                          \
+    IFH_CHECK_ARG((d)->q_ts >= (int64_t)(d)->nheads * (d)->head_dim && (d)->o_ts >= (int64_t)(d)->nheads * (d)->head_dim);           \
+    IFH_CHECK_ARG((d)->v_off >= 0 && (d)->cache_ts >= (int64_t)(d)->v_off + (int64_t)(d)->nkv * (d)->head_dim);                      \
+    IFH_CHECK_ARG((d)->cache_bs / (d)->max_keys >= (d)->cache_ts);                                                                  \
+    IFH_CHECK_ARG((d)->q_ts % 8 == 0 && (d)->o_ts % 8 == 0 && (d)->cache_bs % 8 == 0 && (d)->cache_ts % 8 == 0 && (d)->v_off % 8 == 0); \
+    IFH_CHECK_ARG(((((uintptr_t)(d)->q) | ((uintptr_t)(d)->cache) | ((uintptr_t)(d)->out) | ((uintptr_t)(d)->ws)) & 15) == 0)
+
+extern "C" int ifh_attn_packed_bf16(const ifh_attn_packed_desc *d, ifh_stream_t stream)
+{
+    IFH_CHECK_ARG(d && d->ntokens >= 0 && d->nseqs >= 0);
+    if (d->ntokens == 0 || d->nseqs == 0) return IFH_OK;
+    IFH_CHECK_ARG(d->q && d->cache && d->out && d->cu && d->key_len && d->max_keys >= 1 && d->max_keys <= (1 << 30));
+    IFH_CHECK_HEADS(d);
+    RowsParams p = {};
+    p.q = (const uint16_t *)d->q; p.q_ts = d->q_ts;
+    p.kv = (const uint16_t *)d->cache; p.kv_bs = d->cache_bs; p.kv_ts = d->cache_ts; p.v_off = d->v_off;
+    p.out = (uint16_t *)d->out; p.o_ts = d->o_ts;
+    p.cu = d->cu; p.key_len = d->key_len;
+    p.ntokens = d->ntokens; p.nseqs = d->nseqs; p.nh = d->nheads; p.nkv = d->nkv; p.G = d->nheads / d->nkv; p.T = 1;
+    p.max_keys = d->max_keys; p.scale = d->scale;
+    p.part_rows = (int64_t)d->ntokens * d->nheads;
+    const int64_t blocks = packed_blocks(d->ntokens, d->nseqs, p.G);
+    IFH_CHECK_ARG(blocks < (1ll << 31) && (int64_t)d->ntokens * p.G < (1ll << 30) && p.part_rows < (1ll << 33));
+    p.nsplit = split_parts(blocks * p.nkv, d->max_keys, &p.split_tiles);
+    if (d->ws && p.nsplit > 1) {
+        IFH_CHECK_ARG(d->ws_floats >= part_floats(p.part_rows, p.nsplit, d->head_dim));
+        p.part_o = d->ws;
+        p.part_ml = d->ws + p.part_rows * p.nsplit * d->head_dim;
+    }
+    hipStream_t st = as_stream(stream);
+    rows_launch<ROWS_PACKED>(p, d->head_dim, blocks, st);
+    IFH_LAUNCH_CHECK("attn_packed");
+    if (p.part_o) {
+        join_launch(p, d->head_dim, p.nsplit, st);
+        IFH_LAUNCH_CHECK("attn_packed join");
+    }
+    return IFH_OK;
+}
+
+struct PrefixPlan {
+    int64_t pblocks, oblocks;
+    int pparts, ptiles, oparts, otiles;
+};
+
+static PrefixPlan prefix_plan(int64_t nrows, int64_t T, int prefix_keys, int nheads, int nkv, int max_keys)
+{
+    PrefixPlan r;
+    const int64_t G = nheads / nkv;
+    r.pblocks = (nrows * T * G + kRows - 1) / kRows;
+    r.oblocks = nrows * ((T * G + kRows - 1) / kRows);
+    r.pparts = prefix_keys > 0 ? split_parts(r.pblocks * nkv, prefix_keys, &r.ptiles) : 0;
+    r.oparts = max_keys > 0 ? split_parts(r.oblocks * nkv, max_keys, &r.otiles) : 0;
+    return r;
+}
+
+extern "C" int64_t ifh_attn_prefix_ws_floats(int nrows, int tokens_per_row, int prefix_keys, int nheads, int nkv, int head_dim, int max_keys)
+{
+    if (nrows <= 0 || tokens_per_row <= 0 || nkv <= 0 || nheads < nkv || nheads % nkv) return 0;
+    const PrefixPlan r = prefix_plan(nrows, tokens_per_row, prefix_keys, nheads, nkv, max_keys);
+    return part_floats((int64_t)nrows * tokens_per_row * nheads, r.pparts + r.oparts, head_dim);
+}
+
+extern "C" int ifh_attn_prefix_bf16(const ifh_attn_prefix_desc *d, ifh_stream_t stream)
+{
+    IFH_CHECK_ARG(d && d->nrows >= 0);
+    if (d->nrows == 0) return IFH_OK;
+    IFH_CHECK_ARG(d->q && d->prefix && d->cache && d->out && d->key_len && d->ws && d->tokens_per_row >= 1);
+    IFH_CHECK_ARG(d->prefix_keys >= 1 && d->prefix_keys <= (1 << 30) && d->max_keys >= 1 && d->max_keys <= (1 << 30));
+    IFH_CHECK_HEADS(d);
+    IFH_CHECK_ARG((((uintptr_t)d->prefix) & 15) == 0 && d->prefix_ts % 8 == 0 &&
+                  d->prefix_ts >= (int64_t)d->v_off + (int64_t)d->nkv * d->head_dim);
+    const int64_t ntokens = (int64_t)d->nrows * d->tokens_per_row;
+    IFH_CHECK_ARG(ntokens < (1 << 24));
+    RowsParams p = {};
+    p.q = (const uint16_t *)d->q; p.q_ts = d->q_ts;
+    p.v_off = d->v_off;
+    p.out = (uint16_t *)d->out; p.o_ts = d->o_ts;
+    p.ntokens = (int)ntokens; p.nseqs = d->nrows; p.nh = d->nheads; p.nkv = d->nkv; p.G = d->nheads / d->nkv; p.T = d->tokens_per_row;
+    p.scale = d->scale;
+    p.part_rows = ntokens * d->nheads;
+    const PrefixPlan r = prefix_plan(d->nrows, d->tokens_per_row, d->prefix_keys, d->nheads, d->nkv, d->max_keys);
+    const int parts = r.pparts + r.oparts;
+    IFH_CHECK_ARG(ntokens * p.G < (1ll << 30) && r.oblocks < (1ll << 31) && p.part_rows < (1ll << 33));
+    IFH_CHECK_ARG(d->ws_floats >= part_floats(p.part_rows, parts, d->head_dim));
+    p.part_o = d->ws;
+    p.part_ml = d->ws + p.part_rows * parts * d->head_dim;
+    hipStream_t st = as_stream(stream);
+    p.kv = (const uint16_t *)d->prefix; p.kv_bs = 0; p.kv_ts = d->prefix_ts;
+    p.key_len = d->prefix_len; p.max_keys = d->prefix_keys;
+    p.nsplit = r.pparts; p.split0 = 0; p.split_tiles = r.ptiles;
+    rows_launch<ROWS_PREFIX>(p, d->head_dim, r.pblocks, st);
+    IFH_LAUNCH_CHECK("attn_prefix prefix");
+    p.kv = (const uint16_t *)d->cache; p.kv_bs = d->cache_bs; p.kv_ts = d->cache_ts;
+    p.key_len = d->key_len; p.max_keys = d->max_keys;
+    p.nsplit = r.oparts; p.split0 = r.pparts; p.split_tiles = r.otiles;
+    rows_launch<ROWS_OWN>(p, d->head_dim, r.oblocks, st);
+    IFH_LAUNCH_CHECK("attn_prefix own");
+    join_launch(p, d->head_dim, parts, st);
+    IFH_LAUNCH_CHECK("attn_prefix join");
+    return IFH_OK;
+}

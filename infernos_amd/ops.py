@@ -253,6 +253,93 @@ def sample_topk(logits, uniform, out_tokens, scratch, *, vocab, ld, nrows, tempe
                                               _lib.stream_ptr(logits.device)), 'ifh_sample_topk_f32')
 
 
+def rope_append_packed(qkv, cos_sin, cache, cu, pos0, *, ntokens, nseqs, nheads, nkv, head_dim, max_pos, slot0=None, q_out=None):
+    """rope_append for sequences laid end to end (ifh_rope_append_packed_bf16): token i of the sequence s with cu[s] <= i < cu[s + 1]
+    turns by position pos0[s] + i - cu[s] and goes to slot slot0[s] + i - cu[s] (slot0 None: the position) of cache row s.  q is written
+    to q_out [ntokens, nheads * head_dim], or in place without it."""
+    ts = 2 * nkv * head_dim
+    d = _lib.RopePackedDesc()
+    d.qkv, d.qkv_ld = _addr(qkv), (nheads + 2 * nkv) * head_dim
+    d.q_out, d.q_ld = (d.qkv, d.qkv_ld) if q_out is None else (_addr(q_out), nheads * head_dim)
+    d.cos_sin, d.cache, d.cache_bs, d.cache_ts = _addr(cos_sin), _addr(cache), max_pos * ts, ts
+    d.cu, d.pos0, d.slot0 = _addr(cu), _addr(pos0), _addr(slot0)
+    d.ntokens, d.nseqs, d.nheads, d.nkv, d.head_dim, d.max_pos, d.table_len = ntokens, nseqs, nheads, nkv, head_dim, max_pos, cos_sin.size(0)
+    _lib.check(_lib.lib().ifh_rope_append_packed_bf16(ctypes.byref(d), _lib.stream_ptr(qkv.device)), 'ifh_rope_append_packed_bf16')
+
+
+def _ws(floats, device):
+    return torch.empty(floats, dtype=torch.float32, device=device) if floats > 0 else None
+
+
+def attn_packed_ws(device, *, ntokens, nseqs, nheads, nkv, head_dim, max_keys):
+    """f32 workspace with which attn_packed splits few long rows along their keys; None where it would not.  A caller that captures
+    graphs or uses several streams keeps one for each."""
+    with torch.cuda.device(device):
+        return _ws(_lib.lib().ifh_attn_packed_ws_floats(ntokens, nseqs, nheads, nkv, head_dim, max_keys), device)
+
+
+def attn_packed(q, cache, out, cu, key_len, *, ntokens, nseqs, nheads, nkv, head_dim, max_pos, max_keys, ws=None, q_ts=None):
+    """causal grouped-query attention of sequences laid end to end (ifh_attn_packed_bf16): tokens cu[s] .. cu[s + 1] - 1 of sequence s
+    against the first key_len[s] keys of cache row s, the last token seeing all of them.  q: the first nheads * head_dim columns of rows
+    q_ts apart (None: the fused projection's)"""
+    d = _lib.AttnPackedDesc()
+    d.q, d.q_ts = _addr(q), ((nheads + 2 * nkv) * head_dim if q_ts is None else q_ts)
+    d.cache, d.cache_bs, d.cache_ts, d.v_off = _addr(cache), max_pos * 2 * nkv * head_dim, 2 * nkv * head_dim, nkv * head_dim
+    d.out, d.o_ts, d.cu, d.key_len = _addr(out), nheads * head_dim, _addr(cu), _addr(key_len)
+    d.ntokens, d.nseqs, d.nheads, d.nkv, d.head_dim, d.max_keys = ntokens, nseqs, nheads, nkv, head_dim, max_keys
+    d.scale, d.ws, d.ws_floats = head_dim ** -0.5, _addr(ws), (0 if ws is None else ws.numel())
+    _lib.check(_lib.lib().ifh_attn_packed_bf16(ctypes.byref(d), _lib.stream_ptr(out.device)), 'ifh_attn_packed_bf16')
+    return out
+
+
+def attn_prefix_ws(device, *, nrows, tokens_per_row, prefix_keys, nheads, nkv, head_dim, max_keys):
+    """f32 workspace of attn_prefix, one for each stream / captured graph"""
+    with torch.cuda.device(device):
+        return _ws(_lib.lib().ifh_attn_prefix_ws_floats(nrows, tokens_per_row, prefix_keys, nheads, nkv, head_dim, max_keys), device)
+
+
+def attn_prefix(q, prefix, cache, out, key_len, *, nrows, tokens_per_row, prefix_keys, nheads, nkv, head_dim, max_pos, max_keys, ws,
+                prefix_len=None, q_ts=None):
+    """grouped-query attention of a decode step whose rows share a prefix (ifh_attn_prefix_bf16): token i of row b sees the first
+    prefix_len[b] keys of `prefix` [prefix_keys, 2 * nkv * head_dim] (None: all) and the first key_len[i] keys of cache row b"""
+    d = _lib.AttnPrefixDesc()
+    d.q, d.q_ts = _addr(q), ((nheads + 2 * nkv) * head_dim if q_ts is None else q_ts)
+    d.prefix, d.prefix_ts = _addr(prefix), 2 * nkv * head_dim
+    d.cache, d.cache_bs, d.cache_ts, d.v_off = _addr(cache), max_pos * 2 * nkv * head_dim, 2 * nkv * head_dim, nkv * head_dim
+    d.out, d.o_ts, d.prefix_len, d.key_len = _addr(out), nheads * head_dim, _addr(prefix_len), _addr(key_len)
+    d.nrows, d.tokens_per_row, d.prefix_keys, d.nheads, d.nkv, d.head_dim, d.max_keys = nrows, tokens_per_row, prefix_keys, nheads, nkv, head_dim, max_keys
+    d.scale, d.ws, d.ws_floats = head_dim ** -0.5, _addr(ws), (0 if ws is None else ws.numel())
+    _lib.check(_lib.lib().ifh_attn_prefix_bf16(ctypes.byref(d), _lib.stream_ptr(out.device)), 'ifh_attn_prefix_bf16')
+    return out
+
+
+def verify_drafts_ws(nrows, ndraft, device):
+    """workspace of verify_drafts, one for each stream / captured graph"""
+    return torch.empty(_lib.lib().ifh_verify_drafts_ws_bytes(nrows, ndraft), dtype=torch.uint8, device=device)
+
+
+def verify_drafts(logits, drafts, uniform, out_tokens, out_count, ws, *, vocab, ld, nrows, ndraft, temperature=1.0, draft_probs=None,
+                  q_ld=None, lens=None):
+    """keep or refuse drafted tokens against softmax(logits / temperature) and draw the token behind them (ifh_verify_drafts_f32):
+    logits f32 [nrows * (ndraft + 1), ld], draft_probs f32 [nrows * ndraft, q_ld] or None (drafts that were not drawn), uniform f32
+    [nrows, ndraft + 1] -> out_tokens int32 [nrows, ndraft + 1] (-1 behind the drawn one), out_count int32 [nrows]"""
+    d = _lib.VerifyDesc()
+    d.logits, d.ld, d.draft_probs, d.q_ld = _addr(logits), ld, _addr(draft_probs), (vocab if q_ld is None else q_ld)
+    d.drafts, d.lens, d.uniform = _addr(drafts), _addr(lens), _addr(uniform)
+    d.out_tokens, d.out_count = _addr(out_tokens), _addr(out_count)
+    d.vocab, d.nrows, d.ndraft, d.temperature = vocab, nrows, ndraft, temperature
+    d.ws, d.ws_bytes = _addr(ws), ws.numel() * ws.element_size()
+    _lib.check(_lib.lib().ifh_verify_drafts_f32(ctypes.byref(d), _lib.stream_ptr(logits.device)), 'ifh_verify_drafts_f32')
+
+
+def verify_drafts_topk(cand, probs, drafts, uniform, out_tokens, out_count, *, nrows, ndraft, draft_cand=None, draft_probs=None, lens=None):
+    """verify_drafts on the top-k sampler's distributions (ifh_verify_drafts_topk): cand / probs = sample_topk's out_cand / out_probs on
+    the target's logits, draft_cand / draft_probs the draft's (None: drafts that were not drawn)"""
+    _lib.check(_lib.lib().ifh_verify_drafts_topk(_addr(cand), _addr(probs), _addr(draft_cand), _addr(draft_probs), _addr(drafts), _addr(lens),
+                                                 _addr(uniform), nrows, ndraft, _addr(out_tokens), _addr(out_count),
+                                                 _lib.stream_ptr(cand.device)), 'ifh_verify_drafts_topk')
+
+
 class BeamState:
     """Device-resident state of ifh_beam_step for `nbatch` utterances x `beams` (include/infernos_hip.h: ifh_beam_desc)."""
 
