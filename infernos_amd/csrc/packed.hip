@@ -89,33 +89,64 @@ struct RowsParams {
     float *part_o, *part_ml;               // [parts][part_rows][hd] f32 unnormalised, [parts][part_rows][2] (max, sum); NULL: write out
 };
 
+// max over lanes l and l ^ 32, every lane gets it
+__device__ __forceinline__ float max_half(float m)
+{
+    typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+    const unsigned u = __float_as_uint(m);
+    const u32x2 r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    float a;
+    asm("v_max_f32 %0, %1, %2" : "=v"(a) : "v"(__uint_as_float(r.x)), "v"(__uint_as_float(r.y)));
+    return a;
+}
+
+// 16 bytes a lane from BASE + VOFF (a lane's offset) to LDS address DST + 16 lane
+#define ROWS_DMA(VOFF, BASE, DST)                                                                                          \
+    do {                                                                                                                   \
+        unsigned keep_;                                                                                                    \
+        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0" \
+                     : "=&s"(keep_) : "v"(VOFF), "s"(BASE), "s"(DST) : "memory");                                          \
+    } while (0)
+
 // NW waves of 32 rows each.  S^T = K Q^T and O^T = V^T P^T with the 32 x 32 x 16 MFMA: a lane holds one row's scores of 16 of every 32
 // keys, so the softmax of a row is lane-local up to one exchange with lane ^ 32, and P goes from the accumulators of the first product
 // into the operand of the second without leaving the lane (its 8 keys are 8 half + {0..3, 8..11} + 4 (lane / 32): V^T is read in that
 // order, transposed by ds_read_b64_tr_b16).  P is rounded to bf16 for the second product, as a bf16 model does; sums and maxima are f32.
+//
+// K / V tiles of 64 keys come by LDS-DMA into two buffers, the next tile in flight while this one is multiplied, one barrier a tile.
+// LDS rows are unpadded (the DMA writes 16 bytes a lane in a row), so the 16-byte chunks of key r are permuted on the source side: K chunk
+// c at c ^ (r % 16) (head_dim 64: c ^ (r / 2 % 8)), so that the 16 keys a ds_read_b128 reads at once lie in 16 different bank groups;
+// V chunks in groups of four, group g at g ^ (r % 4) (head_dim 64: g ^ (r / 2 % 2)), so that the four keys x 64 bytes of a transposed
+// read do.
+//
+// The running maximum is raised only when a tile's exceeds it by more than 2^8 in the exponential (a wave decides at once): p then stays
+// below 2^8, sums in f32 lose nothing by it, and the rescaling of the 4 x 16 accumulators is skipped for almost every tile.
 template <int HD, int NW, int MODE>
-__global__ __launch_bounds__(NW * 64) void k_attn_rows(const RowsParams p)
+__global__ __launch_bounds__(NW * 64, 2) void k_attn_rows(const RowsParams p)
 {
-    constexpr int KT = 64, KLD = HD + 8, NS = HD / 16, ND = HD / 32, RV = HD / 8, R = NW * 32;
-    __shared__ __attribute__((aligned(16))) uint16_t Ks[KT * KLD];
-    __shared__ __attribute__((aligned(16))) uint16_t Vs[KT * KLD];
-    const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+    constexpr int KT = 64, NS = HD / 16, ND = HD / 32, R = NW * 32, ROWB = HD * 2, TILE = KT * ROWB, BUF = 2 * TILE;
+    constexpr int CH = HD / 8, PK = 1024 / ROWB;               // chunks of a key, keys of a DMA instruction
+    constexpr int PIECES = TILE / 1024 / NW;                   // DMA instructions a wave issues for K, and for V, of a tile
+    __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * BUF];
+    const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l32 = lane & 31, h2 = lane >> 5;
-    const int kvh = blockIdx.y, G = p.G;
+    const int G = p.G, kvh = blockIdx.x % p.nkv;               // neighbours on different XCDs: with 2, 4 or 8 kv heads an XCD's L2 holds its own heads' keys
+    int xb = blockIdx.x / p.nkv;
 
     // the block's sequence: tokens [n0, n1), first row of the block within it, its cache row and the keys it may read
     int n0, n1, row0, kbatch, klen;
     if (MODE == ROWS_PACKED) {
-        // sequence s owns the block slots floor(cu[s] G / R) + s .. : at least ceil(len G / R) of them, so no table of blocks is needed
-        const int x = blockIdx.x;
+        // sequence s owns the block slots floor(cu[s] G / R) + s .. : at least ceil(len G / R) of them, so no table of blocks is needed;
+        // the last blocks of a long prompt see the most keys and start first
+        xb = gridDim.x / p.nkv - 1 - xb;
         int lo = 0, hi = p.nseqs - 1;
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
-            if ((int)((int64_t)p.cu[mid] * G / R) + mid <= x) lo = mid; else hi = mid - 1;
+            if ((int)((int64_t)p.cu[mid] * G / R) + mid <= xb) lo = mid; else hi = mid - 1;
         }
         n0 = min(max(p.cu[lo], 0), p.ntokens);
         n1 = min(max(p.cu[lo + 1], n0), p.ntokens);
-        const int blk = x - ((int)((int64_t)n0 * G / R) + lo);
+        const int blk = xb - ((int)((int64_t)n0 * G / R) + lo);
         if (blk < 0 || (int64_t)blk * R >= (int64_t)(n1 - n0) * G) return;
         row0 = blk * R;
         kbatch = lo;
@@ -123,20 +154,20 @@ __global__ __launch_bounds__(NW * 64) void k_attn_rows(const RowsParams p)
     } else if (MODE == ROWS_PREFIX) {
         n0 = 0;
         n1 = p.ntokens;
-        row0 = blockIdx.x * R;
+        row0 = xb * R;
         kbatch = 0;
         klen = p.max_keys;
     } else {
         const int blocks = (p.T * G + R - 1) / R;
-        kbatch = blockIdx.x / blocks;
+        kbatch = xb / blocks;
         n0 = kbatch * p.T;
         n1 = n0 + p.T;
-        row0 = (blockIdx.x - kbatch * blocks) * R;
+        row0 = (xb - kbatch * blocks) * R;
         klen = p.max_keys;
     }
     const int n = n1 - n0, row = row0 + wid * 32 + l32, t = row / G, g = row - t * G;
     const bool ok = t < n;
-    const int tok = n0 + (ok ? t : 0), head = kvh * G + g;
+    const int tok = n0 + (ok ? t : 0), head = kvh * G + (ok ? g : 0);
     int lim = 0;                                               // keys this lane's row sees
     if (ok) {
         if (MODE == ROWS_PACKED) lim = klen - (n - 1 - t);
@@ -144,15 +175,22 @@ __global__ __launch_bounds__(NW * 64) void k_attn_rows(const RowsParams p)
         else lim = p.key_len[tok];
         lim = min(max(lim, 0), klen);
     }
-    int wmax = lim;
+    int wmax = lim, wmin = ok ? lim : klen;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) wmax = max(wmax, __shfl_xor(wmax, o, 64));
-    __shared__ int smax[NW];
+    for (int o = 1; o < 32; o <<= 1) {
+        wmax = max(wmax, __shfl_xor(wmax, o, 64));
+        wmin = min(wmin, __shfl_xor(wmin, o, 64));
+    }
+    int *smax = reinterpret_cast<int *>(lds);
     if (lane == 0) smax[wid] = wmax;
+    wmax = __builtin_amdgcn_readfirstlane(wmax);
+    wmin = __builtin_amdgcn_readfirstlane(wmin);
     __syncthreads();
     int kmax = 0;
 #pragma unroll
     for (int w = 0; w < NW; w++) kmax = max(kmax, smax[w]);
+    kmax = __builtin_amdgcn_readfirstlane(kmax);
+    __syncthreads();
     int kt0 = 0, kt1 = (kmax + KT - 1) / KT;
     if (p.part_o) {
         kt0 = blockIdx.z * p.split_tiles;
@@ -162,8 +200,7 @@ __global__ __launch_bounds__(NW * 64) void k_attn_rows(const RowsParams p)
     bf16x8_t qf[NS];
 #pragma unroll
     for (int s = 0; s < NS; s++) {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (ok) v = *reinterpret_cast<const uint4 *>(p.q + (int64_t)tok * p.q_ts + (int64_t)head * HD + 16 * s + 8 * h2);
+        const uint4 v = *reinterpret_cast<const uint4 *>(p.q + (int64_t)tok * p.q_ts + (int64_t)head * HD + 16 * s + 8 * h2);
         qf[s] = __builtin_bit_cast(bf16x8_t, v);
     }
     f32x16 o[ND];
@@ -172,55 +209,103 @@ __global__ __launch_bounds__(NW * 64) void k_attn_rows(const RowsParams p)
 #pragma unroll
         for (int e = 0; e < 16; e++) o[d][e] = 0.0f;
     float mrun = -1e30f, lrun = 0.0f;
-    const float c1 = p.scale * 1.4426950408889634f;
-    const uint16_t *kb = p.kv + (int64_t)kbatch * p.kv_bs + (int64_t)kvh * HD, *vb = kb + p.v_off;
+    const float c1 = p.scale * 1.4426950408889634f, raise = 8.0f / c1;
 
+    // DMA: piece j of wave w brings keys (j NW + w) PK .. + PK - 1 of the tile; lane l -> key l / CH of the piece, LDS chunk l % CH
+    const unsigned lbase = (unsigned)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)lds);
+    const unsigned ts2 = (unsigned)p.kv_ts * 2u;
+    const unsigned char *kbase0 = reinterpret_cast<const unsigned char *>(p.kv + (int64_t)kbatch * p.kv_bs + (int64_t)kvh * HD);
+    const int64_t voff = (int64_t)p.v_off * 2;
+    const int drow = wid * PK + lane / CH, dpos = lane % CH;   // (NW PK is a multiple of 16: the permutation is the same in every piece)
+    const unsigned kch = (unsigned)(HD == 128 ? dpos ^ (drow & 15) : dpos ^ ((drow >> 1) & 7)) * 16u;
+    const unsigned vch = (unsigned)(HD == 128 ? dpos ^ ((drow & 3) << 2) : dpos ^ (((drow >> 1) & 1) << 2)) * 16u;
+    auto issue = [&](int kt) {
+        const unsigned dst = lbase + (unsigned)(kt & 1) * BUF + (unsigned)wid * 1024u;
+        const unsigned char *src = kbase0 + (int64_t)kt * KT * (int64_t)ts2;
+        const int left = kmax - 1 - kt * KT;                   // the last key of the block, relative to the tile
+        if (left >= KT - 1) {
+            const unsigned o0 = (unsigned)drow * ts2;
+#pragma unroll
+            for (int j = 0; j < PIECES; j++) {
+                const unsigned char *sj = src + (int64_t)(j * NW * PK) * (int64_t)ts2;
+                ROWS_DMA(o0 + kch, sj, dst + j * NW * 1024);
+                ROWS_DMA(o0 + vch, sj + voff, dst + TILE + j * NW * 1024);
+            }
+        } else {                                               // past the end: the last key again, masked below
+#pragma unroll
+            for (int j = 0; j < PIECES; j++) {
+                const unsigned o0 = (unsigned)min(drow + j * NW * PK, left) * ts2;
+                ROWS_DMA(o0 + kch, src, dst + j * NW * 1024);
+                ROWS_DMA(o0 + vch, src + voff, dst + TILE + j * NW * 1024);
+            }
+        }
+    };
+    unsigned ka[NS], va[ND];                                   // LDS offsets of this lane's fragments in buffer 0
+#pragma unroll
+    for (int d = 0; d < NS; d++) ka[d] = (unsigned)(l32 * ROWB + ((2 * d + h2) ^ (HD == 128 ? l32 & 15 : (l32 >> 1) & 7)) * 16);
+    {
+        // lane i of a 16-lane group hands in key i / 4, columns 4 (i % 4) .. + 3 of a 4-key x 16-dim block and gets column i
+        const int key = 4 * h2 + ((lane & 15) >> 2), c = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+#pragma unroll
+        for (int d = 0; d < ND; d++) va[d] = (unsigned)(TILE + key * ROWB + ((4 * d + c) ^ (HD == 128 ? (key & 3) << 2 : ((key >> 1) & 1) << 2)) * 16 + (lane & 1) * 8);
+    }
+
+    // (the loads of q are waited for here: left to hipcc their wait falls behind the next tile's DMA)
+#pragma unroll
+    for (int s = 0; s < NS; s++) asm volatile("" : : "v"(qf[s]));
+    if (kt0 < kt1) issue(kt0);
     for (int kt = kt0; kt < kt1; kt++) {
         const int kbase = kt * KT;
-        __syncthreads();
-        for (int v = tid; v < KT * RV; v += NW * 64) {
-            const int key = v / RV, dv = (v - key * RV) * 8;
-            const int64_t off = (int64_t)min(kbase + key, kmax - 1) * p.kv_ts + dv;      // past the end: the last key, masked below
-            *reinterpret_cast<uint4 *>(&Ks[key * KLD + dv]) = *reinterpret_cast<const uint4 *>(kb + off);
-            *reinterpret_cast<uint4 *>(&Vs[key * KLD + dv]) = *reinterpret_cast<const uint4 *>(vb + off);
-        }
-        __syncthreads();
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();                                       // the tile has landed, and the other buffer is no longer read
+        if (kt + 1 < kt1) issue(kt + 1);
+        if (kbase >= wmax) continue;                           // (a wave's rows see nothing of this tile)
+        const unsigned char *buf = lds + (kt & 1) * BUF;
         f32x16 s[2];
 #pragma unroll
         for (int c = 0; c < 2; c++) {
-#pragma unroll
-            for (int e = 0; e < 16; e++) s[c][e] = 0.0f;
+            s[c] = (f32x16){0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int d = 0; d < NS; d++) {
-                const bf16x8_t kf = *reinterpret_cast<const bf16x8_t *>(&Ks[(c * 32 + l32) * KLD + d * 16 + h2 * 8]);
+                const bf16x8_t kf = *reinterpret_cast<const bf16x8_t *>(buf + ka[d] + c * 32 * ROWB);
                 s[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[d], s[c], 0, 0, 0);
             }
         }
-        float mloc = mrun;
+        // the maxima below are asm (fmaxf on MFMA results costs a canonicalising v_max each), for which hipcc inserts no wait states:
+        // 20 here, one more than a 16-pass MFMA's result needs
+        asm volatile("s_nop 15\n\ts_nop 3" : "+v"(s[0]), "+v"(s[1]));
+        if (kbase + KT > wmin) {
+            const int rel = lim - kbase - 4 * h2;
+#pragma unroll
+            for (int c = 0; c < 2; c++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) s[c][e] = c * 32 + 8 * (e >> 2) + (e & 3) < rel ? s[c][e] : -INFINITY;
+        }
+        float mloc = s[0][0];
 #pragma unroll
         for (int c = 0; c < 2; c++)
 #pragma unroll
-            for (int e = 0; e < 16; e++) {
-                const int key = kbase + c * 32 + 8 * (e >> 2) + 4 * h2 + (e & 3);
-                s[c][e] = key < lim ? s[c][e] : -INFINITY;
-                mloc = fmaxf(mloc, s[c][e]);
-            }
-        mloc = fmaxf(mloc, __shfl_xor(mloc, 32, 64));
-        const float ms = mloc * c1, alpha = __builtin_amdgcn_exp2f(mrun * c1 - ms);
-        mrun = mloc;
-        float lsum = 0.0f;
+            for (int e = 0; e < 16; e += 2) asm("v_max3_f32 %0, %0, %1, %2" : "+v"(mloc) : "v"(s[c][e]), "v"(s[c][e + 1]));
+        mloc = max_half(mloc);
+        if (__any(mloc > mrun + raise)) {
+            const float mnew = fmaxf(mrun, mloc), alpha = __builtin_amdgcn_exp2f((mrun - mnew) * c1);
+            mrun = mnew;
+            lrun *= alpha;
+#pragma unroll
+            for (int d = 0; d < ND; d++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) o[d][e] *= alpha;
+        }
+        const float ms = mrun * c1;
+        float ls[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < 2; c++)
 #pragma unroll
             for (int e = 0; e < 16; e++) {
                 s[c][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c][e], c1, -ms));
-                lsum += s[c][e];
+                ls[e & 3] += s[c][e];
             }
-        lrun = lrun * alpha + lsum;
-#pragma unroll
-        for (int d = 0; d < ND; d++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) o[d][e] *= alpha;
+        lrun += (ls[0] + ls[1]) + (ls[2] + ls[3]);
 #pragma unroll
         for (int kk = 0; kk < 4; kk++) {
             const int c = kk >> 1, e0 = (kk & 1) * 8;
@@ -230,13 +315,11 @@ __global__ __launch_bounds__(NW * 64) void k_attn_rows(const RowsParams p)
             pb.z = f32x2_to_bf16x2(s[c][e0 + 4], s[c][e0 + 5]);
             pb.w = f32x2_to_bf16x2(s[c][e0 + 6], s[c][e0 + 7]);
             const bf16x8_t pf = __builtin_bit_cast(bf16x8_t, pb);
-            // lane i of a 16-lane group hands in row i / 4, columns 4 (i % 4) .. + 3 of a 4-key x 16-dim block and gets column i
-            const int key = kk * 16 + 4 * h2 + ((lane & 15) >> 2), col = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
 #pragma unroll
             for (int d = 0; d < ND; d++) {
                 typedef __attribute__((address_space(3))) bf16x4_t *lds4;
-                const bf16x4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)&Vs[key * KLD + 32 * d + col]);
-                const bf16x4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)&Vs[(key + 8) * KLD + 32 * d + col]);
+                const bf16x4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(buf + va[d] + kk * 16 * ROWB));
+                const bf16x4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(buf + va[d] + (kk * 16 + 8) * ROWB));
                 const bf16x8_t vf = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
                 o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf, o[d], 0, 0, 0);
             }
@@ -338,7 +421,7 @@ static int64_t part_floats(int64_t rows, int parts, int hd) { return rows * part
 template <int MODE>
 static void rows_launch(const RowsParams &p, int hd, int64_t blocks, hipStream_t st)
 {
-    const dim3 grid((unsigned)blocks, (unsigned)p.nkv, (unsigned)(p.part_o ? p.nsplit : 1));
+    const dim3 grid((unsigned)(blocks * p.nkv), 1, (unsigned)(p.part_o ? p.nsplit : 1));
     if (hd == 128) hipLaunchKernelGGL((k_attn_rows<128, 4, MODE>), grid, dim3(256), 0, st, p);
     else hipLaunchKernelGGL((k_attn_rows<64, 4, MODE>), grid, dim3(256), 0, st, p);
 }
@@ -371,7 +454,7 @@ extern "C" int64_t ifh_attn_packed_ws_floats(int ntokens, int nseqs, int nheads,
     IFH_CHECK_ARG((d)->scale > 0.0f && (d)->scale < 1e6f);                                                                          \
     IFH_CHECK_ARG((d)->q_ts >= (int64_t)(d)->nheads * (d)->head_dim && (d)->o_ts >= (int64_t)(d)->nheads * (d)->head_dim);           \
     IFH_CHECK_ARG((d)->v_off >= 0 && (d)->cache_ts >= (int64_t)(d)->v_off + (int64_t)(d)->nkv * (d)->head_dim);                      \
-    IFH_CHECK_ARG((d)->cache_bs / (d)->max_keys >= (d)->cache_ts);                                                                  \
+    IFH_CHECK_ARG((d)->cache_ts < (1 << 24) && (d)->cache_bs / (d)->max_keys >= (d)->cache_ts);                                                                  \
     IFH_CHECK_ARG((d)->q_ts % 8 == 0 && (d)->o_ts % 8 == 0 && (d)->cache_bs % 8 == 0 && (d)->cache_ts % 8 == 0 && (d)->v_off % 8 == 0); \
     IFH_CHECK_ARG(((((uintptr_t)(d)->q) | ((uintptr_t)(d)->cache) | ((uintptr_t)(d)->out) | ((uintptr_t)(d)->ws)) & 15) == 0)
 
@@ -390,7 +473,7 @@ extern "C" int ifh_attn_packed_bf16(const ifh_attn_packed_desc *d, ifh_stream_t 
     p.max_keys = d->max_keys; p.scale = d->scale;
     p.part_rows = (int64_t)d->ntokens * d->nheads;
     const int64_t blocks = packed_blocks(d->ntokens, d->nseqs, p.G);
-    IFH_CHECK_ARG(blocks < (1ll << 31) && (int64_t)d->ntokens * p.G < (1ll << 30) && p.part_rows < (1ll << 33));
+    IFH_CHECK_ARG(blocks * p.nkv < (1ll << 31) && (int64_t)d->ntokens * p.G < (1ll << 30) && p.part_rows < (1ll << 33));
     p.nsplit = split_parts(blocks * p.nkv, d->max_keys, &p.split_tiles);
     if (d->ws && p.nsplit > 1) {
         IFH_CHECK_ARG(d->ws_floats >= part_floats(p.part_rows, p.nsplit, d->head_dim));
@@ -437,7 +520,7 @@ extern "C" int ifh_attn_prefix_bf16(const ifh_attn_prefix_desc *d, ifh_stream_t 
     IFH_CHECK_ARG(d->q && d->prefix && d->cache && d->out && d->key_len && d->ws && d->tokens_per_row >= 1);
     IFH_CHECK_ARG(d->prefix_keys >= 1 && d->prefix_keys <= (1 << 30) && d->max_keys >= 1 && d->max_keys <= (1 << 30));
     IFH_CHECK_HEADS(d);
-    IFH_CHECK_ARG((((uintptr_t)d->prefix) & 15) == 0 && d->prefix_ts % 8 == 0 &&
+    IFH_CHECK_ARG((((uintptr_t)d->prefix) & 15) == 0 && d->prefix_ts % 8 == 0 && d->prefix_ts < (1 << 24) &&
                   d->prefix_ts >= (int64_t)d->v_off + (int64_t)d->nkv * d->head_dim);
     const int64_t ntokens = (int64_t)d->nrows * d->tokens_per_row;
     IFH_CHECK_ARG(ntokens < (1 << 24));
@@ -450,7 +533,7 @@ extern "C" int ifh_attn_prefix_bf16(const ifh_attn_prefix_desc *d, ifh_stream_t 
     p.part_rows = ntokens * d->nheads;
     const PrefixPlan r = prefix_plan(d->nrows, d->tokens_per_row, d->prefix_keys, d->nheads, d->nkv, d->max_keys);
     const int parts = r.pparts + r.oparts;
-    IFH_CHECK_ARG(ntokens * p.G < (1ll << 30) && r.oblocks < (1ll << 31) && p.part_rows < (1ll << 33));
+    IFH_CHECK_ARG(ntokens * p.G < (1ll << 30) && r.pblocks * p.nkv < (1ll << 31) && r.oblocks * p.nkv < (1ll << 31) && p.part_rows < (1ll << 33));
     IFH_CHECK_ARG(d->ws_floats >= part_floats(p.part_rows, parts, d->head_dim));
     p.part_o = d->ws;
     p.part_ml = d->ws + p.part_rows * parts * d->head_dim;
