@@ -253,18 +253,30 @@ def sample_topk(logits, uniform, out_tokens, scratch, *, vocab, ld, nrows, tempe
                                               _lib.stream_ptr(logits.device)), 'ifh_sample_topk_f32')
 
 
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _launch(name, like, *args):
+    """fn(*args, the current stream of `like`'s device), with that device current: its tensors may live on another than the caller's"""
+    fn, i = getattr(_lib.lib(), name), like.device.index
+    if i is None:
+        raise _lib.InfernosHipError('%s: a tensor is not on a HIP GPU' % name)
+    if i == torch.cuda.current_device():
+        return _lib.check(fn(*args, _lib.raw_stream(i)), name)
+    with torch.cuda.device(i):
+        return _lib.check(fn(*args, _lib.raw_stream(i)), name)
+
+
 def rope_append_packed(qkv, cos_sin, cache, cu, pos0, *, ntokens, nseqs, nheads, nkv, head_dim, max_pos, slot0=None, q_out=None):
     """rope_append for sequences laid end to end (ifh_rope_append_packed_bf16): token i of the sequence s with cu[s] <= i < cu[s + 1]
     turns by position pos0[s] + i - cu[s] and goes to slot slot0[s] + i - cu[s] (slot0 None: the position) of cache row s.  q is written
     to q_out [ntokens, nheads * head_dim], or in place without it."""
-    ts = 2 * nkv * head_dim
-    d = _lib.RopePackedDesc()
-    d.qkv, d.qkv_ld = _addr(qkv), (nheads + 2 * nkv) * head_dim
-    d.q_out, d.q_ld = (d.qkv, d.qkv_ld) if q_out is None else (_addr(q_out), nheads * head_dim)
-    d.cos_sin, d.cache, d.cache_bs, d.cache_ts = _addr(cos_sin), _addr(cache), max_pos * ts, ts
-    d.cu, d.pos0, d.slot0 = _addr(cu), _addr(pos0), _addr(slot0)
-    d.ntokens, d.nseqs, d.nheads, d.nkv, d.head_dim, d.max_pos, d.table_len = ntokens, nseqs, nheads, nkv, head_dim, max_pos, cos_sin.size(0)
-    _lib.check(_lib.lib().ifh_rope_append_packed_bf16(ctypes.byref(d), _lib.stream_ptr(qkv.device)), 'ifh_rope_append_packed_bf16')
+    ts, ld, x = 2 * nkv * head_dim, (nheads + 2 * nkv) * head_dim, qkv.data_ptr()
+    q, q_ld = (x, ld) if q_out is None else (q_out.data_ptr(), nheads * head_dim)
+    d = _lib.RopePackedDesc(x, ld, q, q_ld, cos_sin.data_ptr(), cache.data_ptr(), max_pos * ts, ts, cu.data_ptr(), pos0.data_ptr(), _ptr(slot0),
+                            ntokens, nseqs, nheads, nkv, head_dim, max_pos, cos_sin.size(0))
+    _launch('ifh_rope_append_packed_bf16', qkv, ctypes.byref(d))
 
 
 def _ws(floats, device):
@@ -282,13 +294,11 @@ def attn_packed(q, cache, out, cu, key_len, *, ntokens, nseqs, nheads, nkv, head
     """causal grouped-query attention of sequences laid end to end (ifh_attn_packed_bf16): tokens cu[s] .. cu[s + 1] - 1 of sequence s
     against the first key_len[s] keys of cache row s, the last token seeing all of them.  q: the first nheads * head_dim columns of rows
     q_ts apart (None: the fused projection's)"""
-    d = _lib.AttnPackedDesc()
-    d.q, d.q_ts = _addr(q), ((nheads + 2 * nkv) * head_dim if q_ts is None else q_ts)
-    d.cache, d.cache_bs, d.cache_ts, d.v_off = _addr(cache), max_pos * 2 * nkv * head_dim, 2 * nkv * head_dim, nkv * head_dim
-    d.out, d.o_ts, d.cu, d.key_len = _addr(out), nheads * head_dim, _addr(cu), _addr(key_len)
-    d.ntokens, d.nseqs, d.nheads, d.nkv, d.head_dim, d.max_keys = ntokens, nseqs, nheads, nkv, head_dim, max_keys
-    d.scale, d.ws, d.ws_floats = head_dim ** -0.5, _addr(ws), (0 if ws is None else ws.numel())
-    _lib.check(_lib.lib().ifh_attn_packed_bf16(ctypes.byref(d), _lib.stream_ptr(out.device)), 'ifh_attn_packed_bf16')
+    kv = nkv * head_dim
+    d = _lib.AttnPackedDesc(q.data_ptr(), nheads * head_dim + 2 * kv if q_ts is None else q_ts, cache.data_ptr(), max_pos * 2 * kv, 2 * kv, kv,
+                            out.data_ptr(), nheads * head_dim, cu.data_ptr(), key_len.data_ptr(), ntokens, nseqs, nheads, nkv, head_dim,
+                            max_keys, head_dim ** -0.5, _ptr(ws), 0 if ws is None else ws.numel())
+    _launch('ifh_attn_packed_bf16', out, ctypes.byref(d))
     return out
 
 
@@ -302,14 +312,11 @@ def attn_prefix(q, prefix, cache, out, key_len, *, nrows, tokens_per_row, prefix
                 prefix_len=None, q_ts=None):
     """grouped-query attention of a decode step whose rows share a prefix (ifh_attn_prefix_bf16): token i of row b sees the first
     prefix_len[b] keys of `prefix` [prefix_keys, 2 * nkv * head_dim] (None: all) and the first key_len[i] keys of cache row b"""
-    d = _lib.AttnPrefixDesc()
-    d.q, d.q_ts = _addr(q), ((nheads + 2 * nkv) * head_dim if q_ts is None else q_ts)
-    d.prefix, d.prefix_ts = _addr(prefix), 2 * nkv * head_dim
-    d.cache, d.cache_bs, d.cache_ts, d.v_off = _addr(cache), max_pos * 2 * nkv * head_dim, 2 * nkv * head_dim, nkv * head_dim
-    d.out, d.o_ts, d.prefix_len, d.key_len = _addr(out), nheads * head_dim, _addr(prefix_len), _addr(key_len)
-    d.nrows, d.tokens_per_row, d.prefix_keys, d.nheads, d.nkv, d.head_dim, d.max_keys = nrows, tokens_per_row, prefix_keys, nheads, nkv, head_dim, max_keys
-    d.scale, d.ws, d.ws_floats = head_dim ** -0.5, _addr(ws), (0 if ws is None else ws.numel())
-    _lib.check(_lib.lib().ifh_attn_prefix_bf16(ctypes.byref(d), _lib.stream_ptr(out.device)), 'ifh_attn_prefix_bf16')
+    kv = nkv * head_dim
+    d = _lib.AttnPrefixDesc(q.data_ptr(), nheads * head_dim + 2 * kv if q_ts is None else q_ts, prefix.data_ptr(), 2 * kv, cache.data_ptr(),
+                            max_pos * 2 * kv, 2 * kv, kv, out.data_ptr(), nheads * head_dim, _ptr(prefix_len), key_len.data_ptr(), nrows,
+                            tokens_per_row, prefix_keys, nheads, nkv, head_dim, max_keys, head_dim ** -0.5, ws.data_ptr(), ws.numel())
+    _launch('ifh_attn_prefix_bf16', out, ctypes.byref(d))
     return out
 
 
@@ -323,21 +330,17 @@ def verify_drafts(logits, drafts, uniform, out_tokens, out_count, ws, *, vocab, 
     """keep or refuse drafted tokens against softmax(logits / temperature) and draw the token behind them (ifh_verify_drafts_f32):
     logits f32 [nrows * (ndraft + 1), ld], draft_probs f32 [nrows * ndraft, q_ld] or None (drafts that were not drawn), uniform f32
     [nrows, ndraft + 1] -> out_tokens int32 [nrows, ndraft + 1] (-1 behind the drawn one), out_count int32 [nrows]"""
-    d = _lib.VerifyDesc()
-    d.logits, d.ld, d.draft_probs, d.q_ld = _addr(logits), ld, _addr(draft_probs), (vocab if q_ld is None else q_ld)
-    d.drafts, d.lens, d.uniform = _addr(drafts), _addr(lens), _addr(uniform)
-    d.out_tokens, d.out_count = _addr(out_tokens), _addr(out_count)
-    d.vocab, d.nrows, d.ndraft, d.temperature = vocab, nrows, ndraft, temperature
-    d.ws, d.ws_bytes = _addr(ws), ws.numel() * ws.element_size()
-    _lib.check(_lib.lib().ifh_verify_drafts_f32(ctypes.byref(d), _lib.stream_ptr(logits.device)), 'ifh_verify_drafts_f32')
+    d = _lib.VerifyDesc(logits.data_ptr(), ld, _ptr(draft_probs), vocab if q_ld is None else q_ld, drafts.data_ptr(), _ptr(lens),
+                        uniform.data_ptr(), out_tokens.data_ptr(), out_count.data_ptr(), vocab, nrows, ndraft, temperature, ws.data_ptr(),
+                        ws.numel() * ws.element_size())
+    _launch('ifh_verify_drafts_f32', logits, ctypes.byref(d))
 
 
 def verify_drafts_topk(cand, probs, drafts, uniform, out_tokens, out_count, *, nrows, ndraft, draft_cand=None, draft_probs=None, lens=None):
     """verify_drafts on the top-k sampler's distributions (ifh_verify_drafts_topk): cand / probs = sample_topk's out_cand / out_probs on
     the target's logits, draft_cand / draft_probs the draft's (None: drafts that were not drawn)"""
-    _lib.check(_lib.lib().ifh_verify_drafts_topk(_addr(cand), _addr(probs), _addr(draft_cand), _addr(draft_probs), _addr(drafts), _addr(lens),
-                                                 _addr(uniform), nrows, ndraft, _addr(out_tokens), _addr(out_count),
-                                                 _lib.stream_ptr(cand.device)), 'ifh_verify_drafts_topk')
+    _launch('ifh_verify_drafts_topk', cand, cand.data_ptr(), probs.data_ptr(), _ptr(draft_cand), _ptr(draft_probs), drafts.data_ptr(), _ptr(lens),
+            uniform.data_ptr(), nrows, ndraft, out_tokens.data_ptr(), out_count.data_ptr())
 
 
 class BeamState:
