@@ -66,19 +66,20 @@ __global__ __launch_bounds__(256) void k_rope_packed(const uint16_t *__restrict_
     *reinterpret_cast<uint4 *>(dst + j + half) = ohi;
 }
 
-// How the rows of a launch find their keys.
-//   PACKED   sequence s has the tokens cu[s] .. cu[s+1]-1 and the first key_len[s] keys of cache row s; its last token sees them all,
+// How the rows of a key set find their keys.
+//   PACKED   sequence s has the tokens cu[s] .. cu[s+1]-1 and the first lim[s] keys of cache row s; its last token sees them all,
 //            each earlier one a key less (causal, aligned at the end)
 //   PREFIX   every token sees the first lim[token / T] keys (all of them without a list) of one shared row
 //   OWN      token i of row b = i / T sees the first lim[i] keys of cache row b
 enum { ROWS_PACKED, ROWS_PREFIX, ROWS_OWN };
 
-// the keys of a launch's workgroups: `parts` parts of part_tiles tiles for each of `blocks` row blocks and each kv head
+// one kind of keys of a launch: `parts` parts of part_tiles tiles for each of `blocks` row blocks and each kv head
 struct KeySet {
     const uint16_t *kv;
     int64_t bs, ts;
     const int32_t *lim;
-    int max_keys, blocks, parts, part_tiles, part0;      // part0: the first part's place in the partial results
+    int mode, narrow, max_keys, blocks, parts, part_tiles;
+    int part0;                             // the first part's place in the partial results
 };
 
 struct RowsParams {
@@ -90,10 +91,13 @@ struct RowsParams {
     const int32_t *cu;
     int ntokens, nseqs, nh, nkv, G, T;
     float scale;
-    KeySet ks;
+    KeySet ks[2];
+    int first;                             // workgroups of ks[0]; the others are ks[1]'s
     int64_t part_rows;                     // rows of one part (ntokens * nh)
     float *part_o, *part_ml;               // [parts][part_rows][hd] f32 unnormalised, [parts][part_rows][2] (max, sum); NULL: write out
 };
+
+constexpr int kWideRows = 128, kWideKeys = 64, kNarrowRows = 32, kNarrowKeys = 32;
 
 // max over lanes l and l ^ 32, every lane gets it
 __device__ __forceinline__ float max_half(float m)
@@ -114,36 +118,161 @@ __device__ __forceinline__ float max_half(float m)
                      : "=&s"(keep_) : "v"(VOFF), "s"(BASE), "s"(DST) : "memory");                                          \
     } while (0)
 
-// NW waves of 32 rows each.  S^T = K Q^T and O^T = V^T P^T with the 32 x 32 x 16 MFMA: a lane holds one row's scores of 16 of every 32
-// keys, so the softmax of a row is lane-local up to one exchange with lane ^ 32, and P goes from the accumulators of the first product
-// into the operand of the second without leaving the lane (its 8 keys are 8 half + {0..3, 8..11} + 4 (lane / 32): V^T is read in that
-// order, transposed by ds_read_b64_tr_b16).  P is rounded to bf16 for the second product, as a bf16 model does; sums and maxima are f32.
-//
-// K / V tiles of 64 keys come by LDS-DMA into two buffers, the next tile in flight while this one is multiplied, one barrier a tile.
-// LDS rows are unpadded (the DMA writes 16 bytes a lane in a row), so the 16-byte chunks of key r are permuted on the source side: K chunk
-// c at c ^ (r % 16) (head_dim 64: c ^ (r / 2 % 8)), so that the 16 keys a ds_read_b128 reads at once lie in 16 different bank groups;
-// V chunks in groups of four, group g at g ^ (r % 4) (head_dim 64: g ^ (r / 2 % 2)), so that the four keys x 64 bytes of a transposed
-// read do.
-//
-// The running maximum is raised only when a tile's exceeds it by more than 2^8 in the exponential (a wave decides at once): p then stays
-// below 2^8, sums in f32 lose nothing by it, and the rescaling of the 4 x 16 accumulators is skipped for almost every tile.
-template <int HD, int NW, int KT, int MODE>
-__global__ __launch_bounds__(NW * 64, 2) void k_attn_rows(const RowsParams p)
+// The keys of a tile in LDS.  Rows are unpadded (the DMA writes 16 bytes a lane in a row), so the 16-byte chunks of key r are permuted on
+// the source side: K chunk c at c ^ (r % 16) (head_dim 64: c ^ (r / 2 % 8)), so that the 16 keys a ds_read_b128 reads at once lie in 16
+// different bank groups; V chunks in groups of four, group g at g ^ (r % 4) (head_dim 64: g ^ (r / 2 % 2)), so that the four keys x 64
+// bytes of a transposed read do.
+template <int HD> __device__ __forceinline__ int kperm(int r) { return HD == 128 ? r & 15 : (r >> 1) & 7; }
+template <int HD> __device__ __forceinline__ int vperm(int r) { return HD == 128 ? (r & 3) << 2 : ((r >> 1) & 1) << 2; }
+
+// A wave's 32 rows: S^T = K Q^T and O^T = V^T P^T with the 32 x 32 x 16 MFMA.  A lane holds one row's scores of 16 of every 32 keys, so the
+// softmax of a row is lane-local up to one exchange with lane ^ 32, and P goes from the accumulators of the first product into the operand
+// of the second without leaving the lane (its 8 keys are 8 half + {0..3, 8..11} + 4 (lane / 32): V^T is read in that order, transposed by
+// ds_read_b64_tr_b16).  P is rounded to bf16 for the second product, as a bf16 model does; sums and maxima are f32.
+template <int HD>
+struct WaveRows {
+    static constexpr int NS = HD / 16, ND = HD / 32, ROWB = HD * 2;
+    bf16x8_t qf[NS];
+    f32x16 o[ND];
+    float m, l;                      // running maximum (of unscaled scores; every lane of a row) and sum (this lane's keys)
+    float c1, raise;
+    unsigned ka[NS], va[ND];         // LDS offsets of this lane's fragments in a tile
+
+    __device__ __forceinline__ void init(float scale, int lane)
+    {
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) o[d][e] = 0.0f;
+        m = -1e30f;
+        l = 0.0f;
+        c1 = scale * 1.4426950408889634f;
+        raise = 8.0f / c1;
+        const int l32 = lane & 31, h2 = lane >> 5;
+#pragma unroll
+        for (int d = 0; d < NS; d++) ka[d] = (unsigned)(l32 * ROWB + ((2 * d + h2) ^ kperm<HD>(l32)) * 16);
+        // lane i of a 16-lane group hands in key i / 4, columns 4 (i % 4) .. + 3 of a 4-key x 16-dim block and gets column i
+        const int key = 4 * h2 + ((lane & 15) >> 2), c = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+#pragma unroll
+        for (int d = 0; d < ND; d++) va[d] = (unsigned)(key * ROWB + ((4 * d + c) ^ vperm<HD>(key)) * 16 + (lane & 1) * 8);
+    }
+    __device__ __forceinline__ void load_q(const uint16_t *q, int h2)
+    {
+#pragma unroll
+        for (int s = 0; s < NS; s++) qf[s] = __builtin_bit_cast(bf16x8_t, *reinterpret_cast<const uint4 *>(q + 16 * s + 8 * h2));
+        // (waited for here: left to hipcc the wait falls behind the next tile's DMA)
+#pragma unroll
+        for (int s = 0; s < NS; s++) asm volatile("" : : "v"(qf[s]));
+    }
+    // scores of NC x 32 keys at K tile kt
+    template <int NC> __device__ __forceinline__ void scores(const unsigned char *kt, f32x16 (&s)[NC])
+    {
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+            s[c] = (f32x16){0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int d = 0; d < NS; d++) {
+                const bf16x8_t kf = *reinterpret_cast<const bf16x8_t *>(kt + ka[d] + c * 32 * ROWB);
+                s[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[d], s[c], 0, 0, 0);
+            }
+        }
+    }
+    // scores -> unnormalised probabilities; rel: keys of the tile this lane's row sees, minus 4 (lane / 32).
+    // The running maximum is raised only when a tile's exceeds it by more than 2^8 in the exponential (a wave decides at once): p then
+    // stays below 2^8, sums in f32 lose nothing by it, and the rescaling of the accumulators is skipped for almost every tile.
+    template <int NC> __device__ __forceinline__ void softmax(f32x16 (&s)[NC], bool mask, int rel)
+    {
+        // the maxima below are asm (fmaxf on MFMA results costs a canonicalising v_max each), for which hipcc inserts no wait states:
+        // 20 here, one more than a 16-pass MFMA's result needs
+        if (NC == 2) asm volatile("s_nop 15\n\ts_nop 3" : "+v"(s[0]), "+v"(s[NC - 1]));
+        else asm volatile("s_nop 15\n\ts_nop 3" : "+v"(s[0]));
+        if (mask) {
+#pragma unroll
+            for (int c = 0; c < NC; c++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) s[c][e] = c * 32 + 8 * (e >> 2) + (e & 3) < rel ? s[c][e] : -INFINITY;
+        }
+        float mloc = s[0][0];
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) asm("v_max3_f32 %0, %0, %1, %2" : "+v"(mloc) : "v"(s[c][e]), "v"(s[c][e + 1]));
+        mloc = max_half(mloc);
+        if (__any(mloc > m + raise)) {
+            const float mnew = fmaxf(m, mloc), alpha = __builtin_amdgcn_exp2f((m - mnew) * c1);
+            m = mnew;
+            l *= alpha;
+#pragma unroll
+            for (int d = 0; d < ND; d++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) o[d][e] *= alpha;
+        }
+        const float ms = m * c1;
+        float ls[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                s[c][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c][e], c1, -ms));
+                ls[e & 3] += s[c][e];
+            }
+        l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+    }
+    // O^T += V^T P^T, V tile vt
+    template <int NC> __device__ __forceinline__ void accumulate(const unsigned char *vt, const f32x16 (&s)[NC])
+    {
+#pragma unroll
+        for (int kk = 0; kk < 2 * NC; kk++) {
+            const int c = kk >> 1, e0 = (kk & 1) * 8;
+            uint4 pb;
+            pb.x = f32x2_to_bf16x2(s[c][e0], s[c][e0 + 1]);
+            pb.y = f32x2_to_bf16x2(s[c][e0 + 2], s[c][e0 + 3]);
+            pb.z = f32x2_to_bf16x2(s[c][e0 + 4], s[c][e0 + 5]);
+            pb.w = f32x2_to_bf16x2(s[c][e0 + 6], s[c][e0 + 7]);
+            const bf16x8_t pf = __builtin_bit_cast(bf16x8_t, pb);
+#pragma unroll
+            for (int d = 0; d < ND; d++) {
+                typedef __attribute__((address_space(3))) bf16x4_t *lds4;
+                const bf16x4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(vt + va[d] + kk * 16 * ROWB));
+                const bf16x4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(vt + va[d] + (kk * 16 + 8) * ROWB));
+                const bf16x8_t vf = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf, o[d], 0, 0, 0);
+            }
+        }
+    }
+};
+
+// Four waves.  Two forms of a workgroup, by KeySet::narrow:
+//   wide    128 rows, a wave 32 of them.  K / V tiles of 64 keys come by LDS-DMA into two buffers, the next tile in flight while this one is
+//           multiplied, one barrier a tile.
+//   narrow  32 rows, shared by the waves: a wave takes every fourth tile of 32 keys, by itself (its own K and V buffer, the next K in flight
+//           from the end of the first product on, no barrier), and the four results are joined in LDS.  For the few rows of a decode step,
+//           whose work is bringing the keys: 128 rows would leave three waves idle.
+// LONG: every workgroup is wide and its rows packed (known to hipcc: 4 % on a long prompt over the kernel that decides at run time)
+template <int HD, bool LONG>
+__global__ __launch_bounds__(256, 2) void k_attn_rows(const RowsParams p)
 {
-    constexpr int NS = HD / 16, ND = HD / 32, NC = KT / 32, R = NW * 32, ROWB = HD * 2, TILE = KT * ROWB, BUF = 2 * TILE;
+    constexpr int ROWB = HD * 2, ND = HD / 32;
     constexpr int CH = HD / 8, PK = 1024 / ROWB;               // chunks of a key, keys of a DMA instruction
-    constexpr int PIECES = TILE / 1024 / NW;                   // DMA instructions a wave issues for K, and for V, of a tile
-    __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * BUF];
+    constexpr int WTILE = kWideKeys * ROWB, NTILE = kNarrowKeys * ROWB;
+    constexpr int JROW = HD * 4 + 16, JWAVE = 32 * JROW;        // narrow: a wave's result in LDS, rows padded by one chunk
+    constexpr int BYTES = 4 * WTILE > 4 * JWAVE + 1024 ? 4 * WTILE : 4 * JWAVE + 1024;
+    __shared__ __attribute__((aligned(1024))) unsigned char lds[BYTES];
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l32 = lane & 31, h2 = lane >> 5;
-    const KeySet &ks = p.ks;
+    const bool second = !LONG && (int)blockIdx.x >= p.first;
+    const KeySet &ks = p.ks[second ? 1 : 0];
+    const bool narrow = !LONG && ks.narrow;
+    const int mode = LONG ? ROWS_PACKED : ks.mode, id = blockIdx.x - (second ? p.first : 0);
     // kv head, row block, part: neighbours on different XCDs, so that with 2, 4 or 8 kv heads an XCD's L2 holds its own heads' keys
-    const int G = p.G, kvh = blockIdx.x % p.nkv, bp = blockIdx.x / p.nkv, part = bp / ks.blocks;
+    const int G = p.G, kvh = id % p.nkv, bp = id / p.nkv, part = bp / ks.blocks;
+    const int rs = narrow ? 5 : 7, R = 1 << rs, KT = narrow ? kNarrowKeys : kWideKeys;       // rows of a block, keys of a tile
+    static_assert(kNarrowRows == 32 && kWideRows == 128, "");
     int xb = bp - part * ks.blocks;
 
     // the block's sequence: tokens [n0, n1), first row of the block within it, its cache row and the keys it may read
     int n0, n1, row0, kbatch, klen;
-    if (MODE == ROWS_PACKED) {
+    if (mode == ROWS_PACKED) {
         // sequence s owns the block slots floor(cu[s] G / R) + s .. : at least ceil(len G / R) of them, so no table of blocks is needed;
         // the last blocks of a long prompt see the most keys and start first.  The lanes probe 64 sequences at a time (one round trip up
         // to 64 sequences, two up to 4096).
@@ -151,7 +280,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_rows(const RowsParams p)
         int lo = 0, range = p.nseqs;
         while (range > 1) {
             const int step = (range + 63) >> 6, at = lo + lane * step;
-            const bool le = lane * step < range && (int)((int64_t)p.cu[at] * G / R) + at <= xb;
+            const bool le = lane * step < range && (int)(((int64_t)p.cu[at] * G) >> rs) + at <= xb;
             const int cnt = __popcll(__ballot(le));
             const int first = (cnt > 0 ? cnt - 1 : 0) * step;
             lo += first;
@@ -160,12 +289,12 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_rows(const RowsParams p)
         lo = __builtin_amdgcn_readfirstlane(lo);
         n0 = min(max(p.cu[lo], 0), p.ntokens);
         n1 = min(max(p.cu[lo + 1], n0), p.ntokens);
-        const int blk = xb - ((int)((int64_t)n0 * G / R) + lo);
+        const int blk = xb - ((int)(((int64_t)n0 * G) >> rs) + lo);
         if (blk < 0 || (int64_t)blk * R >= (int64_t)(n1 - n0) * G) return;
         row0 = blk * R;
         kbatch = lo;
         klen = min(max(ks.lim[lo], 0), ks.max_keys);
-    } else if (MODE == ROWS_PREFIX) {
+    } else if (mode == ROWS_PREFIX) {
         n0 = 0;
         n1 = p.ntokens;
         row0 = xb * R;
@@ -179,20 +308,18 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_rows(const RowsParams p)
         row0 = (xb - kbatch * blocks) * R;
         klen = ks.max_keys;
     }
-    const int n = n1 - n0, row = row0 + wid * 32 + l32, t = row / G, g = row - t * G;
+    const int n = n1 - n0, w0 = row0 + (narrow ? 0 : wid * 32), row = w0 + l32, t = row / G, g = row - t * G;
     const bool ok = t < n;
     const int tok = n0 + (ok ? t : 0), head = kvh * G + (ok ? g : 0);
     int lim, wmax, wmin, kmax;                                 // keys this lane's row sees; most and fewest of the wave's rows; most of the block's
-    if (MODE == ROWS_PACKED) {
-        const int w0 = row0 + wid * 32, past = klen - n + 1;
+    if (mode == ROWS_PACKED) {
+        const int past = klen - n + 1;
         lim = ok ? max(past + t, 0) : 0;
         wmax = w0 / G < n ? max(past + min((w0 + 31) / G, n - 1), 0) : 0;
         wmin = max(past + min(w0 / G, n - 1), 0);
         kmax = max(past + min((row0 + R - 1) / G, n - 1), 0);
-        wmax = __builtin_amdgcn_readfirstlane(wmax);
-        wmin = __builtin_amdgcn_readfirstlane(wmin);
     } else {
-        lim = !ok ? 0 : !ks.lim ? klen : min(max(ks.lim[MODE == ROWS_PREFIX ? tok / p.T : tok], 0), klen);
+        lim = !ok ? 0 : !ks.lim ? klen : min(max(ks.lim[mode == ROWS_PREFIX ? tok / p.T : tok], 0), klen);
         wmax = lim;
         wmin = ok ? lim : klen;
 #pragma unroll
@@ -200,18 +327,17 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_rows(const RowsParams p)
             wmax = max(wmax, __shfl_xor(wmax, o, 64));
             wmin = min(wmin, __shfl_xor(wmin, o, 64));
         }
-        wmax = __builtin_amdgcn_readfirstlane(wmax);
-        wmin = __builtin_amdgcn_readfirstlane(wmin);
         kmax = wmax;
-        if (NW > 1) {
+        if (!narrow) {
             int *smax = reinterpret_cast<int *>(lds);
             if (lane == 0) smax[wid] = wmax;
             __syncthreads();
-#pragma unroll
-            for (int w = 0; w < NW; w++) kmax = max(kmax, smax[w]);
+            kmax = max(max(smax[0], smax[1]), max(smax[2], smax[3]));
             __syncthreads();
         }
     }
+    wmax = __builtin_amdgcn_readfirstlane(wmax);
+    wmin = __builtin_amdgcn_readfirstlane(wmin);
     kmax = __builtin_amdgcn_readfirstlane(kmax);
     int kt0 = 0, kt1 = (kmax + KT - 1) / KT;
     if (p.part_o) {
@@ -219,162 +345,168 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_rows(const RowsParams p)
         kt1 = min(kt1, kt0 + ks.part_tiles);
     }
 
-    f32x16 o[ND];
-#pragma unroll
-    for (int d = 0; d < ND; d++)
-#pragma unroll
-        for (int e = 0; e < 16; e++) o[d][e] = 0.0f;
-    float mrun = -1e30f, lrun = 0.0f;
-    const float c1 = p.scale * 1.4426950408889634f, raise = 8.0f / c1;
-
-    // DMA: piece j of wave w brings keys (j NW + w) PK .. + PK - 1 of the tile; lane l -> key l / CH of the piece, LDS chunk l % CH
+    WaveRows<HD> w;
+    w.init(p.scale, lane);
+    const uint16_t *qrow = p.q + (int64_t)tok * p.q_ts + (int64_t)head * HD;
     const unsigned lbase = (unsigned)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)lds);
     const unsigned ts2 = (unsigned)ks.ts * 2u;
-    const unsigned char *kbase0 = reinterpret_cast<const unsigned char *>(ks.kv + (int64_t)kbatch * ks.bs + (int64_t)kvh * HD);
-    const int64_t voff = (int64_t)p.v_off * 2;
-    const int drow = wid * PK + lane / CH, dpos = lane % CH;
-    const unsigned kch = (unsigned)(HD == 128 ? dpos ^ (drow & 15) : dpos ^ ((drow >> 1) & 7)) * 16u;
-    const unsigned vch = (unsigned)(HD == 128 ? dpos ^ ((drow & 3) << 2) : dpos ^ (((drow >> 1) & 1) << 2)) * 16u;
-    auto kchunk = [&](int j) { return kch ^ (unsigned)((HD == 128 ? (j * NW * PK) & 15 : ((j * NW * PK) >> 1) & 7) * 16); };
-    auto issue = [&](int kt) {
-        const unsigned dst = lbase + (unsigned)(kt & 1) * BUF + (unsigned)wid * 1024u;
-        const unsigned char *src = kbase0 + (int64_t)kt * KT * (int64_t)ts2;
-        const int left = kmax - 1 - kt * KT;                   // the last key of the block, relative to the tile
-        if (left >= KT - 1) {
-            const unsigned o0 = (unsigned)drow * ts2;
-#pragma unroll
-            for (int j = 0; j < PIECES; j++) {
-                const unsigned char *sj = src + (int64_t)(j * NW * PK) * (int64_t)ts2;
-                ROWS_DMA(o0 + kchunk(j), sj, dst + j * NW * 1024);
-                ROWS_DMA(o0 + vch, sj + voff, dst + TILE + j * NW * 1024);
-            }
-        } else {                                               // past the end: the last key again, masked below
-#pragma unroll
-            for (int j = 0; j < PIECES; j++) {
-                const unsigned o0 = (unsigned)min(drow + j * NW * PK, left) * ts2;
-                ROWS_DMA(o0 + kchunk(j), src, dst + j * NW * 1024);
-                ROWS_DMA(o0 + vch, src + voff, dst + TILE + j * NW * 1024);
-            }
-        }
-    };
-    unsigned ka[NS], va[ND];                                   // LDS offsets of this lane's fragments in buffer 0
-#pragma unroll
-    for (int d = 0; d < NS; d++) ka[d] = (unsigned)(l32 * ROWB + ((2 * d + h2) ^ (HD == 128 ? l32 & 15 : (l32 >> 1) & 7)) * 16);
-    {
-        // lane i of a 16-lane group hands in key i / 4, columns 4 (i % 4) .. + 3 of a 4-key x 16-dim block and gets column i
-        const int key = 4 * h2 + ((lane & 15) >> 2), c = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-#pragma unroll
-        for (int d = 0; d < ND; d++) va[d] = (unsigned)(TILE + key * ROWB + ((4 * d + c) ^ (HD == 128 ? (key & 3) << 2 : ((key >> 1) & 1) << 2)) * 16 + (lane & 1) * 8);
-    }
+    const unsigned char *ksrc = reinterpret_cast<const unsigned char *>(ks.kv + (int64_t)kbatch * ks.bs + (int64_t)kvh * HD);
+    const unsigned char *vsrc = ksrc + (int64_t)p.v_off * 2;
+    const int64_t pr = (int64_t)(ks.part0 + part) * p.part_rows;
 
-    if (kt0 < kt1) issue(kt0);
-    bf16x8_t qf[NS];
+    if (!narrow) {
+        // DMA: piece j of wave w brings keys (4 j + w) PK .. + PK - 1 of the tile (the permutation of a chunk is the same in every piece);
+        // lane l -> key l / CH of the piece, LDS chunk l % CH
+        constexpr int PIECES = WTILE / 4096;
+        const int drow = wid * PK + lane / CH, dpos = lane % CH;
+        const unsigned kch = (unsigned)(dpos ^ kperm<HD>(drow)) * 16u, vch = (unsigned)(dpos ^ vperm<HD>(drow)) * 16u;
+        auto issue = [&](int kt) {
+            const unsigned dst = lbase + (unsigned)(kt & 1) * (2 * WTILE) + (unsigned)wid * 1024u;
+            const int64_t off = (int64_t)kt * kWideKeys * (int64_t)ts2;
+            const int left = kmax - 1 - kt * kWideKeys;        // the last key of the block, relative to the tile
+            if (left >= kWideKeys - 1) {
+                const unsigned o0 = (unsigned)drow * ts2;
 #pragma unroll
-    for (int s = 0; s < NS; s++) {
-        const uint4 v = *reinterpret_cast<const uint4 *>(p.q + (int64_t)tok * p.q_ts + (int64_t)head * HD + 16 * s + 8 * h2);
-        qf[s] = __builtin_bit_cast(bf16x8_t, v);
-    }
-    // (the loads of q are waited for here, with the first tile: left to hipcc their wait falls behind the next tile's DMA)
+                for (int j = 0; j < PIECES; j++) {
+                    const int64_t oj = off + (int64_t)(j * 4 * PK) * (int64_t)ts2;
+                    ROWS_DMA(o0 + kch, ksrc + oj, dst + j * 4096);
+                    ROWS_DMA(o0 + vch, vsrc + oj, dst + WTILE + j * 4096);
+                }
+            } else {                                           // past the end: the last key again, masked below
 #pragma unroll
-    for (int s = 0; s < NS; s++) asm volatile("" : : "v"(qf[s]));
-    for (int kt = kt0; kt < kt1; kt++) {
-        const int kbase = kt * KT;
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();                                       // the tile has landed, and the other buffer is no longer read
-        if (kt + 1 < kt1) issue(kt + 1);
-        if (kbase >= wmax) continue;                           // (a wave's rows see nothing of this tile)
-        const unsigned char *buf = lds + (kt & 1) * BUF;
-        f32x16 s[NC];
-#pragma unroll
-        for (int c = 0; c < NC; c++) {
-            s[c] = (f32x16){0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int d = 0; d < NS; d++) {
-                const bf16x8_t kf = *reinterpret_cast<const bf16x8_t *>(buf + ka[d] + c * 32 * ROWB);
-                s[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[d], s[c], 0, 0, 0);
+                for (int j = 0; j < PIECES; j++) {
+                    const unsigned o0 = (unsigned)min(drow + j * 4 * PK, left) * ts2;
+                    ROWS_DMA(o0 + kch, ksrc + off, dst + j * 4096);
+                    ROWS_DMA(o0 + vch, vsrc + off, dst + WTILE + j * 4096);
+                }
             }
+        };
+        if (kt0 < kt1) issue(kt0);
+        w.load_q(qrow, h2);
+        for (int kt = kt0; kt < kt1; kt++) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();                                   // the tile has landed, and the other buffer is no longer read
+            if (kt + 1 < kt1) issue(kt + 1);
+            const int kbase = kt * kWideKeys;
+            if (kbase >= wmax) continue;                       // (a wave's rows see nothing of this tile)
+            const unsigned char *buf = lds + (kt & 1) * (2 * WTILE);
+            f32x16 s[2];
+            w.scores(buf, s);
+            w.softmax(s, kbase + kWideKeys > wmin, lim - kbase - 4 * h2);
+            w.accumulate(buf + WTILE, s);
         }
-        // the maxima below are asm (fmaxf on MFMA results costs a canonicalising v_max each), for which hipcc inserts no wait states:
-        // 20 here, one more than a 16-pass MFMA's result needs
-        if (NC == 2) asm volatile("s_nop 15\n\ts_nop 3" : "+v"(s[0]), "+v"(s[NC - 1]));
-        else asm volatile("s_nop 15\n\ts_nop 3" : "+v"(s[0]));
-        if (kbase + KT > wmin) {
-            const int rel = lim - kbase - 4 * h2;
-#pragma unroll
-            for (int c = 0; c < NC; c++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) s[c][e] = c * 32 + 8 * (e >> 2) + (e & 3) < rel ? s[c][e] : -INFINITY;
-        }
-        float mloc = s[0][0];
-#pragma unroll
-        for (int c = 0; c < NC; c++)
-#pragma unroll
-            for (int e = 0; e < 16; e += 2) asm("v_max3_f32 %0, %0, %1, %2" : "+v"(mloc) : "v"(s[c][e]), "v"(s[c][e + 1]));
-        mloc = max_half(mloc);
-        if (__any(mloc > mrun + raise)) {
-            const float mnew = fmaxf(mrun, mloc), alpha = __builtin_amdgcn_exp2f((mrun - mnew) * c1);
-            mrun = mnew;
-            lrun *= alpha;
+        w.l += __shfl_xor(w.l, 32, 64);
+        const int64_t at = pr + (int64_t)tok * p.nh + head;
+        if (p.part_o) {
+            if (!ok) return;
+            if (h2 == 0) *reinterpret_cast<float2 *>(p.part_ml + at * 2) = make_float2(w.m, w.l);
+            float *po = p.part_o + at * HD + 4 * h2;
 #pragma unroll
             for (int d = 0; d < ND; d++)
 #pragma unroll
-                for (int e = 0; e < 16; e++) o[d][e] *= alpha;
+                for (int e = 0; e < 16; e += 4)
+                    *reinterpret_cast<float4 *>(po + 32 * d + 2 * e) = make_float4(w.o[d][e], w.o[d][e + 1], w.o[d][e + 2], w.o[d][e + 3]);
+            return;
         }
-        const float ms = mrun * c1;
-        float ls[4] = {0.f, 0.f, 0.f, 0.f};
+        // A lane holds dims 8 i + 4 (lane / 32) .. + 3 of its row: halves of neighbouring groups of eight are exchanged with lane ^ 32, so
+        // that a lane stores whole groups (16 bytes of bf16) and a row's two lanes 32 bytes in a row.
+        const float inv = w.l > 0.0f ? 1.0f / w.l : 0.0f;
+        uint16_t *op = p.out + (int64_t)tok * p.o_ts + (int64_t)head * HD + 8 * h2;
 #pragma unroll
-        for (int c = 0; c < NC; c++)
+        for (int d = 0; d < ND; d++)
 #pragma unroll
-            for (int e = 0; e < 16; e++) {
-                s[c][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c][e], c1, -ms));
-                ls[e & 3] += s[c][e];
+            for (int e = 0; e < 16; e += 8) {
+                typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+                const u32x2 x = __builtin_amdgcn_permlane32_swap(f32x2_to_bf16x2(w.o[d][e] * inv, w.o[d][e + 1] * inv),
+                                                                 f32x2_to_bf16x2(w.o[d][e + 4] * inv, w.o[d][e + 5] * inv), false, false);
+                const u32x2 y = __builtin_amdgcn_permlane32_swap(f32x2_to_bf16x2(w.o[d][e + 2] * inv, w.o[d][e + 3] * inv),
+                                                                 f32x2_to_bf16x2(w.o[d][e + 6] * inv, w.o[d][e + 7] * inv), false, false);
+                if (ok) *reinterpret_cast<uint4 *>(op + 32 * d + 2 * e) = make_uint4(x.x, y.x, x.y, y.y);
             }
-        lrun += (ls[0] + ls[1]) + (ls[2] + ls[3]);
-#pragma unroll
-        for (int kk = 0; kk < 2 * NC; kk++) {
-            const int c = kk >> 1, e0 = (kk & 1) * 8;
-            uint4 pb;
-            pb.x = f32x2_to_bf16x2(s[c][e0], s[c][e0 + 1]);
-            pb.y = f32x2_to_bf16x2(s[c][e0 + 2], s[c][e0 + 3]);
-            pb.z = f32x2_to_bf16x2(s[c][e0 + 4], s[c][e0 + 5]);
-            pb.w = f32x2_to_bf16x2(s[c][e0 + 6], s[c][e0 + 7]);
-            const bf16x8_t pf = __builtin_bit_cast(bf16x8_t, pb);
-#pragma unroll
-            for (int d = 0; d < ND; d++) {
-                typedef __attribute__((address_space(3))) bf16x4_t *lds4;
-                const bf16x4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(buf + va[d] + kk * 16 * ROWB));
-                const bf16x4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(buf + va[d] + (kk * 16 + 8) * ROWB));
-                const bf16x8_t vf = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf, o[d], 0, 0, 0);
-            }
-        }
+        return;
     }
-    lrun += __shfl_xor(lrun, 32, 64);
-    const float inv = p.part_o ? 1.0f : lrun > 0.0f ? 1.0f / lrun : 0.0f;
-    const int64_t pr = (int64_t)(ks.part0 + part) * p.part_rows + (int64_t)tok * p.nh + head;
-    if (p.part_o && ok && h2 == 0) *reinterpret_cast<float2 *>(p.part_ml + pr * 2) = make_float2(mrun, lrun);
-    // A lane holds dims 8 i + 4 (lane / 32) .. + 3 of its row: halves of neighbouring groups of eight are exchanged with lane ^ 32, so that
-    // a lane stores whole groups (16 bytes of bf16) and a row's two lanes 32 bytes in a row.
-    uint16_t *op = p.out + (int64_t)tok * p.o_ts + (int64_t)head * HD;
-    float *po = p.part_o + pr * HD;
+
+    // narrow: piece j brings keys j PK .. + PK - 1 of the wave's tile
+    constexpr int PIECES = NTILE / 1024;
+    const unsigned kdst = lbase + (unsigned)wid * (2 * NTILE), vdst = kdst + NTILE;
+    const int drow = lane / CH, dpos = lane % CH;
+    auto issue = [&](int kt, const unsigned char *src, unsigned dst, bool v) {
+        const int left = kmax - 1 - kt * kNarrowKeys;
+        src += (int64_t)kt * kNarrowKeys * (int64_t)ts2;
+#pragma unroll
+        for (int j = 0; j < PIECES; j++) {
+            const int r = drow + j * PK;
+            const unsigned c = (unsigned)(dpos ^ (v ? vperm<HD>(r) : kperm<HD>(r))) * 16u;
+            ROWS_DMA((unsigned)min(r, left) * ts2 + c, src, dst + j * 1024);
+        }
+    };
+    int kt = kt0 + wid;
+    if (kt < kt1) {
+        issue(kt, ksrc, kdst, false);
+        issue(kt, vsrc, vdst, true);
+    }
+    w.load_q(qrow, h2);
+    const unsigned char *kbuf = lds + wid * (2 * NTILE), *vbuf = kbuf + NTILE;
+    for (; kt < kt1; kt += 4) {
+        const bool more = kt + 4 < kt1;
+        const int kbase = kt * kNarrowKeys;
+        f32x16 s[1];
+        // (own DMA only, counted in order: K of this tile is behind V of this tile, which is behind K of the next)
+        if (PIECES == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+        else asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+        w.scores(kbuf, s);
+        asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(s[0]) : : "memory");       // the tile's keys have been read
+        if (more) issue(kt + 4, ksrc, kdst, false);
+        w.softmax(s, kbase + kNarrowKeys > wmin, lim - kbase - 4 * h2);
+        if (!more) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        else if (PIECES == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+        else asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+        w.accumulate(vbuf, s);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (more) issue(kt + 4, vsrc, vdst, true);
+    }
+    w.l += __shfl_xor(w.l, 32, 64);
+    __syncthreads();                                           // the tiles are no longer read
+    float *sml = reinterpret_cast<float *>(lds + 4 * JWAVE);
+    if (h2 == 0) *reinterpret_cast<float2 *>(sml + (wid * 32 + l32) * 2) = make_float2(w.m, w.l);
 #pragma unroll
     for (int d = 0; d < ND; d++)
 #pragma unroll
-        for (int e = 0; e < 16; e += 8) {
-            if (p.part_o) {
-                if (ok) {
-                    *reinterpret_cast<float4 *>(po + 32 * d + 2 * e + 4 * h2) = make_float4(o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]);
-                    *reinterpret_cast<float4 *>(po + 32 * d + 2 * e + 8 + 4 * h2) = make_float4(o[d][e + 4], o[d][e + 5], o[d][e + 6], o[d][e + 7]);
-                }
-            } else {
-                typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
-                const u32x2 x = __builtin_amdgcn_permlane32_swap(f32x2_to_bf16x2(o[d][e] * inv, o[d][e + 1] * inv),
-                                                                 f32x2_to_bf16x2(o[d][e + 4] * inv, o[d][e + 5] * inv), false, false);
-                const u32x2 y = __builtin_amdgcn_permlane32_swap(f32x2_to_bf16x2(o[d][e + 2] * inv, o[d][e + 3] * inv),
-                                                                 f32x2_to_bf16x2(o[d][e + 6] * inv, o[d][e + 7] * inv), false, false);
-                if (ok) *reinterpret_cast<uint4 *>(op + 32 * d + 2 * e + 8 * h2) = make_uint4(x.x, y.x, x.y, y.y);
-            }
+        for (int e = 0; e < 16; e += 4)
+            *reinterpret_cast<float4 *>(lds + wid * JWAVE + l32 * JROW + (32 * d + 2 * e + 4 * h2) * 4) =
+                make_float4(w.o[d][e], w.o[d][e + 1], w.o[d][e + 2], w.o[d][e + 3]);
+    __syncthreads();
+    // eight threads a row, each every eighth group of four dims
+    const int jr = tid >> 3, jt = (row0 + jr) / G, jg = row0 + jr - jt * G;
+    if (jt >= n) return;
+    float mj[4], wj[4], m = -1e30f, l = 0.0f;
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+        mj[u] = sml[(u * 32 + jr) * 2];
+        m = fmaxf(m, mj[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+        wj[u] = __builtin_amdgcn_exp2f((mj[u] - m) * w.c1);
+        l += sml[(u * 32 + jr) * 2 + 1] * wj[u];
+    }
+    const int jtok = n0 + jt, jhead = kvh * G + jg;
+    const int64_t at = pr + (int64_t)jtok * p.nh + jhead;
+    if (p.part_o && (tid & 7) == 0) *reinterpret_cast<float2 *>(p.part_ml + at * 2) = make_float2(m, l);
+    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+#pragma unroll
+    for (int d = (tid & 7) * 4; d < HD; d += 32) {
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const float4 v = *reinterpret_cast<const float4 *>(lds + u * JWAVE + jr * JROW + d * 4);
+            a.x += v.x * wj[u]; a.y += v.y * wj[u]; a.z += v.z * wj[u]; a.w += v.w * wj[u];
         }
+        if (p.part_o) *reinterpret_cast<float4 *>(p.part_o + at * HD + d) = a;
+        else
+            *reinterpret_cast<uint2 *>(p.out + (int64_t)jtok * p.o_ts + (int64_t)jhead * HD + d) =
+                make_uint2(f32x2_to_bf16x2(a.x * inv, a.y * inv), f32x2_to_bf16x2(a.z * inv, a.w * inv));
+    }
 }
 
 // out = sum_j o_j 2^((m_j - m) c1) / sum_j l_j 2^((m_j - m) c1); a row is HD / 4 lanes.  Lane j of a row reads part j's (max, sum), so
@@ -446,19 +578,18 @@ extern "C" int ifh_rope_append_packed_bf16(const ifh_rope_packed_desc *d, ifh_st
     return IFH_OK;
 }
 
-// Row blocks are 128 rows (four waves, 64-key tiles) or, where a sequence has no more than about 32 rows, 32 rows (one wave, 32-key tiles
-// and 32 KB of LDS, so that five workgroups of a CU keep loads in flight).
-struct Tiling {
-    int rows, keys, per_cu;
-};
-static Tiling tiling(int64_t rows_of_a_sequence) { return rows_of_a_sequence <= 40 ? Tiling{32, 32, 5} : Tiling{128, 64, 2}; }
-
-// parts of the keys and tiles per part, for `blocks` workgroups over max_keys keys: enough parts to fill the device, none of fewer than
-// min_keys keys
-static void split_keys(KeySet *k, const Tiling &t, int64_t workgroups, int min_keys)
+// Fills in a key set's split for sequences (rows of a batch) of seq_rows rows: narrow workgroups where a sequence has about a narrow
+// block's rows or fewer.  Keys are split into parts until the device has two workgroups a CU, none of fewer than two tiles a wave.
+static void plan_keys(KeySet *k, int mode, int64_t seq_rows, int64_t blocks_wide, int64_t blocks_narrow, int nkv, int max_keys)
 {
-    const int tiles = (k->max_keys + t.keys - 1) / t.keys, least = min_keys / t.keys;
-    const int64_t want = (int64_t)t.per_cu * device_cu_count_physical() / (workgroups > 0 ? workgroups : 1);
+    k->mode = mode;
+    k->narrow = seq_rows <= 40;
+    const int64_t blocks = k->narrow ? blocks_narrow : blocks_wide;
+    k->blocks = (int)blocks;
+    k->max_keys = max_keys;
+    const int keys = k->narrow ? kNarrowKeys : kWideKeys, least = k->narrow ? 8 : 2;
+    const int tiles = (max_keys + keys - 1) / keys;
+    const int64_t want = 2 * (int64_t)device_cu_count_physical() / (blocks * nkv > 0 ? blocks * nkv : 1);
     int parts = (int)(want < 1 ? 1 : want > 64 ? 64 : want);
     if (parts > tiles / least) parts = tiles / least > 1 ? tiles / least : 1;
     k->part_tiles = (tiles + parts - 1) / parts;
@@ -467,17 +598,14 @@ static void split_keys(KeySet *k, const Tiling &t, int64_t workgroups, int min_k
 
 static int64_t part_floats(int64_t rows, int parts, int hd) { return rows * parts * (hd + 2); }
 
-template <int MODE>
-static void rows_launch(const RowsParams &p, int hd, const Tiling &t, hipStream_t st)
+static void rows_launch(const RowsParams &p, int hd, int64_t workgroups, hipStream_t st)
 {
-    const dim3 grid((unsigned)((int64_t)p.ks.blocks * p.nkv * (p.part_o ? p.ks.parts : 1)));
-    if (t.rows == 32) {
-        if (hd == 128) hipLaunchKernelGGL((k_attn_rows<128, 1, 32, MODE>), grid, dim3(64), 0, st, p);
-        else hipLaunchKernelGGL((k_attn_rows<64, 1, 32, MODE>), grid, dim3(64), 0, st, p);
-    } else {
-        if (hd == 128) hipLaunchKernelGGL((k_attn_rows<128, 4, 64, MODE>), grid, dim3(256), 0, st, p);
-        else hipLaunchKernelGGL((k_attn_rows<64, 4, 64, MODE>), grid, dim3(256), 0, st, p);
-    }
+    const dim3 grid((unsigned)workgroups), block(256);
+    const bool lng = p.ks[0].mode == ROWS_PACKED && !p.ks[0].narrow;
+    if (hd == 128 && lng) hipLaunchKernelGGL((k_attn_rows<128, true>), grid, block, 0, st, p);
+    else if (hd == 128) hipLaunchKernelGGL((k_attn_rows<128, false>), grid, block, 0, st, p);
+    else if (lng) hipLaunchKernelGGL((k_attn_rows<64, true>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((k_attn_rows<64, false>), grid, block, 0, st, p);
 }
 
 static void join_launch(const RowsParams &p, int hd, int parts, hipStream_t st)
@@ -489,25 +617,22 @@ static void join_launch(const RowsParams &p, int hd, int parts, hipStream_t st)
     else hipLaunchKernelGGL(k_attn_join<64>, grid, dim3(256), 0, st, p.part_o, p.part_ml, rows, parts, c1, p.out, p.o_ts, p.nh);
 }
 
-// block slots of a packed launch (the rows' sizes are checked by the callers to fit an int)
-static int64_t packed_blocks(int64_t ntokens, int64_t nseqs, int G, const Tiling &t) { return ntokens * G / t.rows + nseqs; }
-
-static int64_t packed_plan(int64_t ntokens, int64_t nseqs, int G, int nkv, int max_keys, KeySet *k, Tiling *t)
+static void packed_plan(int64_t ntokens, int64_t nseqs, int G, int nkv, int max_keys, KeySet *k)
 {
-    *t = tiling((ntokens * G + nseqs - 1) / nseqs);
-    const int64_t blocks = packed_blocks(ntokens, nseqs, G, *t);
-    k->max_keys = max_keys;
-    k->blocks = (int)blocks;
-    split_keys(k, *t, blocks * nkv, 256);
-    return blocks;
+    plan_keys(k, ROWS_PACKED, (ntokens * G + nseqs - 1) / nseqs, ntokens * G / kWideRows + nseqs, ntokens * G / kNarrowRows + nseqs, nkv, max_keys);
+}
+
+// (the callers check that block counts fit an int)
+static bool packed_fits(int64_t ntokens, int64_t nseqs, int64_t nheads, int64_t nkv)
+{
+    return ntokens * (nheads / nkv) < (1ll << 30) && ntokens * nheads < (1ll << 33) && (ntokens * (nheads / nkv) / kNarrowRows + nseqs) * nkv < (1ll << 25);
 }
 
 extern "C" int64_t ifh_attn_packed_ws_floats(int ntokens, int nseqs, int nheads, int nkv, int head_dim, int max_keys)
 {
-    if (ntokens <= 0 || nseqs <= 0 || nkv <= 0 || nheads < nkv || nheads % nkv || max_keys <= 0) return 0;
+    if (ntokens <= 0 || nseqs <= 0 || nkv <= 0 || nheads < nkv || nheads % nkv || max_keys <= 0 || !packed_fits(ntokens, nseqs, nheads, nkv)) return 0;
     KeySet k = {};
-    Tiling t;
-    packed_plan(ntokens, nseqs, nheads / nkv, nkv, max_keys, &k, &t);
+    packed_plan(ntokens, nseqs, nheads / nkv, nkv, max_keys, &k);
     return k.parts > 1 ? part_floats((int64_t)ntokens * nheads, k.parts, head_dim) : 0;
 }
 
@@ -528,61 +653,56 @@ extern "C" int ifh_attn_packed_bf16(const ifh_attn_packed_desc *d, ifh_stream_t 
     if (d->ntokens == 0 || d->nseqs == 0) return IFH_OK;
     IFH_CHECK_ARG(d->q && d->cache && d->out && d->cu && d->key_len && d->max_keys >= 1 && d->max_keys <= (1 << 30));
     IFH_CHECK_HEADS(d);
-    const int G = d->nheads / d->nkv;
-    IFH_CHECK_ARG((int64_t)d->ntokens * G < (1ll << 30) && (int64_t)d->ntokens * d->nheads < (1ll << 33));
+    IFH_CHECK_ARG(packed_fits(d->ntokens, d->nseqs, d->nheads, d->nkv));
     RowsParams p = {};
-    Tiling t;
-    const int64_t blocks = packed_plan(d->ntokens, d->nseqs, G, d->nkv, d->max_keys, &p.ks, &t);
-    IFH_CHECK_ARG(blocks * d->nkv * p.ks.parts < (1ll << 31));
+    KeySet &k = p.ks[0];
+    p.G = d->nheads / d->nkv;
+    packed_plan(d->ntokens, d->nseqs, p.G, d->nkv, d->max_keys, &k);
+    k.kv = (const uint16_t *)d->cache; k.bs = d->cache_bs; k.ts = d->cache_ts; k.lim = d->key_len;
     p.q = (const uint16_t *)d->q; p.q_ts = d->q_ts; p.v_off = d->v_off;
     p.out = (uint16_t *)d->out; p.o_ts = d->o_ts;
     p.cu = d->cu;
-    p.ks.kv = (const uint16_t *)d->cache; p.ks.bs = d->cache_bs; p.ks.ts = d->cache_ts; p.ks.lim = d->key_len;
-    p.ntokens = d->ntokens; p.nseqs = d->nseqs; p.nh = d->nheads; p.nkv = d->nkv; p.G = G; p.T = 1;
+    p.ntokens = d->ntokens; p.nseqs = d->nseqs; p.nh = d->nheads; p.nkv = d->nkv; p.T = 1;
     p.scale = d->scale;
     p.part_rows = (int64_t)d->ntokens * d->nheads;
-    if (d->ws && p.ks.parts > 1) {
-        IFH_CHECK_ARG(d->ws_floats >= part_floats(p.part_rows, p.ks.parts, d->head_dim));
+    if (d->ws && k.parts > 1) {
+        IFH_CHECK_ARG(d->ws_floats >= part_floats(p.part_rows, k.parts, d->head_dim));
         p.part_o = d->ws;
-        p.part_ml = d->ws + p.part_rows * p.ks.parts * d->head_dim;
-    }
+        p.part_ml = d->ws + p.part_rows * k.parts * d->head_dim;
+    } else
+        k.parts = 1;
+    const int64_t wgs = (int64_t)k.blocks * p.nkv * k.parts;
+    p.first = (int)wgs;
     hipStream_t st = as_stream(stream);
-    rows_launch<ROWS_PACKED>(p, d->head_dim, t, st);
+    rows_launch(p, d->head_dim, wgs, st);
     IFH_LAUNCH_CHECK("attn_packed");
     if (p.part_o) {
-        join_launch(p, d->head_dim, p.ks.parts, st);
+        join_launch(p, d->head_dim, k.parts, st);
         IFH_LAUNCH_CHECK("attn_packed join");
     }
     return IFH_OK;
 }
 
-struct PrefixPlan {
-    KeySet prefix, own;
-    Tiling pt, ot;
-};
-
-static PrefixPlan prefix_plan(int64_t nrows, int64_t T, int prefix_keys, int nheads, int nkv, int max_keys)
+static bool prefix_fits(int64_t ntokens, int64_t nheads, int64_t nkv)
 {
-    PrefixPlan r = {};
-    const int64_t G = nheads / nkv;
-    r.pt = tiling(nrows * T * G);
-    r.ot = tiling(T * G);
-    r.prefix.max_keys = prefix_keys;
-    r.prefix.blocks = (int)((nrows * T * G + r.pt.rows - 1) / r.pt.rows);
-    split_keys(&r.prefix, r.pt, (int64_t)r.prefix.blocks * nkv, 256);
-    r.own.max_keys = max_keys;
-    r.own.blocks = (int)(nrows * ((T * G + r.ot.rows - 1) / r.ot.rows));
-    split_keys(&r.own, r.ot, (int64_t)r.own.blocks * nkv, 256);
-    r.own.part0 = r.prefix.parts;
-    return r;
+    return ntokens < (1 << 24) && ntokens * (nheads / nkv) < (1ll << 30) && (ntokens * (nheads / nkv) / kNarrowRows + ntokens + 1) * nkv < (1ll << 24);
+}
+
+static void prefix_plan(int64_t nrows, int64_t T, int prefix_keys, int nheads, int nkv, int max_keys, KeySet *prefix, KeySet *own)
+{
+    const int64_t r = T * (nheads / nkv), all = nrows * r;
+    plan_keys(prefix, ROWS_PREFIX, all, (all + kWideRows - 1) / kWideRows, (all + kNarrowRows - 1) / kNarrowRows, nkv, prefix_keys);
+    plan_keys(own, ROWS_OWN, r, nrows * ((r + kWideRows - 1) / kWideRows), nrows * ((r + kNarrowRows - 1) / kNarrowRows), nkv, max_keys);
+    own->part0 = prefix->parts;
 }
 
 extern "C" int64_t ifh_attn_prefix_ws_floats(int nrows, int tokens_per_row, int prefix_keys, int nheads, int nkv, int head_dim, int max_keys)
 {
     if (nrows <= 0 || tokens_per_row <= 0 || nkv <= 0 || nheads < nkv || nheads % nkv || prefix_keys <= 0 || max_keys <= 0) return 0;
-    if ((int64_t)nrows * tokens_per_row * (nheads / nkv) >= (1ll << 30)) return 0;
-    const PrefixPlan r = prefix_plan(nrows, tokens_per_row, prefix_keys, nheads, nkv, max_keys);
-    return part_floats((int64_t)nrows * tokens_per_row * nheads, r.prefix.parts + r.own.parts, head_dim);
+    if (!prefix_fits((int64_t)nrows * tokens_per_row, nheads, nkv)) return 0;
+    KeySet a = {}, b = {};
+    prefix_plan(nrows, tokens_per_row, prefix_keys, nheads, nkv, max_keys, &a, &b);
+    return part_floats((int64_t)nrows * tokens_per_row * nheads, a.parts + b.parts, head_dim);
 }
 
 extern "C" int ifh_attn_prefix_bf16(const ifh_attn_prefix_desc *d, ifh_stream_t stream)
@@ -595,31 +715,26 @@ extern "C" int ifh_attn_prefix_bf16(const ifh_attn_prefix_desc *d, ifh_stream_t 
     IFH_CHECK_ARG((((uintptr_t)d->prefix) & 15) == 0 && d->prefix_ts % 8 == 0 && d->prefix_ts < (1 << 24) &&
                   d->prefix_ts >= (int64_t)d->v_off + (int64_t)d->nkv * d->head_dim);
     const int64_t ntokens = (int64_t)d->nrows * d->tokens_per_row;
-    IFH_CHECK_ARG(ntokens < (1 << 24));
-    const int G = d->nheads / d->nkv;
-    IFH_CHECK_ARG(ntokens * G < (1ll << 30) && ntokens * d->nheads < (1ll << 33));
-    const PrefixPlan r = prefix_plan(d->nrows, d->tokens_per_row, d->prefix_keys, d->nheads, d->nkv, d->max_keys);
-    IFH_CHECK_ARG((int64_t)r.prefix.blocks * d->nkv * r.prefix.parts < (1ll << 31) && (int64_t)r.own.blocks * d->nkv * r.own.parts < (1ll << 31));
+    IFH_CHECK_ARG(prefix_fits(ntokens, d->nheads, d->nkv));
     RowsParams p = {};
-    p.q = (const uint16_t *)d->q; p.q_ts = d->q_ts;
-    p.v_off = d->v_off;
+    KeySet &a = p.ks[0], &b = p.ks[1];
+    prefix_plan(d->nrows, d->tokens_per_row, d->prefix_keys, d->nheads, d->nkv, d->max_keys, &a, &b);
+    a.kv = (const uint16_t *)d->prefix; a.ts = d->prefix_ts; a.lim = d->prefix_len;
+    b.kv = (const uint16_t *)d->cache; b.bs = d->cache_bs; b.ts = d->cache_ts; b.lim = d->key_len;
+    p.q = (const uint16_t *)d->q; p.q_ts = d->q_ts; p.v_off = d->v_off;
     p.out = (uint16_t *)d->out; p.o_ts = d->o_ts;
-    p.ntokens = (int)ntokens; p.nseqs = d->nrows; p.nh = d->nheads; p.nkv = d->nkv; p.G = G; p.T = d->tokens_per_row;
+    p.ntokens = (int)ntokens; p.nseqs = d->nrows; p.nh = d->nheads; p.nkv = d->nkv; p.G = d->nheads / d->nkv; p.T = d->tokens_per_row;
     p.scale = d->scale;
     p.part_rows = ntokens * d->nheads;
-    const int parts = r.prefix.parts + r.own.parts;
+    const int parts = a.parts + b.parts;
     IFH_CHECK_ARG(d->ws_floats >= part_floats(p.part_rows, parts, d->head_dim));
     p.part_o = d->ws;
     p.part_ml = d->ws + p.part_rows * parts * d->head_dim;
+    const int64_t na = (int64_t)a.blocks * p.nkv * a.parts, nb = (int64_t)b.blocks * p.nkv * b.parts;
+    p.first = (int)na;
     hipStream_t st = as_stream(stream);
-    p.ks = r.prefix;
-    p.ks.kv = (const uint16_t *)d->prefix; p.ks.ts = d->prefix_ts; p.ks.lim = d->prefix_len;
-    rows_launch<ROWS_PREFIX>(p, d->head_dim, r.pt, st);
-    IFH_LAUNCH_CHECK("attn_prefix prefix");
-    p.ks = r.own;
-    p.ks.kv = (const uint16_t *)d->cache; p.ks.bs = d->cache_bs; p.ks.ts = d->cache_ts; p.ks.lim = d->key_len;
-    rows_launch<ROWS_OWN>(p, d->head_dim, r.ot, st);
-    IFH_LAUNCH_CHECK("attn_prefix own");
+    rows_launch(p, d->head_dim, na + nb, st);
+    IFH_LAUNCH_CHECK("attn_prefix");
     join_launch(p, d->head_dim, parts, st);
     IFH_LAUNCH_CHECK("attn_prefix join");
     return IFH_OK;
