@@ -134,8 +134,8 @@ struct WaveRows {
     static constexpr int NS = HD / 16, ND = HD / 32, ROWB = HD * 2;
     bf16x8_t qf[NS];
     f32x16 o[ND];
-    float m, l;                      // running maximum (of unscaled scores; every lane of a row) and sum (this lane's keys)
-    float c1, raise;
+    float ms, l;                     // about the running maximum, in the exponent (every lane of a row), and the sum (this lane's keys)
+    float c1;                        // scale log2 e
     unsigned ka[NS], va[ND];         // LDS offsets of this lane's fragments in a tile
 
     __device__ __forceinline__ void init(float scale, int lane)
@@ -144,10 +144,9 @@ struct WaveRows {
         for (int d = 0; d < ND; d++)
 #pragma unroll
             for (int e = 0; e < 16; e++) o[d][e] = 0.0f;
-        m = -1e30f;
+        ms = 0.0f;
         l = 0.0f;
         c1 = scale * 1.4426950408889634f;
-        raise = 8.0f / c1;
         const int l32 = lane & 31, h2 = lane >> 5;
 #pragma unroll
         for (int d = 0; d < NS; d++) ka[d] = (unsigned)(l32 * ROWB + ((2 * d + h2) ^ kperm<HD>(l32)) * 16);
@@ -177,46 +176,61 @@ struct WaveRows {
             }
         }
     }
-    // scores -> unnormalised probabilities; rel: keys of the tile this lane's row sees, minus 4 (lane / 32).
-    // The running maximum is raised only when a tile's exceeds it by more than 2^8 in the exponential (a wave decides at once): p then
-    // stays below 2^8, sums in f32 lose nothing by it, and the rescaling of the accumulators is skipped for almost every tile.
-    template <int NC> __device__ __forceinline__ void softmax(f32x16 (&s)[NC], bool mask, int rel)
+    // scores -> unnormalised probabilities 2^(s c1 - ms); rel: keys of the tile this lane's row sees, minus 4 (lane / 32); first: the rows'
+    // first tile.  ms starts as the first tile's maximum (what a row sees is keys 0 .. lim - 1, so a row that sees anything of a range sees
+    // its first key) and is raised only when a later tile exceeds it by more than 8 (a wave decides at once): p stays below 2^8, sums in
+    // f32 lose nothing by it, and the rescaling of the accumulators is skipped for almost every tile.
+    template <int NC> __device__ __forceinline__ void softmax(f32x16 (&s)[NC], bool mask, int rel, bool first)
     {
-        // the maxima below are asm (fmaxf on MFMA results costs a canonicalising v_max each), for which hipcc inserts no wait states:
-        // 20 here, one more than a 16-pass MFMA's result needs
-        if (NC == 2) asm volatile("s_nop 15\n\ts_nop 3" : "+v"(s[0]), "+v"(s[NC - 1]));
-        else asm volatile("s_nop 15\n\ts_nop 3" : "+v"(s[0]));
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) s[c][e] = __builtin_fmaf(s[c][e], c1, -ms);
         if (mask) {
 #pragma unroll
             for (int c = 0; c < NC; c++)
 #pragma unroll
                 for (int e = 0; e < 16; e++) s[c][e] = c * 32 + 8 * (e >> 2) + (e & 3) < rel ? s[c][e] : -INFINITY;
         }
-        float mloc = s[0][0];
+        // (two chains: a maximum of three waits for the one before it)
+        float mx = fmaxf(s[0][0], s[0][1]), my = fmaxf(s[0][2], s[0][3]);
 #pragma unroll
         for (int c = 0; c < NC; c++)
 #pragma unroll
-            for (int e = 0; e < 16; e += 2) asm("v_max3_f32 %0, %0, %1, %2" : "+v"(mloc) : "v"(s[c][e]), "v"(s[c][e + 1]));
-        mloc = max_half(mloc);
-        if (__any(mloc > m + raise)) {
-            const float mnew = fmaxf(m, mloc), alpha = __builtin_amdgcn_exp2f((m - mnew) * c1);
-            m = mnew;
+            for (int e = c == 0 ? 4 : 0; e < 16; e += 4) {
+                mx = fmaxf(fmaxf(mx, s[c][e]), s[c][e + 1]);
+                my = fmaxf(fmaxf(my, s[c][e + 2]), s[c][e + 3]);
+            }
+        mx = max_half(fmaxf(mx, my));
+        if (first || __any(mx > 8.0f)) {
+            const float raise = first ? (mx > -1e30f ? mx : 0.0f) : fmaxf(mx, 0.0f);
+            const float alpha = first ? 1.0f : __builtin_amdgcn_exp2f(-raise);
+            ms += raise;
             l *= alpha;
 #pragma unroll
             for (int d = 0; d < ND; d++)
 #pragma unroll
                 for (int e = 0; e < 16; e++) o[d][e] *= alpha;
+#pragma unroll
+            for (int c = 0; c < NC; c++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) s[c][e] -= raise;
         }
-        const float ms = m * c1;
         float ls[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < NC; c++)
 #pragma unroll
             for (int e = 0; e < 16; e++) {
-                s[c][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c][e], c1, -ms));
+                s[c][e] = __builtin_amdgcn_exp2f(s[c][e]);
                 ls[e & 3] += s[c][e];
             }
         l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+    }
+    // the sum over both lanes of a row; a row that saw nothing counts for nothing in a join
+    __device__ __forceinline__ void finish()
+    {
+        l += __shfl_xor(l, 32, 64);
+        ms = l > 0.0f ? ms : -1e30f;
     }
     // O^T += V^T P^T, V tile vt
     template <int NC> __device__ __forceinline__ void accumulate(const unsigned char *vt, const f32x16 (&s)[NC])
@@ -356,50 +370,69 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(const RowsParams p)
 
     if (!narrow) {
         // DMA: piece j of wave w brings keys (4 j + w) PK .. + PK - 1 of the tile (the permutation of a chunk is the same in every piece);
-        // lane l -> key l / CH of the piece, LDS chunk l % CH
+        // lane l -> key l / CH of the piece, LDS chunk l % CH.  All of a tile in one asm block: LDS addresses step through m0 4 KB at a time.
         constexpr int PIECES = WTILE / 4096;
         const int drow = wid * PK + lane / CH, dpos = lane % CH;
         const unsigned kch = (unsigned)(dpos ^ kperm<HD>(drow)) * 16u, vch = (unsigned)(dpos ^ vperm<HD>(drow)) * 16u;
+        unsigned ro[PIECES];
+#pragma unroll
+        for (int j = 0; j < PIECES; j++) ro[j] = (unsigned)(drow + j * 4 * PK) * ts2;
         auto issue = [&](int kt) {
             const unsigned dst = lbase + (unsigned)(kt & 1) * (2 * WTILE) + (unsigned)wid * 1024u;
             const int64_t off = (int64_t)kt * kWideKeys * (int64_t)ts2;
             const int left = kmax - 1 - kt * kWideKeys;        // the last key of the block, relative to the tile
+            unsigned r[PIECES], keep;
             if (left >= kWideKeys - 1) {
-                const unsigned o0 = (unsigned)drow * ts2;
 #pragma unroll
-                for (int j = 0; j < PIECES; j++) {
-                    const int64_t oj = off + (int64_t)(j * 4 * PK) * (int64_t)ts2;
-                    ROWS_DMA(o0 + kch, ksrc + oj, dst + j * 4096);
-                    ROWS_DMA(o0 + vch, vsrc + oj, dst + WTILE + j * 4096);
-                }
+                for (int j = 0; j < PIECES; j++) r[j] = ro[j];
             } else {                                           // past the end: the last key again, masked below
 #pragma unroll
-                for (int j = 0; j < PIECES; j++) {
-                    const unsigned o0 = (unsigned)min(drow + j * 4 * PK, left) * ts2;
-                    ROWS_DMA(o0 + kch, ksrc + off, dst + j * 4096);
-                    ROWS_DMA(o0 + vch, vsrc + off, dst + WTILE + j * 4096);
-                }
+                for (int j = 0; j < PIECES; j++) r[j] = (unsigned)min(drow + j * 4 * PK, left) * ts2;
             }
+#define ROWS_LD(V, S) "global_load_lds_dwordx4 " V ", " S "\n\t"
+#define ROWS_ST "s_add_u32 m0, m0, 0x1000\n\ts_nop 0\n\t"
+            if constexpr (PIECES == 4)
+                asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %11\n\ts_nop 0\n\t" ROWS_LD("%1", "%9") ROWS_ST ROWS_LD("%2", "%9") ROWS_ST
+                                 ROWS_LD("%3", "%9") ROWS_ST ROWS_LD("%4", "%9") ROWS_ST ROWS_LD("%5", "%10") ROWS_ST ROWS_LD("%6", "%10") ROWS_ST
+                                     ROWS_LD("%7", "%10") ROWS_ST ROWS_LD("%8", "%10") "s_mov_b32 m0, %0"
+                             : "=&s"(keep)
+                             : "v"(r[0] + kch), "v"(r[1] + kch), "v"(r[2] + kch), "v"(r[3 % PIECES] + kch), "v"(r[0] + vch), "v"(r[1] + vch),
+                               "v"(r[2 % PIECES] + vch), "v"(r[3 % PIECES] + vch), "s"(ksrc + off), "s"(vsrc + off), "s"(dst)
+                             : "memory", "scc");
+            else
+                asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %7\n\ts_nop 0\n\t" ROWS_LD("%1", "%5") ROWS_ST ROWS_LD("%2", "%5") ROWS_ST
+                                 ROWS_LD("%3", "%6") ROWS_ST ROWS_LD("%4", "%6") "s_mov_b32 m0, %0"
+                             : "=&s"(keep)
+                             : "v"(r[0] + kch), "v"(r[1] + kch), "v"(r[0] + vch), "v"(r[1] + vch), "s"(ksrc + off), "s"(vsrc + off), "s"(dst)
+                             : "memory", "scc");
+#undef ROWS_LD
+#undef ROWS_ST
         };
         if (kt0 < kt1) issue(kt0);
         w.load_q(qrow, h2);
-        for (int kt = kt0; kt < kt1; kt++) {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();                                   // the tile has landed, and the other buffer is no longer read
-            if (kt + 1 < kt1) issue(kt + 1);
-            const int kbase = kt * kWideKeys;
-            if (kbase >= wmax) continue;                       // (a wave's rows see nothing of this tile)
-            const unsigned char *buf = lds + (kt & 1) * (2 * WTILE);
-            f32x16 s[2];
-            w.scores(buf, s);
-            w.softmax(s, kbase + kWideKeys > wmin, lim - kbase - 4 * h2);
-            w.accumulate(buf + WTILE, s);
-        }
-        w.l += __shfl_xor(w.l, 32, 64);
+        if (wmax == 0)                                         // a wave without rows, or whose rows see nothing: brings its pieces only
+            for (int kt = kt0; kt < kt1; kt++) {
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                __syncthreads();
+                if (kt + 1 < kt1) issue(kt + 1);
+            }
+        else
+            for (int kt = kt0; kt < kt1; kt++) {
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                __syncthreads();                               // the tile has landed, and the other buffer is no longer read
+                if (kt + 1 < kt1) issue(kt + 1);
+                const int kbase = kt * kWideKeys;
+                const unsigned char *buf = lds + (kt & 1) * (2 * WTILE);
+                f32x16 s[2];
+                w.scores(buf, s);
+                w.softmax(s, kbase + kWideKeys > wmin, lim - kbase - 4 * h2, kt == kt0);
+                w.accumulate(buf + WTILE, s);
+            }
+        w.finish();
         const int64_t at = pr + (int64_t)tok * p.nh + head;
         if (p.part_o) {
             if (!ok) return;
-            if (h2 == 0) *reinterpret_cast<float2 *>(p.part_ml + at * 2) = make_float2(w.m, w.l);
+            if (h2 == 0) *reinterpret_cast<float2 *>(p.part_ml + at * 2) = make_float2(w.ms, w.l);
             float *po = p.part_o + at * HD + 4 * h2;
 #pragma unroll
             for (int d = 0; d < ND; d++)
@@ -457,7 +490,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(const RowsParams p)
         w.scores(kbuf, s);
         asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(s[0]) : : "memory");       // the tile's keys have been read
         if (more) issue(kt + 4, ksrc, kdst, false);
-        w.softmax(s, kbase + kNarrowKeys > wmin, lim - kbase - 4 * h2);
+        w.softmax(s, kbase + kNarrowKeys > wmin, lim - kbase - 4 * h2, kt == kt0 + wid);
         if (!more) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         else if (PIECES == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
         else asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
@@ -465,10 +498,10 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(const RowsParams p)
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         if (more) issue(kt + 4, vsrc, vdst, true);
     }
-    w.l += __shfl_xor(w.l, 32, 64);
+    w.finish();
     __syncthreads();                                           // the tiles are no longer read
     float *sml = reinterpret_cast<float *>(lds + 4 * JWAVE);
-    if (h2 == 0) *reinterpret_cast<float2 *>(sml + (wid * 32 + l32) * 2) = make_float2(w.m, w.l);
+    if (h2 == 0) *reinterpret_cast<float2 *>(sml + (wid * 32 + l32) * 2) = make_float2(w.ms, w.l);
 #pragma unroll
     for (int d = 0; d < ND; d++)
 #pragma unroll
@@ -487,7 +520,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(const RowsParams p)
     }
 #pragma unroll
     for (int u = 0; u < 4; u++) {
-        wj[u] = __builtin_amdgcn_exp2f((mj[u] - m) * w.c1);
+        wj[u] = __builtin_amdgcn_exp2f(mj[u] - m);
         l += sml[(u * 32 + jr) * 2 + 1] * wj[u];
     }
     const int jtok = n0 + jt, jhead = kvh * G + jg;
@@ -509,11 +542,11 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(const RowsParams p)
     }
 }
 
-// out = sum_j o_j 2^((m_j - m) c1) / sum_j l_j 2^((m_j - m) c1); a row is HD / 4 lanes.  Lane j of a row reads part j's (max, sum), so
+// out = sum_j o_j 2^(m_j - m) / sum_j l_j 2^(m_j - m); a row is HD / 4 lanes.  Lane j of a row reads part j's (max, sum), so
 // that the weights cost one round trip; the partial rows come eight at a time.
 template <int HD>
 __global__ __launch_bounds__(256) void k_attn_join(const float *__restrict__ part_o, const float *__restrict__ part_ml, int64_t rows,
-                                                   int parts, float c1, uint16_t *__restrict__ out, int64_t o_ts, int nh)
+                                                   int parts, uint16_t *__restrict__ out, int64_t o_ts, int nh)
 {
     constexpr int L = HD / 4, U = 8;
     const int64_t row = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
@@ -529,7 +562,7 @@ __global__ __launch_bounds__(256) void k_attn_join(const float *__restrict__ par
         float w = 0.0f;
         if (j0 + li < parts) {
             const float2 ml = *reinterpret_cast<const float2 *>(part_ml + ((int64_t)(j0 + li) * rows + row) * 2);
-            w = __builtin_amdgcn_exp2f((ml.x - m) * c1);
+            w = __builtin_amdgcn_exp2f(ml.x - m);
             l += ml.y * w;
         }
         const int nj = min(L, parts - j0);
@@ -612,9 +645,8 @@ static void join_launch(const RowsParams &p, int hd, int parts, hipStream_t st)
 {
     const int64_t rows = p.part_rows, per = 256 / (hd / 4);
     const dim3 grid((unsigned)((rows + per - 1) / per));
-    const float c1 = p.scale * 1.4426950408889634f;
-    if (hd == 128) hipLaunchKernelGGL(k_attn_join<128>, grid, dim3(256), 0, st, p.part_o, p.part_ml, rows, parts, c1, p.out, p.o_ts, p.nh);
-    else hipLaunchKernelGGL(k_attn_join<64>, grid, dim3(256), 0, st, p.part_o, p.part_ml, rows, parts, c1, p.out, p.o_ts, p.nh);
+    if (hd == 128) hipLaunchKernelGGL(k_attn_join<128>, grid, dim3(256), 0, st, p.part_o, p.part_ml, rows, parts, p.out, p.o_ts, p.nh);
+    else hipLaunchKernelGGL(k_attn_join<64>, grid, dim3(256), 0, st, p.part_o, p.part_ml, rows, parts, p.out, p.o_ts, p.nh);
 }
 
 static void packed_plan(int64_t ntokens, int64_t nseqs, int G, int nkv, int max_keys, KeySet *k)
