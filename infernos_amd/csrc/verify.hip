@@ -5,38 +5,43 @@
 // that neither the way a sum is split nor the exponential's rounding moves a border past the number (f32 exponentials would move one in
 // every few hundred draws from a flat tail).  The f64 work (a short polynomial, ~20 operations a logit) stays under the time the logits
 // take to arrive.
-//   k_verify_stats   a chunk of a target row each: (max, sum of exp) of the chunk, or its arg-max for temperature 0
-//   k_verify_mass    a chunk each: which draft the row refuses, and where one was, the mass of max(p - q, 0) in the chunk
-//   k_verify_draw    a row each: the chunk and then the token where the cumulated mass passes the uniform number
+//   k_verify_stats   a wave a chunk of a target row: (max, sum of exp), or the arg-max for temperature 0
+//   k_verify_mass    a wave a chunk of the refused position, where the draft has a distribution: the mass of max(p - q, 0)
+//   k_verify_draw    a workgroup a row: the chunk and then the token where the cumulated mass passes the uniform number
+// The rows' verdicts (which draft is refused) are worked out from the chunk statistics by every workgroup that asks, its waves taking the
+// row's positions in parallel: a launch of its own for them would cost more.
 #include "common.h"
 
 namespace ifh {
 
-constexpr int VC_THREADS = 256, VC_VEC = 8, VC = VC_THREADS * VC_VEC * 4;      // logits a chunk: 8192, 32 a thread
+constexpr int VT = 256, VPL = 32, VC = 64 * VPL;        // threads, logits a lane, logits a chunk (a wave's)
+constexpr int kVerifyMaxChunks = VT;                    // 524 288 tokens: the draw gives each chunk a thread
+constexpr float kFltMax = 3.402823466e38f;
 
-// e^x for x <= 0 in f64, relative error below 1e-12: x = k ln 2 + r, |r| <= ln 2 / 2, Taylor polynomial of degree 11 in r
+// e^x for x <= 0 in f64, relative error below 1e-10: x = k ln 2 + r, |r| <= ln 2 / 2 (k by adding and taking off 1.5 2^52), the Taylor
+// polynomial of degree 9, of which the part from r^4 on, no more than 6e-4 of the whole, is f32
 __device__ __forceinline__ double exp_neg(double x)
 {
-    if (!(x > -700.0)) return 0.0;
-    const double k = __builtin_rint(x * 1.4426950408889634);
-    const double r = __builtin_fma(k, -1.9082149292705877e-10, __builtin_fma(k, -0.6931471803691238, x));
-    double e = 2.505210838544172e-8;                       // 1 / 11!
-    e = __builtin_fma(e, r, 2.755731922398589e-7);
-    e = __builtin_fma(e, r, 2.7557319223985893e-6);
-    e = __builtin_fma(e, r, 2.48015873015873e-5);
-    e = __builtin_fma(e, r, 1.984126984126984e-4);
-    e = __builtin_fma(e, r, 1.388888888888889e-3);
-    e = __builtin_fma(e, r, 8.333333333333333e-3);
-    e = __builtin_fma(e, r, 4.1666666666666664e-2);
-    e = __builtin_fma(e, r, 0.16666666666666666);
+    const double big = 6755399441055744.0;
+    const double kb = __builtin_fma(fmax(x, -745.0), 1.4426950408889634, big), k = kb - big;
+    const double r = __builtin_fma(k, -0.6931471805599453, fmax(x, -745.0));
+    const float f = (float)r;
+    float t = 2.7557319e-6f;                               // 1 / 9!
+    t = __builtin_fmaf(t, f, 2.4801587e-5f);
+    t = __builtin_fmaf(t, f, 1.9841270e-4f);
+    t = __builtin_fmaf(t, f, 1.3888889e-3f);
+    t = __builtin_fmaf(t, f, 8.3333333e-3f);
+    t = __builtin_fmaf(t, f, 4.1666667e-2f);
+    double e = __builtin_fma((double)t, r, 0.16666666666666666);
     e = __builtin_fma(e, r, 0.5);
     e = __builtin_fma(e, r, 1.0);
     e = __builtin_fma(e, r, 1.0);
-    return __builtin_ldexp(e, (int)k);
+    const double v = __builtin_ldexp(e, (int)k);
+    return x > -745.0 ? v : 0.0;
 }
 
 // NaN counts as -inf; +inf as the largest finite value (its differences stay finite)
-__device__ __forceinline__ float logit(float l) { return l == l ? fminf(l, 3.402823466e38f) : -INFINITY; }
+__device__ __forceinline__ float logit(float l) { return l == l ? fminf(l, kFltMax) : -INFINITY; }
 
 struct VerifyParams {
     const float *logits;
@@ -49,22 +54,26 @@ struct VerifyParams {
     int vocab, nrows, T, nch;
     double inv_temp;
     int greedy, vec, qvec;
-    float *cmax;                 // [rows * (T+1)][nch] chunk maxima
-    double *csum;                // [rows * (T+1)][nch] chunk sums of exp((l - cmax) / temperature); greedy: the arg-max of the chunk
+    double *csum;                // [rows * (T+1)][nch] chunk sums of exp((l - cmax) / temperature); greedy: the place of the chunk's maximum
     double *mass;                // [rows][nch]
+    float *cmax;                 // [rows * (T+1)][nch] chunk maxima
 };
 
-__device__ __forceinline__ void load_chunk(const float *row, int base, int vocab, int vec, float fill, float (&v)[VC_VEC * 4])
+// a lane's elements of the chunk at `base`: 16 bytes at a time where the row is aligned, else every 64th
+__device__ __forceinline__ int place(int vec, int base, int lane, int e) { return base + (vec ? (e >> 2) * 256 + lane * 4 + (e & 3) : e * 64 + lane); }
+__device__ __forceinline__ void load_chunk(const float *row, int base, int lane, int vocab, int vec, float fill, float (&v)[VPL])
 {
+    if (vec && base + VC <= vocab) {
 #pragma unroll
-    for (int u = 0; u < VC_VEC; u++) {
-        const int j = base + (u * VC_THREADS + (int)threadIdx.x) * 4;
-        if (vec && j + 3 < vocab) {
-            const float4 f = *reinterpret_cast<const float4 *>(row + j);
-            v[4 * u] = f.x; v[4 * u + 1] = f.y; v[4 * u + 2] = f.z; v[4 * u + 3] = f.w;
-        } else {
+        for (int e = 0; e < VPL; e += 4) {
+            const float4 f = *reinterpret_cast<const float4 *>(row + base + e * 64 + lane * 4);
+            v[e] = f.x; v[e + 1] = f.y; v[e + 2] = f.z; v[e + 3] = f.w;
+        }
+    } else {
 #pragma unroll
-            for (int e = 0; e < 4; e++) v[4 * u + e] = j + e < vocab ? row[j + e] : fill;
+        for (int e = 0; e < VPL; e++) {
+            const int j = place(vec, base, lane, e);
+            v[e] = j < vocab ? row[j] : fill;
         }
     }
 }
@@ -76,284 +85,310 @@ __device__ __forceinline__ double wave_sum_d(double v)
     return v;
 }
 
-__global__ __launch_bounds__(VC_THREADS) void k_verify_stats(const VerifyParams p)
+__global__ __launch_bounds__(VT) void k_verify_stats(const VerifyParams p)
 {
-    __shared__ float sm[4];
-    __shared__ double sd[4];
     const int64_t pos = blockIdx.y;
-    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, base = blockIdx.x * VC;
-    float v[VC_VEC * 4];
-    load_chunk(p.logits + pos * p.ld, base, p.vocab, p.vec, -INFINITY, v);
+    const int lane = threadIdx.x & 63, c = blockIdx.x * 4 + (threadIdx.x >> 6), base = c * VC;
+    if (c >= p.nch) return;
+    float v[VPL];
+    load_chunk(p.logits + pos * p.ld, base, lane, p.vocab, p.vec, -INFINITY, v);
     float m = -INFINITY;
 #pragma unroll
-    for (int e = 0; e < VC_VEC * 4; e++) {
+    for (int e = 0; e < VPL; e++) {
         v[e] = logit(v[e]);
         m = fmaxf(m, v[e]);
     }
     m = wave_max(m);
-    if (lane == 0) sm[wid] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
     double s = 0.0;
     if (p.greedy) {
         int at = 0x7fffffff;                                 // the first place of the maximum
 #pragma unroll
-        for (int e = VC_VEC * 4 - 1; e >= 0; e--)
-            if (v[e] == m) at = base + ((e >> 2) * VC_THREADS + (int)threadIdx.x) * 4 + (e & 3);
+        for (int e = 0; e < VPL; e++)
+            if (v[e] == m) at = min(at, place(p.vec, base, lane, e));
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) at = min(at, __shfl_xor(at, o, 64));
         s = (double)at;
-        if (lane == 0) sd[wid] = s;
-        __syncthreads();
-        s = fmin(fmin(sd[0], sd[1]), fmin(sd[2], sd[3]));
     } else {
-        const double md = (double)fmaxf(m, -3.402823466e38f);
+        const double md = (double)fmaxf(m, -kFltMax);
+        double s1 = 0.0;
 #pragma unroll
-        for (int e = 0; e < VC_VEC * 4; e++) s += exp_neg(((double)v[e] - md) * p.inv_temp);
-        s = wave_sum_d(s);
-        if (lane == 0) sd[wid] = s;
-        __syncthreads();
-        s = (sd[0] + sd[1]) + (sd[2] + sd[3]);
+        for (int e = 0; e < VPL; e += 2) {
+            s += exp_neg(((double)v[e] - md) * p.inv_temp);
+            s1 += exp_neg(((double)v[e + 1] - md) * p.inv_temp);
+        }
+        s = wave_sum_d(s + s1);
     }
-    if (threadIdx.x == 0) {
-        p.cmax[pos * p.nch + blockIdx.x] = m;
-        p.csum[pos * p.nch + blockIdx.x] = s;
+    if (lane == 0) {
+        p.cmax[pos * p.nch + c] = m;
+        p.csum[pos * p.nch + c] = s;
     }
 }
 
-// what a row's chunk statistics say: the number of drafts it keeps, whether the next one was refused, and the statistics of the
-// position that is drawn.  One wave; the same sums in the same order in every workgroup that asks.
+// What a row's chunk statistics say: the drafts it keeps, whether the next one is refused, and the statistics of the drawn position.
+// The workgroup's waves take the positions in turn; the same sums in the same order wherever it is asked.
 struct Verdict {
     int kept, refused, best;
     float m;
     double s;
 };
+struct VerdictLds {
+    double s[64];
+    float m[64];
+    int best[64], keep[64];
+};
 
-__device__ __forceinline__ Verdict verdict_of(const VerifyParams &p, int r)
+__device__ __forceinline__ Verdict verdict_of(const VerifyParams &p, int r, VerdictLds &L)
 {
-    const int lane = threadIdx.x & 63;
-    Verdict w = {0, 0, -1, 0.0f, 0.0};
+    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
     const int n = p.lens ? min(max(p.lens[r], 0), p.T) : p.T;
-    for (int i = 0; i <= n; i++) {
+    for (int i = wid; i <= n; i += VT / 64) {
         const int64_t pos = (int64_t)r * (p.T + 1) + i;
-        float m = -INFINITY;
-        for (int c = lane; c < p.nch; c += 64) m = fmaxf(m, p.cmax[pos * p.nch + c]);
+        const int x = i < n ? p.drafts[(int64_t)r * p.T + i] : -1;
+        const bool in = x >= 0 && x < p.vocab;
+        const float lx = in ? p.logits[pos * p.ld + x] : 0.0f;
+        const double qx = in && p.q ? (double)p.q[((int64_t)r * p.T + i) * p.q_ld + x] : 1.0;
+        const double u = i < n ? (double)p.uniform[(int64_t)r * (p.T + 1) + i] : 0.0;
+        float cm[kVerifyMaxChunks / 64], m = -INFINITY;
+        double cs[kVerifyMaxChunks / 64];
+#pragma unroll
+        for (int k = 0; k < kVerifyMaxChunks / 64; k++) {
+            const int c = k * 64 + lane;
+            cm[k] = c < p.nch ? p.cmax[pos * p.nch + c] : -INFINITY;
+            cs[k] = c < p.nch ? p.csum[pos * p.nch + c] : 0.0;
+            m = fmaxf(m, cm[k]);
+        }
         m = wave_max(m);
         const bool any = m > -INFINITY;
         double s = 0.0;
         int best = 0x7fffffff;
         if (p.greedy) {
-            for (int c = lane; c < p.nch; c += 64)
-                if (any && p.cmax[pos * p.nch + c] == m) best = min(best, (int)p.csum[pos * p.nch + c]);
+#pragma unroll
+            for (int k = 0; k < kVerifyMaxChunks / 64; k++)
+                if (any && cm[k] == m) best = min(best, (int)cs[k]);
 #pragma unroll
             for (int o = 32; o > 0; o >>= 1) best = min(best, __shfl_xor(best, o, 64));
         } else {
-            for (int c = lane; c < p.nch; c += 64)
-                s += p.csum[pos * p.nch + c] * exp_neg(((double)fmaxf(p.cmax[pos * p.nch + c], -3.402823466e38f) - (double)fmaxf(m, -3.402823466e38f)) * p.inv_temp);
+            // (no chunk with a finite maximum: every sum is 0)
+#pragma unroll
+            for (int k = 0; k < kVerifyMaxChunks / 64; k++)
+                if (k * 64 < p.nch) s += cs[k] * exp_neg(((double)fmaxf(cm[k], -kFltMax) - (double)fmaxf(m, -kFltMax)) * p.inv_temp);
             s = wave_sum_d(s);
         }
-        w.kept = i;
-        w.m = m;
-        w.s = s;
-        w.best = any ? best : -1;
-        if (i == n) break;
-        const int x = p.drafts[(int64_t)r * p.T + i];
-        bool keep = false;
-        if (x >= 0 && x < p.vocab && any) {
-            const double qx = p.q ? (double)p.q[((int64_t)r * p.T + i) * p.q_ld + x] : 1.0;
-            const double px = p.greedy ? (x == best ? 1.0 : 0.0) : exp_neg(((double)logit(p.logits[pos * p.ld + x]) - (double)m) * p.inv_temp) / s;
-            keep = (double)p.uniform[(int64_t)r * (p.T + 1) + i] * qx < px;
-        }
-        if (!keep) {
-            w.refused = 1;
-            break;
+        if (lane == 0) {
+            const double px = !in || !any ? 0.0 : p.greedy ? (x == best ? 1.0 : 0.0) : exp_neg(((double)logit(lx) - (double)m) * p.inv_temp) / s;
+            L.keep[i] = in && any && u * qx < px;
+            L.m[i] = m;
+            L.s[i] = s;
+            L.best[i] = any ? best : -1;
         }
     }
+    __syncthreads();
+    const unsigned long long refuse = __ballot(lane < n && !L.keep[lane < n ? lane : 0]);
+    Verdict w;
+    w.kept = refuse ? __ffsll((long long)refuse) - 1 : n;
+    w.refused = refuse != 0;
+    w.m = L.m[w.kept];
+    w.s = L.s[w.kept];
+    w.best = L.best[w.kept];
     return w;
 }
 
-// mass of token j at the drawn position: max(p - q, 0) at a refused draft, else p (in units of the sum: the draw is relative)
-__device__ __forceinline__ double rest_of(double e, double inv_s, bool has_q, float qv, bool is_draft)
+__global__ __launch_bounds__(VT) void k_verify_mass(const VerifyParams p)
 {
-    if (has_q) return fmax(e * inv_s - (double)qv, 0.0);
-    return is_draft ? fmax(e * inv_s - 1.0, 0.0) : e * inv_s;
-}
-
-__global__ __launch_bounds__(VC_THREADS) void k_verify_mass(const VerifyParams p)
-{
-    __shared__ double sd[4];
-    const int r = blockIdx.y, lane = threadIdx.x & 63, wid = threadIdx.x >> 6, base = blockIdx.x * VC;
-    const Verdict w = verdict_of(p, r);
-    if (p.greedy || !w.refused || !(w.s > 0.0)) return;
-    float v[VC_VEC * 4], q[VC_VEC * 4];
-    load_chunk(p.logits + ((int64_t)r * (p.T + 1) + w.kept) * p.ld, base, p.vocab, p.vec, -INFINITY, v);
-    if (p.q) load_chunk(p.q + ((int64_t)r * p.T + w.kept) * p.q_ld, base, p.vocab, p.qvec, 0.0f, q);
-    const int x = p.drafts[(int64_t)r * p.T + w.kept];
+    __shared__ VerdictLds L;
+    const int r = blockIdx.y, lane = threadIdx.x & 63, c = blockIdx.x * 4 + (threadIdx.x >> 6), base = c * VC;
+    const Verdict w = verdict_of(p, r, L);
+    if (c >= p.nch || !w.refused || !(w.s > 0.0)) return;
+    float v[VPL], q[VPL];
+    load_chunk(p.logits + ((int64_t)r * (p.T + 1) + w.kept) * p.ld, base, lane, p.vocab, p.vec, -INFINITY, v);
+    load_chunk(p.q + ((int64_t)r * p.T + w.kept) * p.q_ld, base, lane, p.vocab, p.qvec && p.vec, 0.0f, q);
+    if (p.vec && !p.qvec) {                                  // (the two rows have to be read in one order)
+#pragma unroll
+        for (int e = 0; e < VPL; e++) {
+            const int j = place(1, base, lane, e);
+            q[e] = j < p.vocab ? p.q[((int64_t)r * p.T + w.kept) * p.q_ld + j] : 0.0f;
+        }
+    }
     const double inv_s = 1.0 / w.s;
     double s = 0.0;
 #pragma unroll
-    for (int e = 0; e < VC_VEC * 4; e++) {
-        const int j = base + ((e >> 2) * VC_THREADS + (int)threadIdx.x) * 4 + (e & 3);
-        s += rest_of(exp_neg(((double)logit(v[e]) - (double)w.m) * p.inv_temp), inv_s, p.q != nullptr, p.q ? q[e] : 0.0f, j == x);
-    }
+    for (int e = 0; e < VPL; e++)
+        s += fmax(__builtin_fma(exp_neg(((double)logit(v[e]) - (double)w.m) * p.inv_temp), inv_s, -(double)q[e]), 0.0);
     s = wave_sum_d(s);
-    if (lane == 0) sd[wid] = s;
-    __syncthreads();
-    if (threadIdx.x == 0) p.mass[(int64_t)r * p.nch + blockIdx.x] = (sd[0] + sd[1]) + (sd[2] + sd[3]);
+    if (lane == 0) p.mass[(int64_t)r * p.nch + c] = s;
 }
 
-__global__ __launch_bounds__(VC_THREADS) void k_verify_draw(const VerifyParams p)
+// inclusive sums over the workgroup's threads, in thread order
+__device__ __forceinline__ double block_scan(double v, double (&part)[VT / 64])
 {
-    __shared__ double part[VC_THREADS];
-    __shared__ int found, last;
+    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const double b = __shfl_up(v, o, 64);
+        if (lane >= o) v += b;
+    }
+    if (lane == 63) part[wid] = v;
+    __syncthreads();
+    double before = 0.0;
+#pragma unroll
+    for (int w = 0; w < VT / 64; w++) before += w < wid ? part[w] : 0.0;
+    return before + v;
+}
+
+__global__ __launch_bounds__(VT) void k_verify_draw(const VerifyParams p)
+{
+    __shared__ VerdictLds L;
+    __shared__ double part[3][VT / 64], scut[2], without;
+    __shared__ int first[2], last;
     const int r = blockIdx.x, tid = threadIdx.x;
-    const Verdict w = verdict_of(p, r);
+    const Verdict w = verdict_of(p, r, L);
     int token = -1;
     if (p.greedy) token = w.best;
     else if (w.s > 0.0) {
         const int64_t pos = (int64_t)r * (p.T + 1) + w.kept;
-        // the chunks' masses in order, the same in every thread
-        bool rest = w.refused;
-        double total = 0.0;
-        if (rest) {
-            for (int c = 0; c < p.nch; c++) total += p.mass[(int64_t)r * p.nch + c];
-            rest = total > 0.0;
+        const float *row = p.logits + pos * p.ld, *qrow = p.q && w.refused ? p.q + ((int64_t)r * p.T + w.kept) * p.q_ld : nullptr;
+        const int x = w.refused && !p.q ? p.drafts[(int64_t)r * p.T + w.kept] : -1;      // a looked-up draft: everything but itself is left over
+        const double inv_s = 1.0 / w.s, u = (double)p.uniform[(int64_t)r * (p.T + 1) + p.T];
+        auto e_at = [&](int j) { return exp_neg(((double)logit(row[j]) - (double)w.m) * p.inv_temp); };
+        if (tid < 2) first[tid] = 0x7fffffff;
+        if (tid == 2) last = -1;
+        // a thread a chunk: mass of p (in units of the sum), and with a draft's distribution what p has over it
+        double pm = 0.0;
+        if (tid < p.nch) pm = p.csum[pos * p.nch + tid] * exp_neg(((double)fmaxf(p.cmax[pos * p.nch + tid], -kFltMax) - (double)w.m) * p.inv_temp);
+        double cm = pm;
+        bool rest = false;
+        if (x >= 0 && x < p.vocab) {                          // the draft's own chunk again, without it
+            const int base = x / VC * VC;
+            double s = 0.0;
+            for (int e = tid; e < VC; e += VT)
+                if (base + e < p.vocab && base + e != x) s += e_at(base + e);
+            const double t = block_scan(s, part[2]);
+            if (tid == VT - 1) without = t;
+            __syncthreads();
+            if (tid == x / VC) cm = without;
+            rest = true;
+        } else if (qrow) {
+            if (tid < p.nch) cm = p.mass[(int64_t)r * p.nch + tid];
+            rest = true;
         }
-        auto chunk = [&](int c) {
-            return rest ? p.mass[(int64_t)r * p.nch + c]
-                        : p.csum[pos * p.nch + c] * exp_neg(((double)fmaxf(p.cmax[pos * p.nch + c], -3.402823466e38f) - (double)w.m) * p.inv_temp);
-        };
-        if (!rest) {
-            total = 0.0;
-            for (int c = 0; c < p.nch; c++) total += chunk(c);
-        }
-        const double want = (double)p.uniform[(int64_t)r * (p.T + 1) + p.T] * total;
-        double before = 0.0;
-        int c = 0, full = 0;
-        double fbefore = 0.0;
-        for (; c < p.nch; c++) {                              // the first chunk in which the mass passes; rounding past the end: the last with any
-            const double m = chunk(c);
-            if (before + m > want) break;
-            if (m > 0.0) {
-                full = c;
-                fbefore = before;
-            }
-            before += m;
-        }
-        if (c == p.nch) {
-            c = full;
-            before = fbefore;
-        }
-        // inside the chunk: 32 consecutive tokens a thread
-        const float *row = p.logits + pos * p.ld, *qrow = p.q && rest ? p.q + ((int64_t)r * p.T + w.kept) * p.q_ld : nullptr;
-        const int x = rest ? p.drafts[(int64_t)r * p.T + w.kept] : -1, j0 = c * VC + tid * (VC_VEC * 4);
-        const double inv_s = 1.0 / w.s;
-        auto mass_at = [&](int j) {
-            const double e = exp_neg(((double)logit(row[j]) - (double)w.m) * p.inv_temp);
-            return rest ? rest_of(e, inv_s, qrow != nullptr, qrow ? qrow[j] : 0.0f, j == x) : e;
-        };
-        double mine = 0.0;
-        int lastj = -1;
-        for (int e = 0; e < VC_VEC * 4; e++)
-            if (j0 + e < p.vocab) {
-                const double m = mass_at(j0 + e);
-                mine += m;
-                if (m > 0.0) lastj = j0 + e;
-            }
-        part[tid] = mine;
-        if (tid == 0) found = last = -1;
         __syncthreads();
+        double cum = block_scan(tid < p.nch ? cm : 0.0, part[0]);
+        if (tid == VT - 1) scut[0] = cum;
+        __syncthreads();
+        if (rest && !(scut[0] > 0.0)) {                       // nothing is left over: the token comes from p
+            rest = false;
+            cm = pm;
+            __syncthreads();
+            cum = block_scan(tid < p.nch ? cm : 0.0, part[1]);
+            if (tid == VT - 1) scut[0] = cum;
+            __syncthreads();
+        }
+        const double want = u * scut[0];
+        if (tid < p.nch && cum > want) atomicMin(&first[0], tid);
+        __syncthreads();
+        const int c = min(first[0], p.nch - 1);
+        if (tid == c) scut[1] = cum - cm;
+        __syncthreads();
+        // the chunk's tokens, eight consecutive ones a thread
+        constexpr int E = VC / VT;
+        const int j0 = c * VC + tid * E;
+        double mass[E], mine = 0.0;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            const int j = j0 + e;
+            mass[e] = 0.0;
+            if (j < p.vocab) {
+                const double v = e_at(j);
+                if (rest && qrow) mass[e] = fmax(__builtin_fma(v, inv_s, -(double)qrow[j]), 0.0);
+                else if (!(rest && j == x)) mass[e] = v;
+            }
+            mine += mass[e];
+        }
+        const double upto = scut[1] + block_scan(mine, part[2]);
+        int at = -1, lastj = -1;
+        double a = upto - mine;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            a += mass[e];
+            if (mass[e] > 0.0) {
+                lastj = j0 + e;
+                if (at < 0 && a > want) at = j0 + e;
+            }
+        }
+        if (at >= 0) atomicMin(&first[1], at);
         if (lastj >= 0) atomicMax(&last, lastj);
-        double pre = before;
-        for (int t = 0; t < tid; t++) pre += part[t];
-        if (pre <= want && pre + mine > want) {
-            double a = pre;
-            int at = lastj;
-            for (int e = 0; e < VC_VEC * 4; e++)
-                if (j0 + e < p.vocab) {
-                    a += mass_at(j0 + e);
-                    if (a > want) {
-                        at = j0 + e;
-                        break;
-                    }
-                }
-            found = at;
-        }
         __syncthreads();
-        token = found >= 0 ? found : last;
+        token = first[1] != 0x7fffffff ? first[1] : last;     // (rounding past the chunk's end: its last token with any mass)
     }
-    for (int i = tid; i <= p.T; i += VC_THREADS)
+    for (int i = tid; i <= p.T; i += VT)
         p.out_tokens[(int64_t)r * (p.T + 1) + i] = i < w.kept ? p.drafts[(int64_t)r * p.T + i] : i == w.kept ? token : -1;
     if (tid == 0) p.out_count[r] = w.kept + 1;
 }
 
-// One wave a row: lane c holds the target's candidate c, and of the draft's candidates one a step comes round by broadcast.
-__global__ __launch_bounds__(64) void k_verify_topk(const int32_t *__restrict__ cand, const float *__restrict__ probs,
+// A workgroup a row, half a wave a position: lane c holds candidate c.  The first refusal's remaining mass needs the draft's probability of
+// each candidate, looked up in LDS.
+__global__ __launch_bounds__(VT) void k_verify_topk(const int32_t *__restrict__ cand, const float *__restrict__ probs,
                                                     const int32_t *__restrict__ dcand, const float *__restrict__ dprobs,
                                                     const int32_t *__restrict__ drafts, const int32_t *__restrict__ lens,
                                                     const float *__restrict__ uniform, int T, int32_t *__restrict__ out_tokens,
                                                     int32_t *__restrict__ out_count)
 {
+    __shared__ int keep[64], sid[32];
+    __shared__ float sp[32];
     const int64_t r = blockIdx.x;
-    const int lane = threadIdx.x, c = lane & 31;
-    const bool mine = lane < 32;
+    const int tid = threadIdx.x, lane = tid & 63, c = tid & 31;
     const int n = lens ? min(max(lens[r], 0), T) : T;
-    int kept = 0, token = -1;
-    for (int i = 0; i <= n; i++) {
-        const int64_t at = (r * (T + 1) + i) * 32 + c;
-        const int id = cand[at];
-        const float pv = probs[at];
-        const double p = mine && pv > 0.0f ? (double)pv : 0.0;
-        double w = p;
-        if (i < n) {
-            const int x = drafts[r * T + i];
-            int did = -1;
-            float dp = 0.0f;
-            if (dcand) {
-                const int64_t da = (r * T + i) * 32 + c;
-                did = dcand[da];
-                dp = dprobs[da];
-            }
-            double q = 0.0;                                            // the draft's probability of this lane's candidate
-            if (dcand) {
-                for (int k = 0; k < 32; k++) {
-                    const int kid = __shfl(did, k, 64);
-                    const float kp = __shfl(dp, k, 64);                // (by every lane: a lane that is switched off hands nothing out)
-                    q += kid == id ? (double)kp : 0.0;
-                }
-            } else
-                q = id == x ? 1.0 : 0.0;
-            double px = id == x ? p : 0.0, qx = dcand ? (mine && did == x ? (double)dp : 0.0) : 0.0;
+    const float ud = uniform[r * (T + 1) + T];
+    for (int i = tid >> 5; i < n; i += VT / 32) {
+        const int x = drafts[r * T + i];
+        const float u = uniform[r * (T + 1) + i];
+        const int64_t at = (r * (T + 1) + i) * 32 + c, da = (r * T + i) * 32 + c;
+        const int id = cand[at], did = dcand ? dcand[da] : -1;
+        const float pv = probs[at], dv = dcand ? dprobs[da] : 0.0f;
+        double px = id == x && pv > 0.0f ? (double)pv : 0.0, qx = dcand && did == x ? (double)dv : 0.0;
 #pragma unroll
-            for (int o = 32; o > 0; o >>= 1) {
-                px += __shfl_xor(px, o, 64);
-                qx += __shfl_xor(qx, o, 64);
-            }
-            if (!dcand) qx = 1.0;
-            if ((double)uniform[r * (T + 1) + i] * qx < px) {
-                kept = i + 1;
-                continue;
-            }
-            const double rest = mine ? fmax(p - q, 0.0) : 0.0;
-            if (__any(rest > 0.0)) w = rest;
+        for (int o = 16; o > 0; o >>= 1) {
+            px += __shfl_xor(px, o, 32);
+            qx += __shfl_xor(qx, o, 32);
         }
-        // cumulated in the candidates' order
-        double cum = w;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const double b = __shfl_up(cum, o, 64);
-            if (lane >= o) cum += b;
-        }
-        const double total = __shfl(cum, 31, 64);
-        unsigned long long hit = __ballot(mine && cum > (double)uniform[r * (T + 1) + T] * total), some = __ballot(w > 0.0);
-        int k = -1;
-        if (some) k = hit ? __ffsll((long long)hit) - 1 : 63 - __clzll((long long)some);
-        const int tok = __shfl(id, k < 0 ? 0 : k, 64);
-        token = k < 0 ? -1 : tok;
-        break;
+        if (c == 0) keep[i] = (double)u * (dcand ? qx : 1.0) < px;
     }
-    for (int i = lane; i <= T; i += 64) out_tokens[r * (T + 1) + i] = i < kept ? drafts[r * T + i] : i == kept ? token : -1;
-    if (lane == 0) out_count[r] = kept + 1;
+    __syncthreads();
+    const unsigned long long refuse = __ballot(lane < n && !keep[lane < n ? lane : 0]);
+    const int kept = refuse ? __ffsll((long long)refuse) - 1 : n;
+    const int64_t at = (r * (T + 1) + kept) * 32 + c, da = (r * T + kept) * 32 + c;
+    if (refuse && dcand && tid < 32) {
+        sid[c] = dcand[da];
+        sp[c] = dprobs[da];
+    }
+    const int id = cand[at];
+    const float pv = probs[at];
+    const double p = pv > 0.0f ? (double)pv : 0.0;
+    __syncthreads();
+    double w = p;
+    if (refuse) {
+        double q = 0.0;
+        if (dcand) {
+#pragma unroll
+            for (int k = 0; k < 32; k++) q += sid[k] == id ? (double)sp[k] : 0.0;
+        } else
+            q = id == drafts[r * T + kept] ? 1.0 : 0.0;
+        const double rest = fmax(p - q, 0.0);
+        if (__any(rest > 0.0)) w = rest;
+    }
+    // cumulated in the candidates' order (both halves of a wave hold the same)
+    double cum = w;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const double b = __shfl_up(cum, o, 32);
+        if (c >= o) cum += b;
+    }
+    const double total = __shfl(cum, 31, 32);
+    const unsigned hit = (unsigned)__ballot(w > 0.0 && cum > (double)ud * total), some = (unsigned)__ballot(w > 0.0);
+    const int k = hit ? __ffs((int)hit) - 1 : some ? 31 - __clz((int)some) : -1;
+    const int tok = __shfl(id, k < 0 ? 0 : k, 32), token = k < 0 ? -1 : tok;
+    for (int i = tid; i <= T; i += VT) out_tokens[r * (T + 1) + i] = i < kept ? drafts[r * T + i] : i == kept ? token : -1;
+    if (tid == 0) out_count[r] = kept + 1;
 }
 
 }  // namespace ifh
@@ -361,7 +396,6 @@ __global__ __launch_bounds__(64) void k_verify_topk(const int32_t *__restrict__ 
 using namespace ifh;
 
 static int64_t verify_chunks(int vocab) { return ((int64_t)vocab + VC - 1) / VC; }
-constexpr int kVerifyMaxChunks = 64;             // 524 288 tokens
 
 extern "C" int64_t ifh_verify_drafts_ws_bytes(int nrows, int ndraft)
 {
@@ -393,13 +427,13 @@ extern "C" int ifh_verify_drafts_f32(const ifh_verify_desc *d, ifh_stream_t stre
     p.mass = p.csum + positions * p.nch;
     p.cmax = (float *)(p.mass + (int64_t)d->nrows * p.nch);
     hipStream_t st = as_stream(stream);
-    hipLaunchKernelGGL(k_verify_stats, dim3((unsigned)p.nch, (unsigned)positions), dim3(VC_THREADS), 0, st, p);
+    hipLaunchKernelGGL(k_verify_stats, dim3((unsigned)(p.nch + 3) / 4, (unsigned)positions), dim3(VT), 0, st, p);
     IFH_LAUNCH_CHECK("verify stats");
-    if (!p.greedy && p.T > 0) {
-        hipLaunchKernelGGL(k_verify_mass, dim3((unsigned)p.nch, (unsigned)p.nrows), dim3(VC_THREADS), 0, st, p);
+    if (!p.greedy && p.q && p.T > 0) {
+        hipLaunchKernelGGL(k_verify_mass, dim3((unsigned)(p.nch + 3) / 4, (unsigned)p.nrows), dim3(VT), 0, st, p);
         IFH_LAUNCH_CHECK("verify mass");
     }
-    hipLaunchKernelGGL(k_verify_draw, dim3((unsigned)p.nrows), dim3(VC_THREADS), 0, st, p);
+    hipLaunchKernelGGL(k_verify_draw, dim3((unsigned)p.nrows), dim3(VT), 0, st, p);
     IFH_LAUNCH_CHECK("verify draw");
     return IFH_OK;
 }
@@ -413,7 +447,7 @@ extern "C" int ifh_verify_drafts_topk(const int32_t *cand, const float *probs, c
     IFH_CHECK_ARG(ndraft >= 0 && ndraft <= 63);
     IFH_CHECK_ARG(cand && probs && uniform && out_tokens && out_count && (drafts || ndraft == 0));
     IFH_CHECK_ARG((draft_cand == nullptr) == (draft_probs == nullptr));
-    hipLaunchKernelGGL(k_verify_topk, dim3((unsigned)nrows), dim3(64), 0, as_stream(stream), cand, probs, draft_cand, draft_probs, drafts, lens,
+    hipLaunchKernelGGL(k_verify_topk, dim3((unsigned)nrows), dim3(VT), 0, as_stream(stream), cand, probs, draft_cand, draft_probs, drafts, lens,
                        uniform, ndraft, out_tokens, out_count);
     IFH_LAUNCH_CHECK("verify topk");
     return IFH_OK;
