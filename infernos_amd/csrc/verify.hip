@@ -15,7 +15,8 @@
 namespace ifh {
 
 constexpr int VT = 256, VPL = 32, VC = 64 * VPL;        // threads, logits a lane, logits a chunk (a wave's)
-constexpr int kVerifyMaxChunks = VT;                    // 524 288 tokens: the draw gives each chunk a thread
+constexpr int VM = 512, VD = 1024;                      // threads of the mass and the draw launch: 8 and 16 positions' verdicts at a time
+constexpr int kVerifyMaxChunks = 256;                   // 524 288 tokens: the draw gives each chunk a thread
 constexpr float kFltMax = 3.402823466e38f;
 
 // e^x for x <= 0 in f64, relative error below 1e-10: x = k ln 2 + r, |r| <= ln 2 / 2 (k by adding and taking off 1.5 2^52), the Taylor
@@ -78,11 +79,48 @@ __device__ __forceinline__ void load_chunk(const float *row, int base, int lane,
     }
 }
 
-__device__ __forceinline__ double wave_sum_d(double v)
+// Scans over the lanes of a wave as DPP operands (shifts by 1, 2, 4, 8 within 16 lanes, then lane 15 of rows 0 and 2 and lane 31 handed
+// on): a ds_bpermute step of 64 bits costs two LDS round trips, and the draw is a chain of such scans.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_d(double v)
 {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xF, true);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, ROWS, 0xF, true);
+    return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
+__device__ __forceinline__ double wave_scan_d(double v)
+{
+    v += dpp_d<0x111, 0xF>(v);
+    v += dpp_d<0x112, 0xF>(v);
+    v += dpp_d<0x114, 0xF>(v);
+    v += dpp_d<0x118, 0xF>(v);
+    v += dpp_d<0x142, 0xA>(v);
+    v += dpp_d<0x143, 0xC>(v);
     return v;
+}
+__device__ __forceinline__ double lane63_d(double v)
+{
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, 63), hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), 63);
+    return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
+__device__ __forceinline__ double wave_sum_d(double v) { return lane63_d(wave_scan_d(v)); }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp_max(float v)
+{
+    const int ninf = (int)0xff800000;
+    return fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(ninf, __builtin_bit_cast(int, v), CTRL, ROWS, 0xF, false)));
+}
+__device__ __forceinline__ float wave_max_f(float v)
+{
+    v = dpp_max<0x111, 0xF>(v);
+    v = dpp_max<0x112, 0xF>(v);
+    v = dpp_max<0x114, 0xF>(v);
+    v = dpp_max<0x118, 0xF>(v);
+    v = dpp_max<0x142, 0xA>(v);
+    v = dpp_max<0x143, 0xC>(v);
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
 __global__ __launch_bounds__(VT) void k_verify_stats(const VerifyParams p)
@@ -98,7 +136,7 @@ __global__ __launch_bounds__(VT) void k_verify_stats(const VerifyParams p)
         v[e] = logit(v[e]);
         m = fmaxf(m, v[e]);
     }
-    m = wave_max(m);
+    m = wave_max_f(m);
     double s = 0.0;
     if (p.greedy) {
         int at = 0x7fffffff;                                 // the first place of the maximum
@@ -137,11 +175,11 @@ struct VerdictLds {
     int best[64], keep[64];
 };
 
-__device__ __forceinline__ Verdict verdict_of(const VerifyParams &p, int r, VerdictLds &L)
+template <int NT> __device__ __forceinline__ Verdict verdict_of(const VerifyParams &p, int r, VerdictLds &L)
 {
     const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
     const int n = p.lens ? min(max(p.lens[r], 0), p.T) : p.T;
-    for (int i = wid; i <= n; i += VT / 64) {
+    for (int i = wid; i <= n; i += NT / 64) {
         const int64_t pos = (int64_t)r * (p.T + 1) + i;
         const int x = i < n ? p.drafts[(int64_t)r * p.T + i] : -1;
         const bool in = x >= 0 && x < p.vocab;
@@ -157,7 +195,7 @@ __device__ __forceinline__ Verdict verdict_of(const VerifyParams &p, int r, Verd
             cs[k] = c < p.nch ? p.csum[pos * p.nch + c] : 0.0;
             m = fmaxf(m, cm[k]);
         }
-        m = wave_max(m);
+        m = wave_max_f(m);
         const bool any = m > -INFINITY;
         double s = 0.0;
         int best = 0x7fffffff;
@@ -193,11 +231,11 @@ __device__ __forceinline__ Verdict verdict_of(const VerifyParams &p, int r, Verd
     return w;
 }
 
-__global__ __launch_bounds__(VT) void k_verify_mass(const VerifyParams p)
+__global__ __launch_bounds__(VM) void k_verify_mass(const VerifyParams p)
 {
     __shared__ VerdictLds L;
-    const int r = blockIdx.y, lane = threadIdx.x & 63, c = blockIdx.x * 4 + (threadIdx.x >> 6), base = c * VC;
-    const Verdict w = verdict_of(p, r, L);
+    const int r = blockIdx.y, lane = threadIdx.x & 63, c = blockIdx.x * (VM / 64) + (threadIdx.x >> 6), base = c * VC;
+    const Verdict w = verdict_of<VM>(p, r, L);
     if (c >= p.nch || !w.refused || !(w.s > 0.0)) return;
     float v[VPL], q[VPL];
     load_chunk(p.logits + ((int64_t)r * (p.T + 1) + w.kept) * p.ld, base, lane, p.vocab, p.vec, -INFINITY, v);
@@ -218,95 +256,97 @@ __global__ __launch_bounds__(VT) void k_verify_mass(const VerifyParams p)
     if (lane == 0) p.mass[(int64_t)r * p.nch + c] = s;
 }
 
-// inclusive sums over the workgroup's threads, in thread order
-__device__ __forceinline__ double block_scan(double v, double (&part)[VT / 64])
+// inclusive sums over the workgroup's threads, in thread order, and the whole
+__device__ __forceinline__ double block_scan(double v, double (&part)[VD / 64], double *all)
 {
     const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const double b = __shfl_up(v, o, 64);
-        if (lane >= o) v += b;
-    }
+    v = wave_scan_d(v);
     if (lane == 63) part[wid] = v;
     __syncthreads();
-    double before = 0.0;
+    double before = 0.0, a = 0.0;
 #pragma unroll
-    for (int w = 0; w < VT / 64; w++) before += w < wid ? part[w] : 0.0;
+    for (int w = 0; w < VD / 64; w++) {
+        if (w == wid) before = a;
+        a += part[w];
+    }
+    *all = a;
     return before + v;
 }
 
-__global__ __launch_bounds__(VT) void k_verify_draw(const VerifyParams p)
+__global__ __launch_bounds__(VD) void k_verify_draw(const VerifyParams p)
 {
     __shared__ VerdictLds L;
-    __shared__ double part[3][VT / 64], scut[2], without;
+    __shared__ double part[4][VD / 64], cut;
     __shared__ int first[2], last;
     const int r = blockIdx.x, tid = threadIdx.x;
-    const Verdict w = verdict_of(p, r, L);
+    constexpr int E = VC / VD;
+    if (tid < 2) first[tid] = 0x7fffffff;
+    if (tid == 2) last = -1;
+    const double u = (double)p.uniform[(int64_t)r * (p.T + 1) + p.T];
+    const Verdict w = verdict_of<VD>(p, r, L);
     int token = -1;
     if (p.greedy) token = w.best;
     else if (w.s > 0.0) {
-        const int64_t pos = (int64_t)r * (p.T + 1) + w.kept;
-        const float *row = p.logits + pos * p.ld, *qrow = p.q && w.refused ? p.q + ((int64_t)r * p.T + w.kept) * p.q_ld : nullptr;
-        const int x = w.refused && !p.q ? p.drafts[(int64_t)r * p.T + w.kept] : -1;      // a looked-up draft: everything but itself is left over
-        const double inv_s = 1.0 / w.s, u = (double)p.uniform[(int64_t)r * (p.T + 1) + p.T];
-        auto e_at = [&](int j) { return exp_neg(((double)logit(row[j]) - (double)w.m) * p.inv_temp); };
-        if (tid < 2) first[tid] = 0x7fffffff;
-        if (tid == 2) last = -1;
+        const int64_t pos = (int64_t)r * (p.T + 1) + w.kept, qpos = (int64_t)r * p.T + w.kept;
+        const float *row = p.logits + pos * p.ld, *qrow = p.q && w.refused ? p.q + qpos * p.q_ld : nullptr;
+        // a looked-up draft that was refused: everything but itself is left over
+        int x = w.refused && !p.q ? p.drafts[qpos] : -1;
+        if (x >= p.vocab) x = -1;
+        const double inv_s = 1.0 / w.s, md = (double)w.m;
         // a thread a chunk: mass of p (in units of the sum), and with a draft's distribution what p has over it
-        double pm = 0.0;
-        if (tid < p.nch) pm = p.csum[pos * p.nch + tid] * exp_neg(((double)fmaxf(p.cmax[pos * p.nch + tid], -kFltMax) - (double)w.m) * p.inv_temp);
-        double cm = pm;
-        bool rest = false;
-        if (x >= 0 && x < p.vocab) {                          // the draft's own chunk again, without it
-            const int base = x / VC * VC;
-            double s = 0.0;
-            for (int e = tid; e < VC; e += VT)
-                if (base + e < p.vocab && base + e != x) s += e_at(base + e);
-            const double t = block_scan(s, part[2]);
-            if (tid == VT - 1) without = t;
-            __syncthreads();
-            if (tid == x / VC) cm = without;
-            rest = true;
-        } else if (qrow) {
-            if (tid < p.nch) cm = p.mass[(int64_t)r * p.nch + tid];
-            rest = true;
+        const bool mine = tid < p.nch;
+        const float cmx = mine ? p.cmax[pos * p.nch + tid] : -INFINITY;
+        const double csm = mine ? p.csum[pos * p.nch + tid] : 0.0, left = mine && qrow ? p.mass[(int64_t)r * p.nch + tid] : 0.0;
+        float xv[E];
+        if (x >= 0) {                                         // the draft's own chunk, without it
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                const int j = x / VC * VC + e * VD + tid;
+                xv[e] = j < p.vocab && j != x ? row[j] : -INFINITY;
+            }
         }
-        __syncthreads();
-        double cum = block_scan(tid < p.nch ? cm : 0.0, part[0]);
-        if (tid == VT - 1) scut[0] = cum;
-        __syncthreads();
-        if (rest && !(scut[0] > 0.0)) {                       // nothing is left over: the token comes from p
+        const double pm = csm * exp_neg(((double)fmaxf(cmx, -kFltMax) - md) * p.inv_temp);
+        double cm = qrow ? left : pm, total;
+        if (x >= 0) {
+            double s = 0.0, without;
+#pragma unroll
+            for (int e = 0; e < E; e++) s += exp_neg(((double)logit(xv[e]) - md) * p.inv_temp);
+            block_scan(s, part[3], &without);
+            if (tid == x / VC) cm = without;
+        }
+        bool rest = qrow || x >= 0;
+        double cum = block_scan(cm, part[0], &total);
+        if (rest && !(total > 0.0)) {                         // nothing is left over: the token comes from p
             rest = false;
             cm = pm;
-            __syncthreads();
-            cum = block_scan(tid < p.nch ? cm : 0.0, part[1]);
-            if (tid == VT - 1) scut[0] = cum;
-            __syncthreads();
+            cum = block_scan(cm, part[1], &total);
         }
-        const double want = u * scut[0];
-        if (tid < p.nch && cum > want) atomicMin(&first[0], tid);
+        const double want = u * total;
+        // (one LDS atomic a wave: 1024 of them on one word cost 7 us)
+        const int lane = tid & 63;
+        const unsigned long long past = __ballot(mine && cum > want);
+        if (past && lane == __ffsll((long long)past) - 1) atomicMin(&first[0], tid);
         __syncthreads();
         const int c = min(first[0], p.nch - 1);
-        if (tid == c) scut[1] = cum - cm;
-        __syncthreads();
-        // the chunk's tokens, eight consecutive ones a thread
-        constexpr int E = VC / VT;
+        // the chunk's tokens, two consecutive ones a thread
         const int j0 = c * VC + tid * E;
-        double mass[E], mine = 0.0;
+        float lv[E], qv[E];
 #pragma unroll
         for (int e = 0; e < E; e++) {
-            const int j = j0 + e;
-            mass[e] = 0.0;
-            if (j < p.vocab) {
-                const double v = e_at(j);
-                if (rest && qrow) mass[e] = fmax(__builtin_fma(v, inv_s, -(double)qrow[j]), 0.0);
-                else if (!(rest && j == x)) mass[e] = v;
-            }
-            mine += mass[e];
+            lv[e] = j0 + e < p.vocab ? row[j0 + e] : -INFINITY;
+            qv[e] = rest && qrow && j0 + e < p.vocab ? qrow[j0 + e] : 0.0f;
         }
-        const double upto = scut[1] + block_scan(mine, part[2]);
+        if (tid == c) cut = cum - cm;
+        double mass[E], sum = 0.0, all;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            const double v = exp_neg(((double)logit(lv[e]) - md) * p.inv_temp);
+            mass[e] = rest && qrow ? fmax(__builtin_fma(v, inv_s, -(double)qv[e]), 0.0) : rest && j0 + e == x ? 0.0 : v;
+            sum += mass[e];
+        }
+        const double upto = block_scan(sum, part[2], &all) + cut;
         int at = -1, lastj = -1;
-        double a = upto - mine;
+        double a = upto - sum;
 #pragma unroll
         for (int e = 0; e < E; e++) {
             a += mass[e];
@@ -315,12 +355,13 @@ __global__ __launch_bounds__(VT) void k_verify_draw(const VerifyParams p)
                 if (at < 0 && a > want) at = j0 + e;
             }
         }
-        if (at >= 0) atomicMin(&first[1], at);
-        if (lastj >= 0) atomicMax(&last, lastj);
+        const unsigned long long hit = __ballot(at >= 0), some = __ballot(lastj >= 0);
+        if (hit && lane == __ffsll((long long)hit) - 1) atomicMin(&first[1], at);
+        if (some && lane == 63 - __clzll((long long)some)) atomicMax(&last, lastj);
         __syncthreads();
         token = first[1] != 0x7fffffff ? first[1] : last;     // (rounding past the chunk's end: its last token with any mass)
     }
-    for (int i = tid; i <= p.T; i += VT)
+    for (int i = tid; i <= p.T; i += VD)
         p.out_tokens[(int64_t)r * (p.T + 1) + i] = i < w.kept ? p.drafts[(int64_t)r * p.T + i] : i == w.kept ? token : -1;
     if (tid == 0) p.out_count[r] = w.kept + 1;
 }
@@ -430,10 +471,10 @@ extern "C" int ifh_verify_drafts_f32(const ifh_verify_desc *d, ifh_stream_t stre
     hipLaunchKernelGGL(k_verify_stats, dim3((unsigned)(p.nch + 3) / 4, (unsigned)positions), dim3(VT), 0, st, p);
     IFH_LAUNCH_CHECK("verify stats");
     if (!p.greedy && p.q && p.T > 0) {
-        hipLaunchKernelGGL(k_verify_mass, dim3((unsigned)(p.nch + 3) / 4, (unsigned)p.nrows), dim3(VT), 0, st, p);
+        hipLaunchKernelGGL(k_verify_mass, dim3((unsigned)(p.nch + VM / 64 - 1) / (VM / 64), (unsigned)p.nrows), dim3(VM), 0, st, p);
         IFH_LAUNCH_CHECK("verify mass");
     }
-    hipLaunchKernelGGL(k_verify_draw, dim3((unsigned)p.nrows), dim3(VT), 0, st, p);
+    hipLaunchKernelGGL(k_verify_draw, dim3((unsigned)p.nrows), dim3(VD), 0, st, p);
     IFH_LAUNCH_CHECK("verify draw");
     return IFH_OK;
 }
