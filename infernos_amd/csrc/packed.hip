@@ -92,7 +92,8 @@ struct RowsParams {
     int ntokens, nseqs, nh, nkv, G, T;
     float scale;
     KeySet ks[2];
-    int first;                             // workgroups of ks[0]; the others are ks[1]'s
+    int first, pairs;                      // workgroups of ks[0] (the others are ks[1]'s), and how many 256s of both are dealt in turn
+    int joint;                             // ks[1]'s workgroups go through ks[0]'s keys themselves and write out
     int64_t part_rows;                     // rows of one part (ntokens * nh)
     float *part_o, *part_ml;               // [parts][part_rows][hd] f32 unnormalised, [parts][part_rows][2] (max, sum); NULL: write out
 };
@@ -108,6 +109,22 @@ __device__ __forceinline__ float max_half(float m)
     float a;
     asm("v_max_f32 %0, %1, %2" : "=v"(a) : "v"(__uint_as_float(r.x)), "v"(__uint_as_float(r.y)));
     return a;
+}
+
+// the largest of a wave's values, in every lane (shifts within 16 lanes, then lane 15 of rows 0 and 2 and lane 31 handed on)
+template <int CTRL, int ROWS> __device__ __forceinline__ int dpp_max_i(int v)
+{
+    return max(v, __builtin_amdgcn_update_dpp((int)0x80000000, v, CTRL, ROWS, 0xF, false));
+}
+__device__ __forceinline__ int wave_max_i(int v)
+{
+    v = dpp_max_i<0x111, 0xF>(v);
+    v = dpp_max_i<0x112, 0xF>(v);
+    v = dpp_max_i<0x114, 0xF>(v);
+    v = dpp_max_i<0x118, 0xF>(v);
+    v = dpp_max_i<0x142, 0xA>(v);
+    v = dpp_max_i<0x143, 0xC>(v);
+    return __builtin_amdgcn_readlane(v, 63);
 }
 
 // 16 bytes a lane from BASE + VOFF (a lane's offset) to LDS address DST + 16 lane
@@ -159,7 +176,10 @@ struct WaveRows {
     {
 #pragma unroll
         for (int s = 0; s < NS; s++) qf[s] = __builtin_bit_cast(bf16x8_t, *reinterpret_cast<const uint4 *>(q + 16 * s + 8 * h2));
-        // (waited for here: left to hipcc the wait falls behind the next tile's DMA)
+    }
+    // (before the first tile is waited for: left to hipcc the wait for q falls behind the next tile's DMA)
+    __device__ __forceinline__ void wait_q()
+    {
 #pragma unroll
         for (int s = 0; s < NS; s++) asm volatile("" : : "v"(qf[s]));
     }
@@ -176,10 +196,11 @@ struct WaveRows {
             }
         }
     }
-    // scores -> unnormalised probabilities 2^(s c1 - ms); rel: keys of the tile this lane's row sees, minus 4 (lane / 32); first: the rows'
-    // first tile.  ms starts as the first tile's maximum (what a row sees is keys 0 .. lim - 1, so a row that sees anything of a range sees
-    // its first key) and is raised only when a later tile exceeds it by more than 8 (a wave decides at once): p stays below 2^8, sums in
-    // f32 lose nothing by it, and the rescaling of the accumulators is skipped for almost every tile.
+    // scores -> unnormalised probabilities 2^(s c1 - ms); rel: keys of the tile this lane's row sees, minus 4 (lane / 32); first: the wave's
+    // first tile of a range of keys.  ms starts as the maximum of the first tile that a row sees anything of (what it sees of a range is
+    // its keys up to lim, so the range's first tile or none) and is raised only when a later tile exceeds it by more than 8 (a wave
+    // decides at once): p stays below 2^8, sums in f32 lose nothing by it, and the rescaling of the accumulators is skipped for almost
+    // every tile.
     template <int NC> __device__ __forceinline__ void softmax(f32x16 (&s)[NC], bool mask, int rel, bool first)
     {
 #pragma unroll
@@ -203,8 +224,9 @@ struct WaveRows {
             }
         mx = max_half(fmaxf(mx, my));
         if (first || __any(mx > 8.0f)) {
-            const float raise = first ? (mx > -1e30f ? mx : 0.0f) : fmaxf(mx, 0.0f);
-            const float alpha = first ? 1.0f : __builtin_amdgcn_exp2f(-raise);
+            const bool unset = first && l + __shfl_xor(l, 32, 64) == 0.0f;
+            const float raise = unset ? (mx > -1e30f ? mx : 0.0f) : fmaxf(mx, 0.0f);
+            const float alpha = unset ? 1.0f : __builtin_amdgcn_exp2f(-raise);
             ms += raise;
             l *= alpha;
 #pragma unroll
@@ -274,10 +296,25 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(const RowsParams p)
     __shared__ __attribute__((aligned(1024))) unsigned char lds[BYTES];
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l32 = lane & 31, h2 = lane >> 5;
-    const bool second = !LONG && (int)blockIdx.x >= p.first;
+    // Two key sets: 256 workgroups of one, 256 of the other, so that a CU holds one that multiplies (a part of the prefix) beside one that
+    // waits for memory (own keys), then what is left of either.
+    bool second = false;
+    int wg = blockIdx.x;
+    if (!LONG && p.joint) second = true;
+    else if (!LONG) {
+        const int blk = wg >> 8;
+        if (blk < 2 * p.pairs) {
+            second = blk & 1;
+            wg = (blk >> 1) * 256 + (wg & 255);
+        } else {
+            wg -= p.pairs * 256;
+            second = wg >= p.first;
+            wg -= second ? p.first - p.pairs * 256 : 0;
+        }
+    }
     const KeySet &ks = p.ks[second ? 1 : 0];
     const bool narrow = !LONG && ks.narrow;
-    const int mode = LONG ? ROWS_PACKED : ks.mode, id = blockIdx.x - (second ? p.first : 0);
+    const int mode = LONG ? ROWS_PACKED : ks.mode, id = wg;
     // kv head, row block, part: neighbours on different XCDs, so that with 2, 4 or 8 kv heads an XCD's L2 holds its own heads' keys
     const int G = p.G, kvh = id % p.nkv, bp = id / p.nkv, part = bp / ks.blocks;
     const int rs = narrow ? 5 : 7, R = 1 << rs, KT = narrow ? kNarrowKeys : kWideKeys;       // rows of a block, keys of a tile
@@ -325,6 +362,8 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(const RowsParams p)
     const int n = n1 - n0, w0 = row0 + (narrow ? 0 : wid * 32), row = w0 + l32, t = row / G, g = row - t * G;
     const bool ok = t < n;
     const int tok = n0 + (ok ? t : 0), head = kvh * G + (ok ? g : 0);
+    WaveRows<HD> w;
+    w.load_q(p.q + (int64_t)tok * p.q_ts + (int64_t)head * HD, h2);       // in flight while the limits are looked up
     int lim, wmax, wmin, kmax;                                 // keys this lane's row sees; most and fewest of the wave's rows; most of the block's
     if (mode == ROWS_PACKED) {
         const int past = klen - n + 1;
@@ -334,13 +373,8 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(const RowsParams p)
         kmax = max(past + min((row0 + R - 1) / G, n - 1), 0);
     } else {
         lim = !ok ? 0 : !ks.lim ? klen : min(max(ks.lim[mode == ROWS_PREFIX ? tok / p.T : tok], 0), klen);
-        wmax = lim;
-        wmin = ok ? lim : klen;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            wmax = max(wmax, __shfl_xor(wmax, o, 64));
-            wmin = min(wmin, __shfl_xor(wmin, o, 64));
-        }
+        wmax = wave_max_i(lim);
+        wmin = -wave_max_i(ok ? -lim : -klen);
         kmax = wmax;
         if (!narrow) {
             int *smax = reinterpret_cast<int *>(lds);
@@ -359,11 +393,9 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(const RowsParams p)
         kt1 = min(kt1, kt0 + ks.part_tiles);
     }
 
-    WaveRows<HD> w;
     w.init(p.scale, lane);
-    const uint16_t *qrow = p.q + (int64_t)tok * p.q_ts + (int64_t)head * HD;
     const unsigned lbase = (unsigned)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)lds);
-    const unsigned ts2 = (unsigned)ks.ts * 2u;
+    unsigned ts2 = (unsigned)ks.ts * 2u;
     const unsigned char *ksrc = reinterpret_cast<const unsigned char *>(ks.kv + (int64_t)kbatch * ks.bs + (int64_t)kvh * HD);
     const unsigned char *vsrc = ksrc + (int64_t)p.v_off * 2;
     const int64_t pr = (int64_t)(ks.part0 + part) * p.part_rows;
@@ -409,7 +441,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(const RowsParams p)
 #undef ROWS_ST
         };
         if (kt0 < kt1) issue(kt0);
-        w.load_q(qrow, h2);
+        w.wait_q();
         if (wmax == 0)                                         // a wave without rows, or whose rows see nothing: brings its pieces only
             for (int kt = kt0; kt < kt1; kt++) {
                 asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -473,30 +505,44 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(const RowsParams p)
             ROWS_DMA((unsigned)min(r, left) * ts2 + c, src, dst + j * 1024);
         }
     };
-    int kt = kt0 + wid;
-    if (kt < kt1) {
-        issue(kt, ksrc, kdst, false);
-        issue(kt, vsrc, vdst, true);
-    }
-    w.load_q(qrow, h2);
     const unsigned char *kbuf = lds + wid * (2 * NTILE), *vbuf = kbuf + NTILE;
-    for (; kt < kt1; kt += 4) {
-        const bool more = kt + 4 < kt1;
-        const int kbase = kt * kNarrowKeys;
-        f32x16 s[1];
-        // (own DMA only, counted in order: K of this tile is behind V of this tile, which is behind K of the next)
-        if (PIECES == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
-        else asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
-        w.scores(kbuf, s);
-        asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(s[0]) : : "memory");       // the tile's keys have been read
-        if (more) issue(kt + 4, ksrc, kdst, false);
-        w.softmax(s, kbase + kNarrowKeys > wmin, lim - kbase - 4 * h2, kt == kt0 + wid);
-        if (!more) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        else if (PIECES == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
-        else asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
-        w.accumulate(vbuf, s);
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        if (more) issue(kt + 4, vsrc, vdst, true);
+    // (a joint workgroup goes through the prefix and then through its own keys)
+    for (int pass = p.joint ? 0 : 1; pass < 2; pass++) {
+        const bool pre = pass == 0;
+        if (p.joint) {
+            const KeySet &k0 = p.ks[0];
+            const int64_t off = (int64_t)kvh * HD;
+            ts2 = (unsigned)(pre ? k0.ts : ks.ts) * 2u;
+            ksrc = reinterpret_cast<const unsigned char *>(pre ? k0.kv + off : ks.kv + (int64_t)kbatch * ks.bs + off);
+            vsrc = ksrc + (int64_t)p.v_off * 2;
+            kmax = pre ? (k0.lim ? min(max(k0.lim[kbatch], 0), k0.max_keys) : k0.max_keys) : wmax;
+            kt1 = (kmax + kNarrowKeys - 1) / kNarrowKeys;
+        }
+        const int plim = pre ? kmax : lim, pmin = pre ? kmax : wmin;
+        int kt = kt0 + wid;
+        if (kt < kt1) {
+            issue(kt, ksrc, kdst, false);
+            issue(kt, vsrc, vdst, true);
+        }
+        w.wait_q();
+        for (; kt < kt1; kt += 4) {
+            const bool more = kt + 4 < kt1;
+            const int kbase = kt * kNarrowKeys;
+            f32x16 s[1];
+            // (own DMA only, counted in order: K of this tile is behind V of this tile, which is behind K of the next)
+            if (PIECES == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+            else asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+            w.scores(kbuf, s);
+            asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(s[0]) : : "memory");       // the tile's keys have been read
+            if (more) issue(kt + 4, ksrc, kdst, false);
+            w.softmax(s, kbase + kNarrowKeys > pmin, plim - kbase - 4 * h2, kt == kt0 + wid);
+            if (!more) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            else if (PIECES == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+            else asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+            w.accumulate(vbuf, s);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            if (more) issue(kt + 4, vsrc, vdst, true);
+        }
     }
     w.finish();
     __syncthreads();                                           // the tiles are no longer read
@@ -720,6 +766,13 @@ static bool prefix_fits(int64_t ntokens, int64_t nheads, int64_t nkv)
     return ntokens < (1 << 24) && ntokens * (nheads / nkv) < (1ll << 30) && (ntokens * (nheads / nkv) / kNarrowRows + ntokens + 1) * nkv < (1ll << 24);
 }
 
+// A short prefix is not worth a launch to share it: up to 768 keys in all (six tiles a wave) and two workgroups a CU, the workgroup of a
+// row's own keys reads the prefix too (from L2) and writes the result.  Two rows behind 333 keys: TODO_JOINT.
+static bool prefix_joint(int64_t workgroups, int prefix_keys, int max_keys, bool narrow)
+{
+    return narrow && (int64_t)prefix_keys + max_keys <= 768 && workgroups <= 2 * (int64_t)device_cu_count_physical();
+}
+
 static void prefix_plan(int64_t nrows, int64_t T, int prefix_keys, int nheads, int nkv, int max_keys, KeySet *prefix, KeySet *own)
 {
     const int64_t r = T * (nheads / nkv), all = nrows * r;
@@ -760,11 +813,18 @@ extern "C" int ifh_attn_prefix_bf16(const ifh_attn_prefix_desc *d, ifh_stream_t 
     p.part_rows = ntokens * d->nheads;
     const int parts = a.parts + b.parts;
     IFH_CHECK_ARG(d->ws_floats >= part_floats(p.part_rows, parts, d->head_dim));
+    hipStream_t st = as_stream(stream);
+    if (prefix_joint((int64_t)b.blocks * p.nkv, d->prefix_keys, d->max_keys, b.narrow)) {
+        p.joint = 1;
+        rows_launch(p, d->head_dim, (int64_t)b.blocks * p.nkv, st);
+        IFH_LAUNCH_CHECK("attn_prefix joint");
+        return IFH_OK;
+    }
     p.part_o = d->ws;
     p.part_ml = d->ws + p.part_rows * parts * d->head_dim;
     const int64_t na = (int64_t)a.blocks * p.nkv * a.parts, nb = (int64_t)b.blocks * p.nkv * b.parts;
     p.first = (int)na;
-    hipStream_t st = as_stream(stream);
+    p.pairs = (int)((na < nb ? na : nb) / 256);
     rows_launch(p, d->head_dim, na + nb, st);
     IFH_LAUNCH_CHECK("attn_prefix");
     join_launch(p, d->head_dim, parts, st);
