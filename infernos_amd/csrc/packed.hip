@@ -6,6 +6,8 @@
 //   k_attn_join      joins the partial results of row blocks whose keys were split.
 #include "common.h"
 
+#include <type_traits>
+
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -128,12 +130,8 @@ __device__ __forceinline__ int wave_max_i(int v)
 }
 
 // 16 bytes a lane from BASE + VOFF (a lane's offset) to LDS address DST + 16 lane
-#define ROWS_DMA(VOFF, BASE, DST)                                                                                          \
-    do {                                                                                                                   \
-        unsigned keep_;                                                                                                    \
-        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0" \
-                     : "=&s"(keep_) : "v"(VOFF), "s"(BASE), "s"(DST) : "memory");                                          \
-    } while (0)
+#define ROWS_DMA(VOFF, BASE, DST) \
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(VOFF), "s"(BASE), "s"(DST) : "memory", "m0")
 
 // The keys of a tile in LDS.  Rows are unpadded (the DMA writes 16 bytes a lane in a row), so the 16-byte chunks of key r are permuted on
 // the source side: K chunk c at c ^ (r % 16) (head_dim 64: c ^ (r / 2 % 8)), so that the 16 keys a ds_read_b128 reads at once lie in 16
@@ -183,17 +181,22 @@ struct WaveRows {
 #pragma unroll
         for (int s = 0; s < NS; s++) asm volatile("" : : "v"(qf[s]));
     }
-    // scores of NC x 32 keys at K tile kt
-    template <int NC> __device__ __forceinline__ void scores(const unsigned char *kt, f32x16 (&s)[NC])
+    // scores of NC x 32 keys at K tile kt: the key blocks in turn (a product waits for the one before it on the same accumulators), the
+    // fragments AHEAD products ahead; between(i) is called before product i
+    template <int NC, typename F> __device__ __forceinline__ void scores(const unsigned char *kt, f32x16 (&s)[NC], F between)
     {
+        constexpr int N = NC * NS, AHEAD = 4;
+        bf16x8_t kf[AHEAD];
+        auto frag = [&](int i) { return *reinterpret_cast<const bf16x8_t *>(kt + ka[i / NC] + (i % NC) * 32 * ROWB); };
 #pragma unroll
-        for (int c = 0; c < NC; c++) {
-            s[c] = (f32x16){0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        for (int c = 0; c < NC; c++) s[c] = (f32x16){0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int d = 0; d < NS; d++) {
-                const bf16x8_t kf = *reinterpret_cast<const bf16x8_t *>(kt + ka[d] + c * 32 * ROWB);
-                s[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[d], s[c], 0, 0, 0);
-            }
+        for (int i = 0; i < AHEAD; i++) kf[i] = frag(i);
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            between(i);
+            s[i % NC] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[i % AHEAD], qf[i / NC], s[i % NC], 0, 0, 0);
+            if (i + AHEAD < N) kf[i % AHEAD] = frag(i + AHEAD);
         }
     }
     // scores -> unnormalised probabilities 2^(s c1 - ms); rel: keys of the tile this lane's row sees, minus 4 (lane / 32); first: the wave's
@@ -254,12 +257,24 @@ struct WaveRows {
         l += __shfl_xor(l, 32, 64);
         ms = l > 0.0f ? ms : -1e30f;
     }
-    // O^T += V^T P^T, V tile vt
-    template <int NC> __device__ __forceinline__ void accumulate(const unsigned char *vt, const f32x16 (&s)[NC])
+    // O^T += V^T P^T, V tile vt; v: the fragments of its first 16 keys, read before the softmax
+    __device__ __forceinline__ void values(const unsigned char *vt, int kk, bf16x8_t (&v)[ND])
+    {
+        typedef __attribute__((address_space(3))) bf16x4_t *lds4;
+#pragma unroll
+        for (int d = 0; d < ND; d++) {
+            const bf16x4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(vt + va[d] + kk * 16 * ROWB));
+            const bf16x4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(vt + va[d] + (kk * 16 + 8) * ROWB));
+            v[d] = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+    }
+    template <int NC> __device__ __forceinline__ void accumulate(const unsigned char *vt, const f32x16 (&s)[NC], bf16x8_t (&v)[ND])
     {
 #pragma unroll
         for (int kk = 0; kk < 2 * NC; kk++) {
             const int c = kk >> 1, e0 = (kk & 1) * 8;
+            bf16x8_t next[ND];
+            if (kk + 1 < 2 * NC) values(vt, kk + 1, next);
             uint4 pb;
             pb.x = f32x2_to_bf16x2(s[c][e0], s[c][e0 + 1]);
             pb.y = f32x2_to_bf16x2(s[c][e0 + 2], s[c][e0 + 3]);
@@ -267,12 +282,10 @@ struct WaveRows {
             pb.w = f32x2_to_bf16x2(s[c][e0 + 6], s[c][e0 + 7]);
             const bf16x8_t pf = __builtin_bit_cast(bf16x8_t, pb);
 #pragma unroll
-            for (int d = 0; d < ND; d++) {
-                typedef __attribute__((address_space(3))) bf16x4_t *lds4;
-                const bf16x4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(vt + va[d] + kk * 16 * ROWB));
-                const bf16x4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(vt + va[d] + (kk * 16 + 8) * ROWB));
-                const bf16x8_t vf = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf, o[d], 0, 0, 0);
+            for (int d = 0; d < ND; d++) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[d], pf, o[d], 0, 0, 0);
+            if (kk + 1 < 2 * NC) {
+#pragma unroll
+                for (int d = 0; d < ND; d++) v[d] = next[d];
             }
         }
     }
@@ -402,64 +415,55 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(const RowsParams p)
 
     if (!narrow) {
         // DMA: piece j of wave w brings keys (4 j + w) PK .. + PK - 1 of the tile (the permutation of a chunk is the same in every piece);
-        // lane l -> key l / CH of the piece, LDS chunk l % CH.  All of a tile in one asm block: LDS addresses step through m0 4 KB at a time.
+        // lane l -> key l / CH of the piece, LDS chunk l % CH.  The pieces of the next tile go out one by one between the products of this
+        // one's scores: eight in a row hold a wave up for 500 clocks, with the matrix unit idle.
         constexpr int PIECES = WTILE / 4096;
         const int drow = wid * PK + lane / CH, dpos = lane % CH;
         const unsigned kch = (unsigned)(dpos ^ kperm<HD>(drow)) * 16u, vch = (unsigned)(dpos ^ vperm<HD>(drow)) * 16u;
         unsigned ro[PIECES];
 #pragma unroll
         for (int j = 0; j < PIECES; j++) ro[j] = (unsigned)(drow + j * 4 * PK) * ts2;
-        auto issue = [&](int kt) {
-            const unsigned dst = lbase + (unsigned)(kt & 1) * (2 * WTILE) + (unsigned)wid * 1024u;
-            const int64_t off = (int64_t)kt * kWideKeys * (int64_t)ts2;
-            const int left = kmax - 1 - kt * kWideKeys;        // the last key of the block, relative to the tile
-            unsigned r[PIECES], keep;
-            if (left >= kWideKeys - 1) {
-#pragma unroll
-                for (int j = 0; j < PIECES; j++) r[j] = ro[j];
-            } else {                                           // past the end: the last key again, masked below
-#pragma unroll
-                for (int j = 0; j < PIECES; j++) r[j] = (unsigned)min(drow + j * 4 * PK, left) * ts2;
-            }
-#define ROWS_LD(V, S) "global_load_lds_dwordx4 " V ", " S "\n\t"
-#define ROWS_ST "s_add_u32 m0, m0, 0x1000\n\ts_nop 0\n\t"
-            if constexpr (PIECES == 4)
-                asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %11\n\ts_nop 0\n\t" ROWS_LD("%1", "%9") ROWS_ST ROWS_LD("%2", "%9") ROWS_ST
-                                 ROWS_LD("%3", "%9") ROWS_ST ROWS_LD("%4", "%9") ROWS_ST ROWS_LD("%5", "%10") ROWS_ST ROWS_LD("%6", "%10") ROWS_ST
-                                     ROWS_LD("%7", "%10") ROWS_ST ROWS_LD("%8", "%10") "s_mov_b32 m0, %0"
-                             : "=&s"(keep)
-                             : "v"(r[0] + kch), "v"(r[1] + kch), "v"(r[2] + kch), "v"(r[3 % PIECES] + kch), "v"(r[0] + vch), "v"(r[1] + vch),
-                               "v"(r[2 % PIECES] + vch), "v"(r[3 % PIECES] + vch), "s"(ksrc + off), "s"(vsrc + off), "s"(dst)
-                             : "memory", "scc");
-            else
-                asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %7\n\ts_nop 0\n\t" ROWS_LD("%1", "%5") ROWS_ST ROWS_LD("%2", "%5") ROWS_ST
-                                 ROWS_LD("%3", "%6") ROWS_ST ROWS_LD("%4", "%6") "s_mov_b32 m0, %0"
-                             : "=&s"(keep)
-                             : "v"(r[0] + kch), "v"(r[1] + kch), "v"(r[0] + vch), "v"(r[1] + vch), "s"(ksrc + off), "s"(vsrc + off), "s"(dst)
-                             : "memory", "scc");
-#undef ROWS_LD
-#undef ROWS_ST
+        // piece j of K (j < PIECES) or V of tile kt; past the end of the block's keys: the last key again, masked below
+        auto piece = [&](int kt, int j) {
+            const bool v = j >= PIECES;
+            const int jj = v ? j - PIECES : j;
+            const unsigned end = (unsigned)min(kmax - 1 - kt * kWideKeys, kWideKeys - 1) * ts2;
+            const unsigned dst = lbase + (unsigned)(kt & 1) * (2 * WTILE) + (unsigned)wid * 1024u + (unsigned)((v ? WTILE : 0) + jj * 4096);
+            ROWS_DMA(min(ro[jj], end) + (v ? vch : kch), (v ? vsrc : ksrc) + (int64_t)kt * kWideKeys * (int64_t)ts2, dst);
         };
-        if (kt0 < kt1) issue(kt0);
+        if (kt0 < kt1)
+#pragma unroll
+            for (int j = 0; j < 2 * PIECES; j++) piece(kt0, j);
         w.wait_q();
+        auto landed = [&]() {                                  // the tile has landed, and the other buffer is no longer read
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+        };
+        auto tile = [&](int kt, auto more) {
+            landed();
+            const int kbase = kt * kWideKeys;
+            const unsigned char *buf = lds + (kt & 1) * (2 * WTILE);
+            f32x16 s[2];
+            w.scores(buf, s, [&](int i) {
+                if constexpr (decltype(more)::value)
+                    if (i % 2 == 0) piece(kt + 1, i / 2);
+            });
+            bf16x8_t v[ND];
+            w.values(buf + WTILE, 0, v);
+            w.softmax(s, kbase + kWideKeys > wmin, lim - kbase - 4 * h2, kt == kt0);
+            w.accumulate(buf + WTILE, s, v);
+        };
         if (wmax == 0)                                         // a wave without rows, or whose rows see nothing: brings its pieces only
             for (int kt = kt0; kt < kt1; kt++) {
-                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-                __syncthreads();
-                if (kt + 1 < kt1) issue(kt + 1);
+                landed();
+                if (kt + 1 < kt1)
+#pragma unroll
+                    for (int j = 0; j < 2 * PIECES; j++) piece(kt + 1, j);
             }
-        else
-            for (int kt = kt0; kt < kt1; kt++) {
-                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-                __syncthreads();                               // the tile has landed, and the other buffer is no longer read
-                if (kt + 1 < kt1) issue(kt + 1);
-                const int kbase = kt * kWideKeys;
-                const unsigned char *buf = lds + (kt & 1) * (2 * WTILE);
-                f32x16 s[2];
-                w.scores(buf, s);
-                w.softmax(s, kbase + kWideKeys > wmin, lim - kbase - 4 * h2, kt == kt0);
-                w.accumulate(buf + WTILE, s);
-            }
+        else if (kt0 < kt1) {
+            for (int kt = kt0; kt + 1 < kt1; kt++) tile(kt, std::true_type{});
+            tile(kt1 - 1, std::false_type{});
+        }
         w.finish();
         const int64_t at = pr + (int64_t)tok * p.nh + head;
         if (p.part_o) {
@@ -532,14 +536,16 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(const RowsParams p)
             // (own DMA only, counted in order: K of this tile is behind V of this tile, which is behind K of the next)
             if (PIECES == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
             else asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
-            w.scores(kbuf, s);
+            w.scores(kbuf, s, [](int) {});
             asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(s[0]) : : "memory");       // the tile's keys have been read
             if (more) issue(kt + 4, ksrc, kdst, false);
             w.softmax(s, kbase + kNarrowKeys > pmin, plim - kbase - 4 * h2, kt == kt0 + wid);
             if (!more) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             else if (PIECES == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
             else asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
-            w.accumulate(vbuf, s);
+            bf16x8_t v[ND];
+            w.values(vbuf, 0, v);
+            w.accumulate(vbuf, s, v);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             if (more) issue(kt + 4, vsrc, vdst, true);
         }
