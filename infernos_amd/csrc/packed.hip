@@ -130,8 +130,12 @@ __device__ __forceinline__ int wave_max_i(int v)
 }
 
 // 16 bytes a lane from BASE + VOFF (a lane's offset) to LDS address DST + 16 lane
-#define ROWS_DMA(VOFF, BASE, DST) \
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(VOFF), "s"(BASE), "s"(DST) : "memory", "m0")
+#define ROWS_DMA(VOFF, BASE, DST)                                                                                          \
+    do {                                                                                                                   \
+        unsigned keep_;                                                                                                    \
+        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0" \
+                     : "=&s"(keep_) : "v"(VOFF), "s"(BASE), "s"(DST) : "memory");                                          \
+    } while (0)
 
 // The keys of a tile in LDS.  Rows are unpadded (the DMA writes 16 bytes a lane in a row), so the 16-byte chunks of key r are permuted on
 // the source side: K chunk c at c ^ (r % 16) (head_dim 64: c ^ (r / 2 % 8)), so that the 16 keys a ds_read_b128 reads at once lie in 16
