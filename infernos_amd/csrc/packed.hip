@@ -96,11 +96,13 @@ struct RowsParams {
     KeySet ks[2];
     int first, pairs;                      // workgroups of ks[0] (the others are ks[1]'s), and how many 256s of both are dealt in turn
     int joint;                             // ks[1]'s workgroups go through ks[0]'s keys themselves and write out
-    int64_t part_rows;                     // rows of one part (ntokens * nh)
-    float *part_o, *part_ml;               // [parts][part_rows][hd] f32 unnormalised, [parts][part_rows][2] (max, sum); NULL: write out
+    // Partial results, or NULL: write out.  The rows of a kv head (token G + head of the group) in tiles of 32, a tile as the accumulators
+    // hold it: part_o f32 [parts][nkv][row_tiles][hd / 4][32 rows][4], unnormalised; part_ml f32 [parts][nkv][row_tiles][32][2] (max, sum).
+    int row_tiles;
+    float *part_o, *part_ml;
 };
 
-constexpr int kWideRows = 128, kWideKeys = 64, kNarrowRows = 32, kNarrowKeys = 32;
+constexpr int kWideRows = 128, kNarrowRows = 32, kKeys = 32;
 
 // max over lanes l and l ^ 32, every lane gets it
 __device__ __forceinline__ float max_half(float m)
@@ -185,22 +187,20 @@ struct WaveRows {
 #pragma unroll
         for (int s = 0; s < NS; s++) asm volatile("" : : "v"(qf[s]));
     }
-    // scores of NC x 32 keys at K tile kt: the key blocks in turn (a product waits for the one before it on the same accumulators), the
-    // fragments AHEAD products ahead; between(i) is called before product i
-    template <int NC, typename F> __device__ __forceinline__ void scores(const unsigned char *kt, f32x16 (&s)[NC], F between)
+    // scores of the 32 keys of K tile kt, the fragments AHEAD products ahead; between(i) is called before product i
+    template <typename F> __device__ __forceinline__ void scores(const unsigned char *kt, f32x16 &s, F between)
     {
-        constexpr int N = NC * NS, AHEAD = 4;
+        constexpr int AHEAD = 4;
         bf16x8_t kf[AHEAD];
-        auto frag = [&](int i) { return *reinterpret_cast<const bf16x8_t *>(kt + ka[i / NC] + (i % NC) * 32 * ROWB); };
-#pragma unroll
-        for (int c = 0; c < NC; c++) s[c] = (f32x16){0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        auto frag = [&](int i) { return *reinterpret_cast<const bf16x8_t *>(kt + ka[i]); };
+        s = (f32x16){0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < AHEAD; i++) kf[i] = frag(i);
 #pragma unroll
-        for (int i = 0; i < N; i++) {
+        for (int i = 0; i < NS; i++) {
             between(i);
-            s[i % NC] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[i % AHEAD], qf[i / NC], s[i % NC], 0, 0, 0);
-            if (i + AHEAD < N) kf[i % AHEAD] = frag(i + AHEAD);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[i % AHEAD], qf[i], s, 0, 0, 0);
+            if (i + AHEAD < NS) kf[i % AHEAD] = frag(i + AHEAD);
         }
     }
     // scores -> unnormalised probabilities 2^(s c1 - ms); rel: keys of the tile this lane's row sees, minus 4 (lane / 32); first: the wave's
@@ -208,27 +208,21 @@ struct WaveRows {
     // its keys up to lim, so the range's first tile or none) and is raised only when a later tile exceeds it by more than 8 (a wave
     // decides at once): p stays below 2^8, sums in f32 lose nothing by it, and the rescaling of the accumulators is skipped for almost
     // every tile.
-    template <int NC> __device__ __forceinline__ void softmax(f32x16 (&s)[NC], bool mask, int rel, bool first)
+    __device__ __forceinline__ void softmax(f32x16 &s, bool mask, int rel, bool first)
     {
 #pragma unroll
-        for (int c = 0; c < NC; c++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) s[c][e] = __builtin_fmaf(s[c][e], c1, -ms);
+        for (int e = 0; e < 16; e++) s[e] = __builtin_fmaf(s[e], c1, -ms);
         if (mask) {
 #pragma unroll
-            for (int c = 0; c < NC; c++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) s[c][e] = c * 32 + 8 * (e >> 2) + (e & 3) < rel ? s[c][e] : -INFINITY;
+            for (int e = 0; e < 16; e++) s[e] = 8 * (e >> 2) + (e & 3) < rel ? s[e] : -INFINITY;
         }
         // (two chains: a maximum of three waits for the one before it)
-        float mx = fmaxf(s[0][0], s[0][1]), my = fmaxf(s[0][2], s[0][3]);
+        float mx = fmaxf(s[0], s[1]), my = fmaxf(s[2], s[3]);
 #pragma unroll
-        for (int c = 0; c < NC; c++)
-#pragma unroll
-            for (int e = c == 0 ? 4 : 0; e < 16; e += 4) {
-                mx = fmaxf(fmaxf(mx, s[c][e]), s[c][e + 1]);
-                my = fmaxf(fmaxf(my, s[c][e + 2]), s[c][e + 3]);
-            }
+        for (int e = 4; e < 16; e += 4) {
+            mx = fmaxf(fmaxf(mx, s[e]), s[e + 1]);
+            my = fmaxf(fmaxf(my, s[e + 2]), s[e + 3]);
+        }
         mx = max_half(fmaxf(mx, my));
         if (first || __any(mx > 8.0f)) {
             const bool unset = first && l + __shfl_xor(l, 32, 64) == 0.0f;
@@ -241,18 +235,14 @@ struct WaveRows {
 #pragma unroll
                 for (int e = 0; e < 16; e++) o[d][e] *= alpha;
 #pragma unroll
-            for (int c = 0; c < NC; c++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) s[c][e] -= raise;
+            for (int e = 0; e < 16; e++) s[e] -= raise;
         }
         float ls[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int c = 0; c < NC; c++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) {
-                s[c][e] = __builtin_amdgcn_exp2f(s[c][e]);
-                ls[e & 3] += s[c][e];
-            }
+        for (int e = 0; e < 16; e++) {
+            s[e] = __builtin_amdgcn_exp2f(s[e]);
+            ls[e & 3] += s[e];
+        }
         l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
     }
     // the sum over both lanes of a row; a row that saw nothing counts for nothing in a join
@@ -272,22 +262,22 @@ struct WaveRows {
             v[d] = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
         }
     }
-    template <int NC> __device__ __forceinline__ void accumulate(const unsigned char *vt, const f32x16 (&s)[NC], bf16x8_t (&v)[ND])
+    __device__ __forceinline__ void accumulate(const unsigned char *vt, const f32x16 &s, bf16x8_t (&v)[ND])
     {
 #pragma unroll
-        for (int kk = 0; kk < 2 * NC; kk++) {
-            const int c = kk >> 1, e0 = (kk & 1) * 8;
+        for (int kk = 0; kk < 2; kk++) {
+            const int e0 = kk * 8;
             bf16x8_t next[ND];
-            if (kk + 1 < 2 * NC) values(vt, kk + 1, next);
+            if (kk == 0) values(vt, 1, next);
             uint4 pb;
-            pb.x = f32x2_to_bf16x2(s[c][e0], s[c][e0 + 1]);
-            pb.y = f32x2_to_bf16x2(s[c][e0 + 2], s[c][e0 + 3]);
-            pb.z = f32x2_to_bf16x2(s[c][e0 + 4], s[c][e0 + 5]);
-            pb.w = f32x2_to_bf16x2(s[c][e0 + 6], s[c][e0 + 7]);
+            pb.x = f32x2_to_bf16x2(s[e0], s[e0 + 1]);
+            pb.y = f32x2_to_bf16x2(s[e0 + 2], s[e0 + 3]);
+            pb.z = f32x2_to_bf16x2(s[e0 + 4], s[e0 + 5]);
+            pb.w = f32x2_to_bf16x2(s[e0 + 6], s[e0 + 7]);
             const bf16x8_t pf = __builtin_bit_cast(bf16x8_t, pb);
 #pragma unroll
             for (int d = 0; d < ND; d++) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[d], pf, o[d], 0, 0, 0);
-            if (kk + 1 < 2 * NC) {
+            if (kk == 0) {
 #pragma unroll
                 for (int d = 0; d < ND; d++) v[d] = next[d];
             }
@@ -303,13 +293,13 @@ struct WaveRows {
 //           whose work is bringing the keys: 128 rows would leave three waves idle.
 // LONG: every workgroup is wide and its rows packed (known to hipcc: 4 % on a long prompt over the kernel that decides at run time)
 template <int HD, bool LONG>
-__global__ __launch_bounds__(256, 2) void k_attn_rows(const RowsParams p)
+__global__ __launch_bounds__(256, LONG ? 3 : 2) void k_attn_rows(const RowsParams p)
 {
     constexpr int ROWB = HD * 2, ND = HD / 32;
     constexpr int CH = HD / 8, PK = 1024 / ROWB;               // chunks of a key, keys of a DMA instruction
-    constexpr int WTILE = kWideKeys * ROWB, NTILE = kNarrowKeys * ROWB;
+    constexpr int TILE = kKeys * ROWB;
     constexpr int JROW = HD * 4 + 16, JWAVE = 32 * JROW;        // narrow: a wave's result in LDS, rows padded by one chunk
-    constexpr int BYTES = 4 * WTILE > 4 * JWAVE + 1024 ? 4 * WTILE : 4 * JWAVE + 1024;
+    constexpr int BYTES = LONG ? 4 * TILE : 8 * TILE > 4 * JWAVE + 1024 ? 8 * TILE : 4 * JWAVE + 1024;
     __shared__ __attribute__((aligned(1024))) unsigned char lds[BYTES];
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l32 = lane & 31, h2 = lane >> 5;
@@ -334,7 +324,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(const RowsParams p)
     const int mode = LONG ? ROWS_PACKED : ks.mode, id = wg;
     // kv head, row block, part: neighbours on different XCDs, so that with 2, 4 or 8 kv heads an XCD's L2 holds its own heads' keys
     const int G = p.G, kvh = id % p.nkv, bp = id / p.nkv, part = bp / ks.blocks;
-    const int rs = narrow ? 5 : 7, R = 1 << rs, KT = narrow ? kNarrowKeys : kWideKeys;       // rows of a block, keys of a tile
+    const int rs = narrow ? 5 : 7, R = 1 << rs;                // rows of a block
     static_assert(kNarrowRows == 32 && kWideRows == 128, "");
     int xb = bp - part * ks.blocks;
 
@@ -404,7 +394,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(const RowsParams p)
     wmax = __builtin_amdgcn_readfirstlane(wmax);
     wmin = __builtin_amdgcn_readfirstlane(wmin);
     kmax = __builtin_amdgcn_readfirstlane(kmax);
-    int kt0 = 0, kt1 = (kmax + KT - 1) / KT;
+    int kt0 = 0, kt1 = (kmax + kKeys - 1) / kKeys;
     if (p.part_o) {
         kt0 = part * ks.part_tiles;
         kt1 = min(kt1, kt0 + ks.part_tiles);
@@ -415,13 +405,13 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(const RowsParams p)
     unsigned ts2 = (unsigned)ks.ts * 2u;
     const unsigned char *ksrc = reinterpret_cast<const unsigned char *>(ks.kv + (int64_t)kbatch * ks.bs + (int64_t)kvh * HD);
     const unsigned char *vsrc = ksrc + (int64_t)p.v_off * 2;
-    const int64_t pr = (int64_t)(ks.part0 + part) * p.part_rows;
+    const int64_t pt = ((int64_t)(ks.part0 + part) * p.nkv + kvh) * p.row_tiles;        // first tile of this part and kv head
 
     if (!narrow) {
         // DMA: piece j of wave w brings keys (4 j + w) PK .. + PK - 1 of the tile (the permutation of a chunk is the same in every piece);
         // lane l -> key l / CH of the piece, LDS chunk l % CH.  The pieces of the next tile go out one by one between the products of this
         // one's scores: eight in a row hold a wave up for 500 clocks, with the matrix unit idle.
-        constexpr int PIECES = WTILE / 4096;
+        constexpr int PIECES = TILE / 4096;
         const int drow = wid * PK + lane / CH, dpos = lane % CH;
         const unsigned kch = (unsigned)(dpos ^ kperm<HD>(drow)) * 16u, vch = (unsigned)(dpos ^ vperm<HD>(drow)) * 16u;
         unsigned ro[PIECES];
@@ -431,9 +421,9 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(const RowsParams p)
         auto piece = [&](int kt, int j) {
             const bool v = j >= PIECES;
             const int jj = v ? j - PIECES : j;
-            const unsigned end = (unsigned)min(kmax - 1 - kt * kWideKeys, kWideKeys - 1) * ts2;
-            const unsigned dst = lbase + (unsigned)(kt & 1) * (2 * WTILE) + (unsigned)wid * 1024u + (unsigned)((v ? WTILE : 0) + jj * 4096);
-            ROWS_DMA(min(ro[jj], end) + (v ? vch : kch), (v ? vsrc : ksrc) + (int64_t)kt * kWideKeys * (int64_t)ts2, dst);
+            const unsigned end = (unsigned)min(kmax - 1 - kt * kKeys, kKeys - 1) * ts2;
+            const unsigned dst = lbase + (unsigned)(kt & 1) * (2 * TILE) + (unsigned)wid * 1024u + (unsigned)((v ? TILE : 0) + jj * 4096);
+            ROWS_DMA(min(ro[jj], end) + (v ? vch : kch), (v ? vsrc : ksrc) + (int64_t)kt * kKeys * (int64_t)ts2, dst);
         };
         if (kt0 < kt1)
 #pragma unroll
@@ -445,17 +435,17 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(const RowsParams p)
         };
         auto tile = [&](int kt, auto more) {
             landed();
-            const int kbase = kt * kWideKeys;
-            const unsigned char *buf = lds + (kt & 1) * (2 * WTILE);
-            f32x16 s[2];
+            const int kbase = kt * kKeys;
+            const unsigned char *buf = lds + (kt & 1) * (2 * TILE);
+            f32x16 s;
             w.scores(buf, s, [&](int i) {
                 if constexpr (decltype(more)::value)
                     if (i % 2 == 0) piece(kt + 1, i / 2);
             });
             bf16x8_t v[ND];
-            w.values(buf + WTILE, 0, v);
-            w.softmax(s, kbase + kWideKeys > wmin, lim - kbase - 4 * h2, kt == kt0);
-            w.accumulate(buf + WTILE, s, v);
+            w.values(buf + TILE, 0, v);
+            w.softmax(s, kbase + kKeys > wmin, lim - kbase - 4 * h2, kt == kt0);
+            w.accumulate(buf + TILE, s, v);
         };
         if (wmax == 0)                                         // a wave without rows, or whose rows see nothing: brings its pieces only
             for (int kt = kt0; kt < kt1; kt++) {
@@ -469,20 +459,21 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(const RowsParams p)
             tile(kt1 - 1, std::false_type{});
         }
         w.finish();
-        const int64_t at = pr + (int64_t)tok * p.nh + head;
         if (p.part_o) {
             if (!ok) return;
+            const int r = tok * G + g;
+            const int64_t at = (pt + (r >> 5)) * 32 + (r & 31);
             if (h2 == 0) *reinterpret_cast<float2 *>(p.part_ml + at * 2) = make_float2(w.ms, w.l);
-            float *po = p.part_o + at * HD + 4 * h2;
+            float *po = p.part_o + (pt + (r >> 5)) * (32 * HD) + ((r & 31) + 32 * h2) * 4;
 #pragma unroll
             for (int d = 0; d < ND; d++)
 #pragma unroll
                 for (int e = 0; e < 16; e += 4)
-                    *reinterpret_cast<float4 *>(po + 32 * d + 2 * e) = make_float4(w.o[d][e], w.o[d][e + 1], w.o[d][e + 2], w.o[d][e + 3]);
+                    *reinterpret_cast<float4 *>(po + (8 * d + e / 2) * 128) = make_float4(w.o[d][e], w.o[d][e + 1], w.o[d][e + 2], w.o[d][e + 3]);
             return;
         }
         // A lane holds dims 8 i + 4 (lane / 32) .. + 3 of its row: halves of neighbouring groups of eight are exchanged with lane ^ 32, so
-        // that a lane stores whole groups (16 bytes of bf16) and a row's two lanes 32 bytes in a row.
+        // that a lane stores whole groups (16 bytes of bf16) and a row's two lanes 32 bytes in a row.  (Whole rows by way of LDS: no gain.)
         const float inv = w.l > 0.0f ? 1.0f / w.l : 0.0f;
         uint16_t *op = p.out + (int64_t)tok * p.o_ts + (int64_t)head * HD + 8 * h2;
 #pragma unroll
@@ -500,12 +491,12 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(const RowsParams p)
     }
 
     // narrow: piece j brings keys j PK .. + PK - 1 of the wave's tile
-    constexpr int PIECES = NTILE / 1024;
-    const unsigned kdst = lbase + (unsigned)wid * (2 * NTILE), vdst = kdst + NTILE;
+    constexpr int PIECES = TILE / 1024;
+    const unsigned kdst = lbase + (unsigned)wid * (2 * TILE), vdst = kdst + TILE;
     const int drow = lane / CH, dpos = lane % CH;
     auto issue = [&](int kt, const unsigned char *src, unsigned dst, bool v) {
-        const int left = kmax - 1 - kt * kNarrowKeys;
-        src += (int64_t)kt * kNarrowKeys * (int64_t)ts2;
+        const int left = kmax - 1 - kt * kKeys;
+        src += (int64_t)kt * kKeys * (int64_t)ts2;
 #pragma unroll
         for (int j = 0; j < PIECES; j++) {
             const int r = drow + j * PK;
@@ -513,7 +504,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(const RowsParams p)
             ROWS_DMA((unsigned)min(r, left) * ts2 + c, src, dst + j * 1024);
         }
     };
-    const unsigned char *kbuf = lds + wid * (2 * NTILE), *vbuf = kbuf + NTILE;
+    const unsigned char *kbuf = lds + wid * (2 * TILE), *vbuf = kbuf + TILE;
     // (a joint workgroup goes through the prefix and then through its own keys)
     for (int pass = p.joint ? 0 : 1; pass < 2; pass++) {
         const bool pre = pass == 0;
@@ -524,7 +515,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(const RowsParams p)
             ksrc = reinterpret_cast<const unsigned char *>(pre ? k0.kv + off : ks.kv + (int64_t)kbatch * ks.bs + off);
             vsrc = ksrc + (int64_t)p.v_off * 2;
             kmax = pre ? (k0.lim ? min(max(k0.lim[kbatch], 0), k0.max_keys) : k0.max_keys) : wmax;
-            kt1 = (kmax + kNarrowKeys - 1) / kNarrowKeys;
+            kt1 = (kmax + kKeys - 1) / kKeys;
         }
         const int plim = pre ? kmax : lim, pmin = pre ? kmax : wmin;
         int kt = kt0 + wid;
@@ -535,15 +526,15 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(const RowsParams p)
         w.wait_q();
         for (; kt < kt1; kt += 4) {
             const bool more = kt + 4 < kt1;
-            const int kbase = kt * kNarrowKeys;
-            f32x16 s[1];
+            const int kbase = kt * kKeys;
+            f32x16 s;
             // (own DMA only, counted in order: K of this tile is behind V of this tile, which is behind K of the next)
             if (PIECES == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
             else asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
             w.scores(kbuf, s, [](int) {});
-            asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(s[0]) : : "memory");       // the tile's keys have been read
+            asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(s) : : "memory");       // the tile's keys have been read
             if (more) issue(kt + 4, ksrc, kdst, false);
-            w.softmax(s, kbase + kNarrowKeys > pmin, plim - kbase - 4 * h2, kt == kt0 + wid);
+            w.softmax(s, kbase + kKeys > pmin, plim - kbase - 4 * h2, kt == kt0 + wid);
             if (!more) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             else if (PIECES == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
             else asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
@@ -565,8 +556,9 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(const RowsParams p)
             *reinterpret_cast<float4 *>(lds + wid * JWAVE + l32 * JROW + (32 * d + 2 * e + 4 * h2) * 4) =
                 make_float4(w.o[d][e], w.o[d][e + 1], w.o[d][e + 2], w.o[d][e + 3]);
     __syncthreads();
-    // eight threads a row, each every eighth group of four dims
-    const int jr = tid >> 3, jt = (row0 + jr) / G, jg = row0 + jr - jt * G;
+    // eight threads a row, each every eighth group of four dims; neighbouring threads at neighbouring rows of a partial result's tile, or at
+    // neighbouring groups of a row
+    const int jr = p.part_o ? tid & 31 : tid >> 3, jq = p.part_o ? tid >> 5 : tid & 7, jt = (row0 + jr) / G, jg = row0 + jr - jt * G;
     if (jt >= n) return;
     float mj[4], wj[4], m = -1e30f, l = 0.0f;
 #pragma unroll
@@ -579,68 +571,104 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(const RowsParams p)
         wj[u] = __builtin_amdgcn_exp2f(mj[u] - m);
         l += sml[(u * 32 + jr) * 2 + 1] * wj[u];
     }
-    const int jtok = n0 + jt, jhead = kvh * G + jg;
-    const int64_t at = pr + (int64_t)jtok * p.nh + jhead;
-    if (p.part_o && (tid & 7) == 0) *reinterpret_cast<float2 *>(p.part_ml + at * 2) = make_float2(m, l);
+    const int jtok = n0 + jt, r = jtok * G + jg;
+    if (p.part_o && jq == 0) *reinterpret_cast<float2 *>(p.part_ml + ((pt + (r >> 5)) * 32 + (r & 31)) * 2) = make_float2(m, l);
     const float inv = l > 0.0f ? 1.0f / l : 0.0f;
 #pragma unroll
-    for (int d = (tid & 7) * 4; d < HD; d += 32) {
+    for (int q = jq; q < HD / 4; q += 8) {
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int u = 0; u < 4; u++) {
-            const float4 v = *reinterpret_cast<const float4 *>(lds + u * JWAVE + jr * JROW + d * 4);
+            const float4 v = *reinterpret_cast<const float4 *>(lds + u * JWAVE + jr * JROW + q * 16);
             a.x += v.x * wj[u]; a.y += v.y * wj[u]; a.z += v.z * wj[u]; a.w += v.w * wj[u];
         }
-        if (p.part_o) *reinterpret_cast<float4 *>(p.part_o + at * HD + d) = a;
+        if (p.part_o) *reinterpret_cast<float4 *>(p.part_o + (pt + (r >> 5)) * (32 * HD) + (q * 32 + (r & 31)) * 4) = a;
         else
-            *reinterpret_cast<uint2 *>(p.out + (int64_t)jtok * p.o_ts + (int64_t)jhead * HD + d) =
+            *reinterpret_cast<uint2 *>(p.out + (int64_t)jtok * p.o_ts + (int64_t)(kvh * G + jg) * HD + q * 4) =
                 make_uint2(f32x2_to_bf16x2(a.x * inv, a.y * inv), f32x2_to_bf16x2(a.z * inv, a.w * inv));
     }
 }
 
-// out = sum_j o_j 2^(m_j - m) / sum_j l_j 2^(m_j - m); a row is HD / 4 lanes.  Lane j of a row reads part j's (max, sum), so
-// that the weights cost one round trip; the partial rows come eight at a time.
-template <int HD>
-__global__ __launch_bounds__(256) void k_attn_join(const float *__restrict__ part_o, const float *__restrict__ part_ml, int64_t rows,
-                                                   int parts, uint16_t *__restrict__ out, int64_t o_ts, int nh)
+// out = sum_j o_j 2^(m_j - m) / sum_j l_j 2^(m_j - m) over the parts j, a workgroup 32 DG dims of a tile of 32 rows: thread (row, q) sums DG
+// groups of four dims (512 bytes in a row for 32 neighbours), eight loads in flight, and works out the weights of every eighth part.  The
+// result goes through LDS so that a row's dims are stored in a row.  DG: whole rows where there are tiles for the device, else 32 dims.
+constexpr int kMaxParts = 128;
+template <int HD, int DG>
+__global__ __launch_bounds__(256) void k_attn_join(const float *__restrict__ part_o, const float *__restrict__ part_ml, int row_tiles, int nkv,
+                                                   int parts, uint16_t *__restrict__ out, int64_t o_ts, int G, int rows)
 {
-    constexpr int L = HD / 4, U = 8;
-    const int64_t row = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
-    if (row >= rows) return;                                   // (whole rows: the exchanges below stay within a row's lanes)
-    const int li = threadIdx.x % L, d = li * 4;
+    constexpr int U = DG == 1 ? 16 : 8 / DG, KS = 4, OROW = 64 * DG + 16, CH = 4 * DG;
+    __shared__ float wts[kMaxParts][32], red[8][32], reds[8][32];
+    __shared__ __attribute__((aligned(16))) unsigned char tile[32 * OROW];
+    const int tt = blockIdx.x, d0 = blockIdx.y * 32, kvh = tt / row_tiles, r0 = (tt - kvh * row_tiles) * 32;
+    const int tid = threadIdx.x, row = tid & 31, q = tid >> 5;
+    const bool ok = r0 + row < rows;
+    const int64_t step = (int64_t)nkv * row_tiles;
+    const float *po = part_o + (int64_t)tt * (32 * HD) + ((d0 / 4 + q) * 32 + row) * 4;
+    float4 v[U][DG];
+    auto load = [&](int j, float4 (&x)[DG]) {
+#pragma unroll
+        for (int g = 0; g < DG; g++)
+            x[g] = ok && j < parts ? *reinterpret_cast<const float4 *>(po + j * step * (32 * HD) + g * 1024) : make_float4(0.f, 0.f, 0.f, 0.f);
+    };
+    auto stat = [&](int j) {
+        return ok ? *reinterpret_cast<const float2 *>(part_ml + ((j * step + tt) * 32 + row) * 2) : make_float2(-1e30f, 0.0f);
+    };
+#pragma unroll
+    for (int u = 0; u < U; u++) load(u, v[u]);                 // (on their way while the weights are worked out)
     float m = -1e30f;
-    for (int j = li; j < parts; j += L) m = fmaxf(m, part_ml[((int64_t)j * rows + row) * 2]);
+    float2 st[KS];                                             // the first 32 parts' stay in registers
 #pragma unroll
-    for (int o = 1; o < L; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, L));
+    for (int k = 0; k < KS; k++) st[k] = q + 8 * k < parts ? stat(q + 8 * k) : make_float2(-1e30f, 0.0f);
+#pragma unroll
+    for (int k = 0; k < KS; k++) m = fmaxf(m, st[k].x);
+    for (int j = q + 8 * KS; j < parts; j += 8) m = fmaxf(m, stat(j).x);
+    red[q][row] = m;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 8; k++) m = fmaxf(m, red[k][row]);
     float l = 0.0f;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int j0 = 0; j0 < parts; j0 += L) {
-        float w = 0.0f;
-        if (j0 + li < parts) {
-            const float2 ml = *reinterpret_cast<const float2 *>(part_ml + ((int64_t)(j0 + li) * rows + row) * 2);
-            w = __builtin_amdgcn_exp2f(ml.x - m);
-            l += ml.y * w;
-        }
-        const int nj = min(L, parts - j0);
-        for (int j = 0; j < nj; j += U) {
-            float4 v[U];
+    auto weigh = [&](int j, float2 ml) {
+        const float w = __builtin_amdgcn_exp2f(ml.x - m);
+        wts[j][row] = w;
+        l += ml.y * w;
+    };
 #pragma unroll
-            for (int u = 0; u < U; u++)
-                v[u] = *reinterpret_cast<const float4 *>(part_o + ((int64_t)min(j0 + j + u, parts - 1) * rows + row) * HD + d);
+    for (int k = 0; k < KS; k++)
+        if (q + 8 * k < parts) weigh(q + 8 * k, st[k]);
+    for (int j = q + 8 * KS; j < parts; j += 8) weigh(j, stat(j));
+    reds[q][row] = l;
+    __syncthreads();
+    l = 0.0f;
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                const float wu = j + u < nj ? __shfl(w, (j + u) & (L - 1), L) : 0.0f;
-                a.x += v[u].x * wu; a.y += v[u].y * wu; a.z += v[u].z * wu; a.w += v[u].w * wu;
+    for (int k = 0; k < 8; k++) l += reds[k][row];
+    float4 a[DG];
+#pragma unroll
+    for (int g = 0; g < DG; g++) a[g] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int j = 0; j < parts; j += U) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (j + u >= parts) break;
+            const float w = wts[j + u][row];
+#pragma unroll
+            for (int g = 0; g < DG; g++) {
+                a[g].x += v[u][g].x * w; a[g].y += v[u][g].y * w; a[g].z += v[u][g].z * w; a[g].w += v[u][g].w * w;
             }
+            load(j + u + U, v[u]);
         }
     }
-#pragma unroll
-    for (int o = 1; o < L; o <<= 1) l += __shfl_xor(l, o, L);
     const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-    uint2 w;
-    w.x = f32x2_to_bf16x2(a.x * inv, a.y * inv);
-    w.y = f32x2_to_bf16x2(a.z * inv, a.w * inv);
-    *reinterpret_cast<uint2 *>(out + (row / nh) * o_ts + (row % nh) * HD + d) = w;
+#pragma unroll
+    for (int g = 0; g < DG; g++)
+        *reinterpret_cast<uint2 *>(tile + row * OROW + (q + 8 * g) * 8) =
+            make_uint2(f32x2_to_bf16x2(a[g].x * inv, a[g].y * inv), f32x2_to_bf16x2(a[g].z * inv, a[g].w * inv));
+    __syncthreads();
+    for (int i = tid; i < 32 * CH; i += 256) {
+        const int rr = i / CH, c = i % CH, r = r0 + rr;
+        if (r < rows)
+            *reinterpret_cast<uint4 *>(out + (int64_t)(r / G) * o_ts + (int64_t)(kvh * G + r % G) * HD + d0 + c * 8) =
+                *reinterpret_cast<const uint4 *>(tile + rr * OROW + c * 16);
+    }
 }
 
 }  // namespace ifh
@@ -676,8 +704,7 @@ static void plan_keys(KeySet *k, int mode, int64_t seq_rows, int64_t blocks_wide
     const int64_t blocks = k->narrow ? blocks_narrow : blocks_wide;
     k->blocks = (int)blocks;
     k->max_keys = max_keys;
-    const int keys = k->narrow ? kNarrowKeys : kWideKeys, least = k->narrow ? 8 : 2;
-    const int tiles = (max_keys + keys - 1) / keys;
+    const int tiles = (max_keys + kKeys - 1) / kKeys, least = k->narrow ? 8 : 4;
     const int64_t want = 2 * (int64_t)device_cu_count_physical() / (blocks * nkv > 0 ? blocks * nkv : 1);
     int parts = (int)(want < 1 ? 1 : want > 64 ? 64 : want);
     if (parts > tiles / least) parts = tiles / least > 1 ? tiles / least : 1;
@@ -685,7 +712,8 @@ static void plan_keys(KeySet *k, int mode, int64_t seq_rows, int64_t blocks_wide
     k->parts = (tiles + k->part_tiles - 1) / k->part_tiles;
 }
 
-static int64_t part_floats(int64_t rows, int parts, int hd) { return rows * parts * (hd + 2); }
+static int64_t part_floats(int64_t row_tiles, int nkv, int parts, int hd) { return row_tiles * nkv * parts * 32 * (hd + 2); }
+static int64_t row_tiles_of(int64_t ntokens, int G) { return (ntokens * G + 31) / 32; }
 
 static void rows_launch(const RowsParams &p, int hd, int64_t workgroups, hipStream_t st)
 {
@@ -699,10 +727,16 @@ static void rows_launch(const RowsParams &p, int hd, int64_t workgroups, hipStre
 
 static void join_launch(const RowsParams &p, int hd, int parts, hipStream_t st)
 {
-    const int64_t rows = p.part_rows, per = 256 / (hd / 4);
-    const dim3 grid((unsigned)((rows + per - 1) / per));
-    if (hd == 128) hipLaunchKernelGGL(k_attn_join<128>, grid, dim3(256), 0, st, p.part_o, p.part_ml, rows, parts, p.out, p.o_ts, p.nh);
-    else hipLaunchKernelGGL(k_attn_join<64>, grid, dim3(256), 0, st, p.part_o, p.part_ml, rows, parts, p.out, p.o_ts, p.nh);
+    const int tiles = p.row_tiles * p.nkv, rows = p.ntokens * p.G;
+    const bool whole = tiles >= device_cu_count_physical();
+    const dim3 grid((unsigned)tiles, (unsigned)(whole ? 1 : hd / 32)), block(256);
+#define ROWS_JOIN(HD, DG) hipLaunchKernelGGL((k_attn_join<HD, DG>), grid, block, 0, st, p.part_o, p.part_ml, p.row_tiles, p.nkv, parts, p.out, p.o_ts, p.G, rows)
+    if (hd == 128) {
+        if (whole) ROWS_JOIN(128, 4); else ROWS_JOIN(128, 1);
+    } else {
+        if (whole) ROWS_JOIN(64, 2); else ROWS_JOIN(64, 1);
+    }
+#undef ROWS_JOIN
 }
 
 static void packed_plan(int64_t ntokens, int64_t nseqs, int G, int nkv, int max_keys, KeySet *k)
@@ -721,7 +755,7 @@ extern "C" int64_t ifh_attn_packed_ws_floats(int ntokens, int nseqs, int nheads,
     if (ntokens <= 0 || nseqs <= 0 || nkv <= 0 || nheads < nkv || nheads % nkv || max_keys <= 0 || !packed_fits(ntokens, nseqs, nheads, nkv)) return 0;
     KeySet k = {};
     packed_plan(ntokens, nseqs, nheads / nkv, nkv, max_keys, &k);
-    return k.parts > 1 ? part_floats((int64_t)ntokens * nheads, k.parts, head_dim) : 0;
+    return k.parts > 1 ? part_floats(row_tiles_of(ntokens, nheads / nkv), nkv, k.parts, head_dim) : 0;
 }
 
 // what the two attention descriptors share
@@ -752,11 +786,12 @@ extern "C" int ifh_attn_packed_bf16(const ifh_attn_packed_desc *d, ifh_stream_t 
     p.cu = d->cu;
     p.ntokens = d->ntokens; p.nseqs = d->nseqs; p.nh = d->nheads; p.nkv = d->nkv; p.T = 1;
     p.scale = d->scale;
-    p.part_rows = (int64_t)d->ntokens * d->nheads;
+    p.row_tiles = (int)row_tiles_of(d->ntokens, p.G);
     if (d->ws && k.parts > 1) {
-        IFH_CHECK_ARG(d->ws_floats >= part_floats(p.part_rows, k.parts, d->head_dim));
+        const int64_t floats = part_floats(p.row_tiles, p.nkv, k.parts, d->head_dim);
+        IFH_CHECK_ARG(d->ws_floats >= floats);
         p.part_o = d->ws;
-        p.part_ml = d->ws + p.part_rows * k.parts * d->head_dim;
+        p.part_ml = d->ws + floats / (d->head_dim + 2) * d->head_dim;
     } else
         k.parts = 1;
     const int64_t wgs = (int64_t)k.blocks * p.nkv * k.parts;
@@ -797,7 +832,7 @@ extern "C" int64_t ifh_attn_prefix_ws_floats(int nrows, int tokens_per_row, int 
     if (!prefix_fits((int64_t)nrows * tokens_per_row, nheads, nkv)) return 0;
     KeySet a = {}, b = {};
     prefix_plan(nrows, tokens_per_row, prefix_keys, nheads, nkv, max_keys, &a, &b);
-    return part_floats((int64_t)nrows * tokens_per_row * nheads, a.parts + b.parts, head_dim);
+    return part_floats(row_tiles_of((int64_t)nrows * tokens_per_row, nheads / nkv), nkv, a.parts + b.parts, head_dim);
 }
 
 extern "C" int ifh_attn_prefix_bf16(const ifh_attn_prefix_desc *d, ifh_stream_t stream)
@@ -820,9 +855,10 @@ extern "C" int ifh_attn_prefix_bf16(const ifh_attn_prefix_desc *d, ifh_stream_t 
     p.out = (uint16_t *)d->out; p.o_ts = d->o_ts;
     p.ntokens = (int)ntokens; p.nseqs = d->nrows; p.nh = d->nheads; p.nkv = d->nkv; p.G = d->nheads / d->nkv; p.T = d->tokens_per_row;
     p.scale = d->scale;
-    p.part_rows = ntokens * d->nheads;
+    p.row_tiles = (int)row_tiles_of(ntokens, p.G);
     const int parts = a.parts + b.parts;
-    IFH_CHECK_ARG(d->ws_floats >= part_floats(p.part_rows, parts, d->head_dim));
+    const int64_t floats = part_floats(p.row_tiles, p.nkv, parts, d->head_dim);
+    IFH_CHECK_ARG(d->ws_floats >= floats);
     hipStream_t st = as_stream(stream);
     if (prefix_joint((int64_t)b.blocks * p.nkv, d->prefix_keys, d->max_keys, b.narrow)) {
         p.joint = 1;
@@ -831,7 +867,7 @@ extern "C" int ifh_attn_prefix_bf16(const ifh_attn_prefix_desc *d, ifh_stream_t 
         return IFH_OK;
     }
     p.part_o = d->ws;
-    p.part_ml = d->ws + p.part_rows * parts * d->head_dim;
+    p.part_ml = d->ws + floats / (d->head_dim + 2) * d->head_dim;
     const int64_t na = (int64_t)a.blocks * p.nkv * a.parts, nb = (int64_t)b.blocks * p.nkv * b.parts;
     p.first = (int)na;
     p.pairs = (int)((na < nb ? na : nb) / 256);
