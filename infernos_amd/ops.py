@@ -280,11 +280,11 @@ def rope_append_packed(qkv, cos_sin, cache, cu, pos0, *, ntokens, nseqs, nheads,
 
 
 def _ws(floats, device):
-    return torch.empty(floats, dtype=torch.float32, device=device) if floats > 0 else None
+    return torch.empty(floats, dtype=torch.float32, device=device)
 
 
 def attn_packed_ws(device, *, ntokens, nseqs, nheads, nkv, head_dim, max_keys):
-    """f32 workspace with which attn_packed splits few long rows along their keys; None where it would not.  A caller that captures
+    """f32 workspace with which attn_packed splits few long rows along their keys; empty where it would not.  A caller that captures
     graphs or uses several streams keeps one for each."""
     with torch.cuda.device(device):
         return _ws(_lib.lib().ifh_attn_packed_ws_floats(ntokens, nseqs, nheads, nkv, head_dim, max_keys), device)
@@ -297,7 +297,7 @@ def attn_packed(q, cache, out, cu, key_len, *, ntokens, nseqs, nheads, nkv, head
     kv = nkv * head_dim
     d = _lib.AttnPackedDesc(q.data_ptr(), nheads * head_dim + 2 * kv if q_ts is None else q_ts, cache.data_ptr(), max_pos * 2 * kv, 2 * kv, kv,
                             out.data_ptr(), nheads * head_dim, cu.data_ptr(), key_len.data_ptr(), ntokens, nseqs, nheads, nkv, head_dim,
-                            max_keys, head_dim ** -0.5, _ptr(ws), 0 if ws is None else ws.numel())
+                            max_keys, head_dim ** -0.5, _ptr(ws), 0 if ws is None else ws.numel())       # (an empty tensor's address is NULL)
     _launch('ifh_attn_packed_bf16', out, ctypes.byref(d))
     return out
 

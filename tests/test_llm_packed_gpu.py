@@ -120,7 +120,7 @@ def test_attn_packed_long(dev, heads, lens, past):
     for split in (False, True):
         out, ws = run_packed(c, dev, split)
         w = check_rows(out.view(-1, nh, hd), rows, 'packed split=%s' % split)
-        print('attn_packed ok', heads, lens, past, 'split', ws is not None, 'worst share %.2f' % w)
+        print('attn_packed ok', heads, lens, past, 'split', ws is not None and ws.numel() > 0, 'worst share %.2f' % w)
 
 
 def test_attn_packed_rows_that_see_nothing_and_tokens_behind_the_last(dev):
@@ -519,7 +519,7 @@ def test_other_stream_and_captured_graph_replays(dev):
     logits, u = torch.randn(B * 2, V, device=dev), torch.rand(B, 2, device=dev)
     drafts = i32([[1], [2], [3], [4], [5], [6]], dev)
     pw = ops.attn_packed_ws(dev, ntokens=c['N'], nseqs=3, nheads=nh, nkv=nkv, head_dim=hd, max_keys=c['max_keys'])
-    assert pw is not None
+    assert pw.numel() > 0
     xw = ops.attn_prefix_ws(dev, nrows=6, tokens_per_row=2, prefix_keys=900, nheads=nh, nkv=nkv, head_dim=hd, max_keys=x['max_keys'])
     vw = ops.verify_drafts_ws(B, T, dev)
     o1, o2 = torch.zeros(c['N'], nh * hd, dtype=BF, device=dev), torch.zeros(12, nh * hd, dtype=BF, device=dev)
