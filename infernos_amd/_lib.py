@@ -418,12 +418,6 @@ def stream_ptr(device=None):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
-def raw_stream(index):
-    """the current stream of device `index` as an integer (0: the default stream), without a torch Stream object around it"""
-    import torch
-    return torch._C._cuda_getCurrentRawStream(index)
-
-
 def ptr(t):
     """Raw device (or host) pointer of a contiguous torch tensor / None."""
     if t is None:

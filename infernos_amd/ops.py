@@ -258,14 +258,18 @@ def _ptr(t):
 
 
 def _launch(name, like, *args):
-    """fn(*args, the current stream of `like`'s device), with that device current: its tensors may live on another than the caller's"""
-    fn, i = getattr(_lib.lib(), name), like.device.index
-    if i is None:
+    """fn(*args, the current stream of `like`'s device), with that device current: its tensors may live on another than the caller's.
+    (torch's own accessors underneath current_device() and current_stream(): a call of a few microseconds is half made of those)"""
+    fn, i, C = getattr(_lib.lib(), name), like.get_device(), torch._C
+    if i < 0:
         raise _lib.InfernosHipError('%s: a tensor is not on a HIP GPU' % name)
-    if i == torch.cuda.current_device():
-        return _lib.check(fn(*args, _lib.raw_stream(i)), name)
-    with torch.cuda.device(i):
-        return _lib.check(fn(*args, _lib.raw_stream(i)), name)
+    if i == C._cuda_getDevice():
+        rc = fn(*args, C._cuda_getCurrentRawStream(i))
+    else:
+        with torch.cuda.device(i):
+            rc = fn(*args, C._cuda_getCurrentRawStream(i))
+    if rc:
+        _lib.check(rc, name)
 
 
 def rope_append_packed(qkv, cos_sin, cache, cu, pos0, *, ntokens, nseqs, nheads, nkv, head_dim, max_pos, slot0=None, q_out=None):
