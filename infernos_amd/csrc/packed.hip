@@ -14,15 +14,20 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 namespace ifh {
 
-// index s of the sequence with cu[s] <= i < cu[s + 1] (cu non-decreasing, n + 1 entries); n where there is none
+// Last s with cu[s] <= i, or 0 (cu non-decreasing, n + 1 entries; i the same in the whole wave): the lanes probe 64 entries at a time, one
+// round trip up to 64 sequences, two up to 4096.
 __device__ __forceinline__ int packed_seq(const int32_t *__restrict__ cu, int n, int i)
 {
-    int lo = 0, hi = n;
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (cu[mid + 1] <= i) lo = mid + 1; else hi = mid;
+    const int lane = threadIdx.x & 63;
+    int lo = 0, range = n;
+    while (range > 1) {
+        const int step = (range + 63) >> 6;
+        const int cnt = __popcll(__ballot(lane * step < range && cu[lo + lane * step] <= i));
+        const int first = (cnt > 0 ? cnt - 1 : 0) * step;
+        lo += first;
+        range = min(step, range - first);
     }
-    return lo < n && cu[lo] <= i ? lo : n;
+    return __builtin_amdgcn_readfirstlane(lo);
 }
 
 // One thread per (token, head slot, 8 pairs j .. j + 7 of the head): the arithmetic and the roundings of k_rope_append (llm.hip).
@@ -33,20 +38,27 @@ __global__ __launch_bounds__(256) void k_rope_packed(const uint16_t *__restrict_
                                                      const int32_t *__restrict__ slot0, int nseqs, int nh, int nkv, int hd, int max_pos,
                                                      int64_t total)
 {
-    const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (idx >= total) return;
+    const int64_t idx0 = (int64_t)blockIdx.x * 256 + threadIdx.x, idx = idx0 < total ? idx0 : total - 1;      // (whole waves: they search together)
     const int half = hd >> 1, groups = half >> 3, slots = nh + 2 * nkv;
     const int j = (int)(idx % groups) * 8, slot = (int)((idx / groups) % slots);
-    const int64_t i = idx / ((int64_t)groups * slots);
-    const int s = packed_seq(cu, nseqs, (int)i);
-    if (s >= nseqs) return;
-    const int t = (int)i - cu[s], pos = pos0[s] + t, at = (slot0 ? slot0[s] : pos0[s]) + t;
+    const int i = (int)(idx / ((int64_t)groups * slots));
+    const uint16_t *src = qkv + i * qkv_ld + (int64_t)slot * hd;
+    const uint4 lo = *reinterpret_cast<const uint4 *>(src + j), hi = *reinterpret_cast<const uint4 *>(src + j + half);
+    // the wave's first token's sequence; a later token's lies behind it
+    int s = packed_seq(cu, nseqs, __builtin_amdgcn_readfirstlane(i));
+    if (cu[s + 1] <= i) {
+        int hi_s = nseqs;
+        while (s < hi_s) {
+            const int mid = (s + hi_s) >> 1;
+            if (cu[mid + 1] <= i) s = mid + 1; else hi_s = mid;
+        }
+    }
+    if (idx0 >= total || s >= nseqs || i < cu[s]) return;
+    const int t = i - cu[s], pos = pos0[s] + t, at = (slot0 ? slot0[s] : pos0[s]) + t;
     if (pos < 0 || pos >= table_len) return;
     if (slot >= nh && (at < 0 || at >= max_pos)) return;
-    const uint16_t *src = qkv + i * qkv_ld + (int64_t)slot * hd;
     uint16_t *dst = slot < nh ? q_out + i * q_ld + (int64_t)slot * hd
                               : cache + (int64_t)s * cache_bs + (int64_t)at * cache_ts + (int64_t)(slot - nh) * hd;
-    const uint4 lo = *reinterpret_cast<const uint4 *>(src + j), hi = *reinterpret_cast<const uint4 *>(src + j + half);
     if (slot >= nh + nkv) {                 // value head: plain copy
         *reinterpret_cast<uint4 *>(dst + j) = lo;
         *reinterpret_cast<uint4 *>(dst + j + half) = hi;

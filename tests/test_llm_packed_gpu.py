@@ -328,6 +328,31 @@ def test_rope_append_packed(dev, heads):
     assert torch.equal(cache[3, 1:], cache0[3, 1:]) and bool((q[:6] == 7.0).all())
 
 
+@pytest.mark.parametrize('n', [65, 300, 5000])
+def test_many_sequences_most_of_them_empty(dev, n):
+    """hundreds and thousands of sequences, one token or none each: every one found (rows and positions by their number)"""
+    from infernos_amd import ops
+    nh, nkv, hd = 4, 1, 64
+    g = torch.Generator(device=dev).manual_seed(n)
+    lens = [(1 if (s * 7919) % 5 == 0 else 0) + (3 if s % 97 == 5 else 0) for s in range(n)]
+    N = sum(lens)
+    key_len = [a + s % 3 for s, a in enumerate(lens)]
+    c = packed_case(dev, (nh, nkv, hd), lens, key_len, seed=n)
+    out, _ = run_packed(c, dev)
+    for (i, h), o, t in packed_rows(c, sample=2 if n > 1000 else None):
+        assert bool(((out.view(N, nh, hd)[i, h].double() - o).abs() <= t).all()), (i, h)
+    ang = torch.arange(16, device=dev, dtype=F64)[:, None] * 1.0e4 ** (-torch.arange(0, hd, 2, device=dev, dtype=F64) / hd)
+    cs = torch.stack([ang.cos(), ang.sin()], -1).float().contiguous()
+    cache = torch.zeros(n, 8, 2 * nkv * hd, dtype=BF, device=dev)
+    pos0 = [s % 4 for s in range(n)]
+    ops.rope_append_packed(c['qkv'], cs, cache, c['cu'], i32(pos0, dev), ntokens=N, nseqs=n, nheads=nh, nkv=nkv, head_dim=hd, max_pos=8)
+    ref, i = torch.zeros_like(cache), 0
+    for s, a in enumerate(lens):
+        ref[s, pos0[s]:pos0[s] + a, hd:] = c['qkv'][i:i + a, (nh + 1) * hd:]
+        i += a
+    assert torch.equal(cache[:, :, hd:], ref[:, :, hd:])
+
+
 # ---- drafts -------------------------------------------------------------------------------------------------------------
 def verify64(p, q, drafts, u, n):
     """p [n + 1, V], q [n, V] f64 rows of one request -> (kept, mass of the drawn position, margin of the closest decision)"""
