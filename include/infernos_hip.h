@@ -677,10 +677,10 @@ int ifh_rope_append_packed_bf16(const ifh_rope_packed_desc *desc, ifh_stream_t s
  * keys of cache row s; its last token sees all of them, the one before one fewer, and so on (new tokens behind what the row already
  * holds, themselves appended before).  A token that sees no key gets zeros; tokens behind cu[nseqs] keep what out holds.  Any number of
  * query heads per kv head; head_dim 64 or 128.  softmax(scale q.k) v, f32 sums; the probabilities are rounded to bf16 for the second
- * product.  V rows a token does not see, inside the 64-key tile its last key is in, are multiplied by zero: they have to be finite
- * up to key_len.  Slots from key_len on are not used.
- * ws: f32 workspace of ifh_attn_packed_ws_floats() elements, with which few long rows are split along their keys (NULL, or
- * where that function says 0: they are not).  A workspace belongs to one stream / graph at a time. */
+ * product.  K and V from slot key_len on are not used, whatever they hold.  A K row that is not finite reaches only the tokens that see
+ * it; V rows below key_len have to be finite, for a token multiplies those of its tiles that it does not see by zero.
+ * ws: f32 workspace, with which few long rows are split along their keys: ifh_attn_packed_ws_floats() elements for the split that fills
+ * the device (0: none is needed), a smaller one splits less, NULL not at all.  A workspace belongs to one stream / graph at a time. */
 typedef struct ifh_attn_packed_desc {
     const void *q;
     int64_t q_ts;
@@ -700,7 +700,9 @@ int ifh_attn_packed_bf16(const ifh_attn_packed_desc *desc, ifh_stream_t stream);
 /* Grouped-query attention of a decode step whose rows share a prefix: token i of row b = i / tokens_per_row sees the first
  * prefix_len[b] keys of the one row `prefix` (bf16 [prefix_keys][prefix_ts]; prefix_len NULL: all of them; 0: none) and the first
  * key_len[i] keys of cache row b.  The prefix is read once for all rows, not once a row.  A token that sees no key gets zeros.
- * tokens_per_row > 1: drafted tokens, each with its own key_len.  ws: ifh_attn_prefix_ws_floats() f32, of one stream / graph at a time. */
+ * tokens_per_row > 1: drafted tokens, each with its own key_len.  V rows of the prefix, and a row's own below its largest key_len, have
+ * to be finite (see above).  ws: ifh_attn_prefix_ws_floats() f32 for the split that fills the device; a smaller one splits less, down to
+ * two partial results a query row.  Of one stream / graph at a time. */
 typedef struct ifh_attn_prefix_desc {
     const void *q;
     int64_t q_ts;

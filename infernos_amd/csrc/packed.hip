@@ -727,6 +727,14 @@ static void plan_keys(KeySet *k, int mode, int64_t seq_rows, int64_t blocks_wide
 static int64_t part_floats(int64_t row_tiles, int nkv, int parts, int hd) { return row_tiles * nkv * parts * 32 * (hd + 2); }
 static int64_t row_tiles_of(int64_t ntokens, int G) { return (ntokens * G + 31) / 32; }
 
+// one part fewer
+static void fewer_parts(KeySet *k)
+{
+    const int tiles = (k->max_keys + kKeys - 1) / kKeys, parts = k->parts - 1;
+    k->part_tiles = (tiles + parts - 1) / parts;
+    k->parts = (tiles + k->part_tiles - 1) / k->part_tiles;
+}
+
 static void rows_launch(const RowsParams &p, int hd, int64_t workgroups, hipStream_t st)
 {
     const dim3 grid((unsigned)workgroups), block(256);
@@ -799,13 +807,11 @@ extern "C" int ifh_attn_packed_bf16(const ifh_attn_packed_desc *d, ifh_stream_t 
     p.ntokens = d->ntokens; p.nseqs = d->nseqs; p.nh = d->nheads; p.nkv = d->nkv; p.T = 1;
     p.scale = d->scale;
     p.row_tiles = (int)row_tiles_of(d->ntokens, p.G);
-    if (d->ws && k.parts > 1) {
-        const int64_t floats = part_floats(p.row_tiles, p.nkv, k.parts, d->head_dim);
-        IFH_CHECK_ARG(d->ws_floats >= floats);
+    while (k.parts > 1 && (!d->ws || part_floats(p.row_tiles, p.nkv, k.parts, d->head_dim) > d->ws_floats)) fewer_parts(&k);
+    if (k.parts > 1) {
         p.part_o = d->ws;
-        p.part_ml = d->ws + floats / (d->head_dim + 2) * d->head_dim;
-    } else
-        k.parts = 1;
+        p.part_ml = d->ws + (int64_t)p.row_tiles * p.nkv * k.parts * 32 * d->head_dim;
+    }
     const int64_t wgs = (int64_t)k.blocks * p.nkv * k.parts;
     p.first = (int)wgs;
     hipStream_t st = as_stream(stream);
@@ -835,7 +841,6 @@ static void prefix_plan(int64_t nrows, int64_t T, int prefix_keys, int nheads, i
     const int64_t r = T * (nheads / nkv), all = nrows * r;
     plan_keys(prefix, ROWS_PREFIX, all, (all + kWideRows - 1) / kWideRows, (all + kNarrowRows - 1) / kNarrowRows, nkv, prefix_keys);
     plan_keys(own, ROWS_OWN, r, nrows * ((r + kWideRows - 1) / kWideRows), nrows * ((r + kNarrowRows - 1) / kNarrowRows), nkv, max_keys);
-    own->part0 = prefix->parts;
 }
 
 extern "C" int64_t ifh_attn_prefix_ws_floats(int nrows, int tokens_per_row, int prefix_keys, int nheads, int nkv, int head_dim, int max_keys)
@@ -868,9 +873,10 @@ extern "C" int ifh_attn_prefix_bf16(const ifh_attn_prefix_desc *d, ifh_stream_t 
     p.ntokens = (int)ntokens; p.nseqs = d->nrows; p.nh = d->nheads; p.nkv = d->nkv; p.G = d->nheads / d->nkv; p.T = d->tokens_per_row;
     p.scale = d->scale;
     p.row_tiles = (int)row_tiles_of(ntokens, p.G);
+    while (a.parts + b.parts > 2 && part_floats(p.row_tiles, p.nkv, a.parts + b.parts, d->head_dim) > d->ws_floats) fewer_parts(a.parts >= b.parts ? &a : &b);
     const int parts = a.parts + b.parts;
-    const int64_t floats = part_floats(p.row_tiles, p.nkv, parts, d->head_dim);
-    IFH_CHECK_ARG(d->ws_floats >= floats);
+    b.part0 = a.parts;
+    IFH_CHECK_ARG(d->ws_floats >= part_floats(p.row_tiles, p.nkv, parts, d->head_dim));
     hipStream_t st = as_stream(stream);
     if (prefix_joint((int64_t)b.blocks * p.nkv, d->prefix_keys, d->max_keys, b.narrow)) {
         p.joint = 1;
@@ -879,7 +885,7 @@ extern "C" int ifh_attn_prefix_bf16(const ifh_attn_prefix_desc *d, ifh_stream_t 
         return IFH_OK;
     }
     p.part_o = d->ws;
-    p.part_ml = d->ws + floats / (d->head_dim + 2) * d->head_dim;
+    p.part_ml = d->ws + (int64_t)p.row_tiles * p.nkv * parts * 32 * d->head_dim;
     const int64_t na = (int64_t)a.blocks * p.nkv * a.parts, nb = (int64_t)b.blocks * p.nkv * b.parts;
     p.first = (int)na;
     p.pairs = (int)((na < nb ? na : nb) / 256);

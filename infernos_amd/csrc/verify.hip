@@ -277,11 +277,11 @@ __global__ __launch_bounds__(VD) void k_verify_draw(const VerifyParams p)
 {
     __shared__ VerdictLds L;
     __shared__ double part[4][VD / 64], cut;
-    __shared__ int first[2], last;
+    __shared__ int first[2], last[2];
     const int r = blockIdx.x, tid = threadIdx.x;
     constexpr int E = VC / VD;
     if (tid < 2) first[tid] = 0x7fffffff;
-    if (tid == 2) last = -1;
+    if (tid < 2) last[tid] = -1;
     const double u = (double)p.uniform[(int64_t)r * (p.T + 1) + p.T];
     const Verdict w = verdict_of<VD>(p, r, L);
     int token = -1;
@@ -325,9 +325,11 @@ __global__ __launch_bounds__(VD) void k_verify_draw(const VerifyParams p)
         // (one LDS atomic a wave: 1024 of them on one word cost 7 us)
         const int lane = tid & 63;
         const unsigned long long past = __ballot(mine && cum > want);
+        const unsigned long long with = __ballot(mine && cm > 0.0);
         if (past && lane == __ffsll((long long)past) - 1) atomicMin(&first[0], tid);
+        if (with && lane == 63 - __clzll((long long)with)) atomicMax(&last[0], tid);
         __syncthreads();
-        const int c = min(first[0], p.nch - 1);
+        const int c = first[0] != 0x7fffffff ? first[0] : max(last[0], 0);     // (a number of 1 or more: the last chunk with any mass)
         // the chunk's tokens, two consecutive ones a thread
         const int j0 = c * VC + tid * E;
         float lv[E], qv[E];
@@ -357,9 +359,9 @@ __global__ __launch_bounds__(VD) void k_verify_draw(const VerifyParams p)
         }
         const unsigned long long hit = __ballot(at >= 0), some = __ballot(lastj >= 0);
         if (hit && lane == __ffsll((long long)hit) - 1) atomicMin(&first[1], at);
-        if (some && lane == 63 - __clzll((long long)some)) atomicMax(&last, lastj);
+        if (some && lane == 63 - __clzll((long long)some)) atomicMax(&last[1], lastj);
         __syncthreads();
-        token = first[1] != 0x7fffffff ? first[1] : last;     // (rounding past the chunk's end: its last token with any mass)
+        token = first[1] != 0x7fffffff ? first[1] : last[1];  // (rounding past the chunk's end: its last token with any mass)
     }
     for (int i = tid; i <= p.T; i += VD)
         p.out_tokens[(int64_t)r * (p.T + 1) + i] = i < w.kept ? p.drafts[(int64_t)r * p.T + i] : i == w.kept ? token : -1;

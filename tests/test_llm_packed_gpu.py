@@ -123,6 +123,32 @@ def test_attn_packed_long(dev, heads, lens, past):
         print('attn_packed ok', heads, lens, past, 'split', ws is not None and ws.numel() > 0, 'worst share %.2f' % w)
 
 
+@pytest.mark.parametrize('share', [0.9, 0.5, 0.26, 0.1, 0.0])
+def test_smaller_workspaces_split_less(dev, share):
+    """a workspace made for another batch: as many parts as it holds, the same results within the roundings"""
+    heads = (12, 2, 128)
+    c = packed_case(dev, heads, [20, 3], [3000, 1500], seed=12)
+    full = run_packed(c, dev)[1]
+    assert full.numel() > 0
+    from infernos_amd import ops
+    out = torch.empty(23, 12 * 128, dtype=BF, device=dev)
+    n = int(full.numel() * share)
+    guard = torch.full((n + 256,), 3.0, device=dev)
+    ops.attn_packed(c['qkv'], c['cache'], out, c['cu'], c['key_len'], ntokens=23, nseqs=2, nheads=12, nkv=2, head_dim=128, max_pos=c['S'],
+                    max_keys=c['max_keys'], ws=guard[:n])
+    check_rows(out.view(-1, 12, 128), packed_rows(c, sample=4), 'packed')
+    assert bool((guard[n:] == 3.0).all())
+    x = prefix_case(dev, heads, 5, 2, 1500, [700, 20, 0, 300, 90], seed=13)
+    kw = dict(nrows=5, tokens_per_row=2, prefix_keys=1500, nheads=12, nkv=2, head_dim=128, max_keys=x['max_keys'])
+    full = ops.attn_prefix_ws(dev, **kw)
+    two = 2 * 2 * 2 * 32 * 130                                       # parts x kv heads x row tiles x rows x (head_dim + 2)
+    assert full.numel() > two
+    n = max(two, int(full.numel() * share))
+    guard = torch.full((n + 256,), 3.0, device=dev)
+    check_rows(run_prefix(x, dev, ws=guard[:n]).view(-1, 12, 128), prefix_rows(x), 'prefix')
+    assert bool((guard[n:] == 3.0).all())
+
+
 def test_attn_packed_rows_that_see_nothing_and_tokens_behind_the_last(dev):
     """fewer keys than tokens: the first tokens see none and get zeros; tokens behind the last sequence keep what was there"""
     heads = (12, 2, 128)
@@ -470,6 +496,11 @@ def test_verify_drafts_greedy_ties_and_masks(dev):
     assert tok.tolist() == [[0, -1]]
     tok, cnt = run_verify(dev, l, i32([[0]], dev), torch.tensor([[0.999, 0.0]], device=dev), V, 1.0)
     assert tok.tolist() == [[1, -1]]
+    # a number at or past 1 (a caller's rounding): the last token with any mass
+    l2 = torch.full((1, V), -inf, device=dev)
+    l2[0, 3], l2[0, 4000] = 1.0, 2.0
+    tok, cnt = run_verify(dev, l2, i32([[0]], dev), torch.tensor([[1.0]], device=dev), V, 1.0)
+    assert tok.tolist() == [[4000]] and cnt.tolist() == [1]
     # the draft's distribution covers the target's: nothing is left over, so the token comes from p
     big = torch.ones(1, V, device=dev)
     tok, cnt = run_verify(dev, l, i32([[77]], dev), torch.tensor([[0.999, 0.99999]], device=dev), V, 1.0, q=big)
