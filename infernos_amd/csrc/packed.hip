@@ -298,7 +298,7 @@ struct WaveRows {
 };
 
 // Four waves.  Two forms of a workgroup, by KeySet::narrow:
-//   wide    128 rows, a wave 32 of them.  K / V tiles of 64 keys come by LDS-DMA into two buffers, the next tile in flight while this one is
+//   wide    128 rows, a wave 32 of them.  K / V tiles of 32 keys come by LDS-DMA into two buffers, the next tile in flight while this one is
 //           multiplied, one barrier a tile.
 //   narrow  32 rows, shared by the waves: a wave takes every fourth tile of 32 keys, by itself (its own K and V buffer, the next K in flight
 //           from the end of the first product on, no barrier), and the four results are joined in LDS.  For the few rows of a decode step,
@@ -707,18 +707,27 @@ extern "C" int ifh_rope_append_packed_bf16(const ifh_rope_packed_desc *d, ifh_st
     return IFH_OK;
 }
 
-// Fills in a key set's split for sequences (rows of a batch) of seq_rows rows: narrow workgroups where a sequence has about a narrow
-// block's rows or fewer.  Keys are split into parts until the device has two workgroups a CU, none of fewer than two tiles a wave.
+// Fills in a key set's split for sequences (rows of a batch) of seq_rows rows.
+// Narrow workgroups where a narrow block holds a sequence's rows: with more, its keys are read once for every 32 rows.  Measured, narrow and
+// wide: 36 rows of 32 sequences behind 1000 keys 18.9 and 14.2 us, 64 rows of 4 behind 4000 16.3 and 15.3 us; with 6 rows (a decode step
+// of 64 sequences behind 1000 keys) 17.6 and 24 us.
+// Keys are split into parts until the device has two workgroups a CU, and no further than that pays for the join's launch (2.5 us) and for
+// what each part costs it: none of fewer than eight tiles (narrow: two a wave) or four (wide), wide blocks of up to 512 keys not at all
+// unless the results are joined anyway (64 sequences, 300 keys: 7.4 us, split 9.4 us; one prompt of 300 rows 9.4, split 11.9 us; of 700 keys 15.7, split 12.8 us), and at most
+// 1.6 sqrt(tiles) parts, the time of a part being tiles / parts and that of the join parts (4 sequences of 4000 keys: 31 parts 15.7 us, 16
+// parts 14.0 us, 10 parts 15.5 us; one of 8000: 63 parts 17.2 us, 25 parts 15.6 us, 15 parts 17.7 us).
 static void plan_keys(KeySet *k, int mode, int64_t seq_rows, int64_t blocks_wide, int64_t blocks_narrow, int nkv, int max_keys)
 {
     k->mode = mode;
-    k->narrow = seq_rows <= 40;
+    k->narrow = seq_rows <= kNarrowRows;
     const int64_t blocks = k->narrow ? blocks_narrow : blocks_wide;
     k->blocks = (int)blocks;
     k->max_keys = max_keys;
     const int tiles = (max_keys + kKeys - 1) / kKeys, least = k->narrow ? 8 : 4;
     const int64_t want = 2 * (int64_t)device_cu_count_physical() / (blocks * nkv > 0 ? blocks * nkv : 1);
     int parts = (int)(want < 1 ? 1 : want > 64 ? 64 : want);
+    if (mode == ROWS_PACKED && !k->narrow && tiles <= 16) parts = 1;
+    while (2 * (int64_t)parts * parts > 5 * (int64_t)tiles && parts > 1) parts--;
     if (parts > tiles / least) parts = tiles / least > 1 ? tiles / least : 1;
     k->part_tiles = (tiles + parts - 1) / parts;
     k->parts = (tiles + k->part_tiles - 1) / k->part_tiles;
@@ -829,11 +838,13 @@ static bool prefix_fits(int64_t ntokens, int64_t nheads, int64_t nkv)
     return ntokens < (1 << 24) && ntokens * (nheads / nkv) < (1ll << 30) && (ntokens * (nheads / nkv) / kNarrowRows + ntokens + 1) * nkv < (1ll << 24);
 }
 
-// A short prefix is not worth a launch to share it: up to 768 keys in all (six tiles a wave) and two workgroups a CU, the workgroup of a
-// row's own keys reads the prefix too (from L2) and writes the result.  Two rows behind 333 keys: TODO_JOINT.
+// A short prefix is not worth a launch to share it: up to 640 keys in all (five tiles a wave) and two workgroups a CU, the workgroup of a
+// row's own keys reads the prefix too (from L2) and writes the result.  Measured, joint and shared: 2 rows of 333 + 40 keys 6.8 and 10.3
+// us, 64 rows of 300 + 200 15.1 and 18.4 us (40 / 8 heads); the shared form gains from about 700 keys on (64 rows of 600 + 150 12.2 and
+// 11.5 us, 16 rows of 2000 + 200 35.8 and 11.7 us).
 static bool prefix_joint(int64_t workgroups, int prefix_keys, int max_keys, bool narrow)
 {
-    return narrow && (int64_t)prefix_keys + max_keys <= 768 && workgroups <= 2 * (int64_t)device_cu_count_physical();
+    return narrow && (int64_t)prefix_keys + max_keys <= 640 && workgroups <= 2 * (int64_t)device_cu_count_physical();
 }
 
 static void prefix_plan(int64_t nrows, int64_t T, int prefix_keys, int nheads, int nkv, int max_keys, KeySet *prefix, KeySet *own)
