@@ -607,10 +607,12 @@ __global__ __launch_bounds__(256, LONG ? 3 : 2) void k_attn_rows(const RowsParam
 constexpr int kMaxParts = 128;
 template <int HD, int DG>
 __global__ __launch_bounds__(256) void k_attn_join(const float *__restrict__ part_o, const float *__restrict__ part_ml, int row_tiles, int nkv,
-                                                   int parts, uint16_t *__restrict__ out, int64_t o_ts, int G, int rows)
+                                                   int parts, uint16_t *__restrict__ out, int64_t o_ts, int G, int rows,
+                                                   const int32_t *__restrict__ cu, int nseqs)
 {
     constexpr int U = DG == 1 ? 16 : 8 / DG, KS = 4, OROW = 64 * DG + 16, CH = 4 * DG;
     __shared__ float wts[kMaxParts][32], red[8][32], reds[8][32];
+    __shared__ int edges[2];
     __shared__ __attribute__((aligned(16))) unsigned char tile[32 * OROW];
     const int tt = blockIdx.x, d0 = blockIdx.y * 32, kvh = tt / row_tiles, r0 = (tt - kvh * row_tiles) * 32;
     const int tid = threadIdx.x, row = tid & 31, q = tid >> 5;
@@ -628,6 +630,7 @@ __global__ __launch_bounds__(256) void k_attn_join(const float *__restrict__ par
     };
 #pragma unroll
     for (int u = 0; u < U; u++) load(u, v[u]);                 // (on their way while the weights are worked out)
+    const int edge = cu && tid < 2 ? cu[tid ? nseqs : 0] : tid ? rows : 0;
     float m = -1e30f;
     float2 st[KS];                                             // the first 32 parts' stay in registers
 #pragma unroll
@@ -636,6 +639,7 @@ __global__ __launch_bounds__(256) void k_attn_join(const float *__restrict__ par
     for (int k = 0; k < KS; k++) m = fmaxf(m, st[k].x);
     for (int j = q + 8 * KS; j < parts; j += 8) m = fmaxf(m, stat(j).x);
     red[q][row] = m;
+    if (tid < 2) edges[tid] = edge;
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < 8; k++) m = fmaxf(m, red[k][row]);
@@ -677,7 +681,7 @@ __global__ __launch_bounds__(256) void k_attn_join(const float *__restrict__ par
     __syncthreads();
     for (int i = tid; i < 32 * CH; i += 256) {
         const int rr = i / CH, c = i % CH, r = r0 + rr;
-        if (r < rows)
+        if (r < rows && r / G >= edges[0] && r / G < edges[1])       // (tokens in front of the first sequence or behind the last: none)
             *reinterpret_cast<uint4 *>(out + (int64_t)(r / G) * o_ts + (int64_t)(kvh * G + r % G) * HD + d0 + c * 8) =
                 *reinterpret_cast<const uint4 *>(tile + rr * OROW + c * 16);
     }
@@ -759,7 +763,7 @@ static void join_launch(const RowsParams &p, int hd, int parts, hipStream_t st)
     const int tiles = p.row_tiles * p.nkv, rows = p.ntokens * p.G;
     const bool whole = tiles >= device_cu_count_physical();
     const dim3 grid((unsigned)tiles, (unsigned)(whole ? 1 : hd / 32)), block(256);
-#define ROWS_JOIN(HD, DG) hipLaunchKernelGGL((k_attn_join<HD, DG>), grid, block, 0, st, p.part_o, p.part_ml, p.row_tiles, p.nkv, parts, p.out, p.o_ts, p.G, rows)
+#define ROWS_JOIN(HD, DG) hipLaunchKernelGGL((k_attn_join<HD, DG>), grid, block, 0, st, p.part_o, p.part_ml, p.row_tiles, p.nkv, parts, p.out, p.o_ts, p.G, rows, p.cu, p.nseqs)
     if (hd == 128) {
         if (whole) ROWS_JOIN(128, 4); else ROWS_JOIN(128, 1);
     } else {
