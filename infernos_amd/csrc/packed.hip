@@ -114,6 +114,7 @@ struct RowsParams {
     float *part_o, *part_ml;
 };
 
+enum { ROWS_MIXED, ROWS_LONG, ROWS_BOTH };
 constexpr int kWideRows = 128, kNarrowRows = 32, kKeys = 32;
 
 // max over lanes l and l ^ 32, every lane gets it
@@ -162,14 +163,14 @@ template <int HD> __device__ __forceinline__ int vperm(int r) { return HD == 128
 // softmax of a row is lane-local up to one exchange with lane ^ 32, and P goes from the accumulators of the first product into the operand
 // of the second without leaving the lane (its 8 keys are 8 half + {0..3, 8..11} + 4 (lane / 32): V^T is read in that order, transposed by
 // ds_read_b64_tr_b16).  P is rounded to bf16 for the second product, as a bf16 model does; sums and maxima are f32.
-template <int HD>
+template <int HD, bool FEW>
 struct WaveRows {
     static constexpr int NS = HD / 16, ND = HD / 32, ROWB = HD * 2;
     bf16x8_t qf[NS];
     f32x16 o[ND];
     float ms, l;                     // about the running maximum, in the exponent (every lane of a row), and the sum (this lane's keys)
     float c1;                        // scale log2 e
-    unsigned ka[NS], va[ND];         // LDS offsets of this lane's fragments in a tile
+    unsigned ka, va;                 // LDS offsets of this lane's first fragments in a tile: the others' differ in one bit field
 
     __device__ __forceinline__ void init(float scale, int lane)
     {
@@ -181,12 +182,10 @@ struct WaveRows {
         l = 0.0f;
         c1 = scale * 1.4426950408889634f;
         const int l32 = lane & 31, h2 = lane >> 5;
-#pragma unroll
-        for (int d = 0; d < NS; d++) ka[d] = (unsigned)(l32 * ROWB + ((2 * d + h2) ^ kperm<HD>(l32)) * 16);
+        ka = (unsigned)(l32 * ROWB + (h2 ^ kperm<HD>(l32)) * 16);
         // lane i of a 16-lane group hands in key i / 4, columns 4 (i % 4) .. + 3 of a 4-key x 16-dim block and gets column i
         const int key = 4 * h2 + ((lane & 15) >> 2), c = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-#pragma unroll
-        for (int d = 0; d < ND; d++) va[d] = (unsigned)(key * ROWB + ((4 * d + c) ^ vperm<HD>(key)) * 16 + (lane & 1) * 8);
+        va = (unsigned)(key * ROWB + (c ^ vperm<HD>(key)) * 16 + (lane & 1) * 8);
     }
     __device__ __forceinline__ void load_q(const uint16_t *q, int h2)
     {
@@ -200,11 +199,13 @@ struct WaveRows {
         for (int s = 0; s < NS; s++) asm volatile("" : : "v"(qf[s]));
     }
     // scores of the 32 keys of K tile kt, the fragments AHEAD products ahead; between(i) is called before product i
-    template <typename F> __device__ __forceinline__ void scores(const unsigned char *kt, f32x16 &s, F between)
+    template <typename F> __device__ __forceinline__ void scores(const unsigned char *lds, unsigned at, f32x16 &s, F between)
     {
         constexpr int AHEAD = 4;
         bf16x8_t kf[AHEAD];
-        auto frag = [&](int i) { return *reinterpret_cast<const bf16x8_t *>(kt + ka[i]); };
+        unsigned k0 = at + ka;
+        if constexpr (FEW) asm volatile("" : "+v"(k0));         // (else hipcc keeps every fragment's address in a register)
+        auto frag = [&](int i) { return *reinterpret_cast<const bf16x8_t *>(lds + (k0 ^ (32u * i))); };
         s = (f32x16){0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < AHEAD; i++) kf[i] = frag(i);
@@ -264,23 +265,25 @@ struct WaveRows {
         ms = l > 0.0f ? ms : -1e30f;
     }
     // O^T += V^T P^T, V tile vt; v: the fragments of its first 16 keys, read before the softmax
-    __device__ __forceinline__ void values(const unsigned char *vt, int kk, bf16x8_t (&v)[ND])
+    __device__ __forceinline__ void values(const unsigned char *lds, unsigned at, int kk, bf16x8_t (&v)[ND])
     {
         typedef __attribute__((address_space(3))) bf16x4_t *lds4;
+        unsigned v0 = at + va;
+        if constexpr (FEW) asm volatile("" : "+v"(v0));
 #pragma unroll
         for (int d = 0; d < ND; d++) {
-            const bf16x4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(vt + va[d] + kk * 16 * ROWB));
-            const bf16x4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(vt + va[d] + (kk * 16 + 8) * ROWB));
+            const bf16x4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(lds + (v0 ^ (64u * d)) + kk * 16 * ROWB));
+            const bf16x4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(lds + (v0 ^ (64u * d)) + (kk * 16 + 8) * ROWB));
             v[d] = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
         }
     }
-    __device__ __forceinline__ void accumulate(const unsigned char *vt, const f32x16 &s, bf16x8_t (&v)[ND])
+    __device__ __forceinline__ void accumulate(const unsigned char *lds, unsigned at, const f32x16 &s, bf16x8_t (&v)[ND])
     {
 #pragma unroll
         for (int kk = 0; kk < 2; kk++) {
             const int e0 = kk * 8;
             bf16x8_t next[ND];
-            if (kk == 0) values(vt, 1, next);
+            if (kk == 0) values(lds, at, 1, next);
             uint4 pb;
             pb.x = f32x2_to_bf16x2(s[e0], s[e0 + 1]);
             pb.y = f32x2_to_bf16x2(s[e0 + 2], s[e0 + 3]);
@@ -298,20 +301,32 @@ struct WaveRows {
 };
 
 // Four waves.  Two forms of a workgroup, by KeySet::narrow:
-//   wide    128 rows, a wave 32 of them.  K / V tiles of 32 keys come by LDS-DMA into two buffers, the next tile in flight while this one is
-//           multiplied, one barrier a tile.
+//   wide    128 rows, a wave 32 of them.  K / V tiles of 32 keys come by LDS-DMA into a ring of buffers, the next tile (ROWS_BOTH: the next
+//           two) in flight while this one is multiplied, one barrier a tile.
 //   narrow  32 rows, shared by the waves: a wave takes every fourth tile of 32 keys, by itself (its own K and V buffer, the next K in flight
 //           from the end of the first product on, no barrier), and the four results are joined in LDS.  For the few rows of a decode step,
 //           whose work is bringing the keys: 128 rows would leave three waves idle.
-// LONG: every workgroup is wide and its rows packed (known to hipcc: 4 % on a long prompt over the kernel that decides at run time)
-template <int HD, bool LONG>
-__global__ __launch_bounds__(256, LONG ? 3 : 2) void k_attn_rows(const RowsParams p)
+// and three instances of the kernel:
+//   ROWS_LONG    every workgroup is wide and its rows packed.  Three workgroups a CU (165 registers, 32 KB).  Bound by the matrix unit and
+//                the vector unit in turn, at the clock that the power budget leaves (a tile of a wave: 512 clocks of products, ~400 of
+//                softmax): one prompt of 8191 tokens, 40 / 8 heads of 128, 625-655 us = 1.05-1.10 PFLOP/s.
+//   ROWS_MIXED   either form, decided at run time.  Two workgroups a CU (narrow: 68 KB, for four waves' buffers and results).  Bound by the
+//                latency of a few dependent loads: a step of 64 rows behind 2048 shared keys 11 us + 4 us for the join.
+//   ROWS_BOTH    wide and narrow ones that share a CU, where both key sets fill the device: two that multiply beside one that waits for
+//                memory.  A narrow workgroup has three waves with keys, so that three workgroups fit a CU's LDS, and fragment addresses are
+//                worked out again for every tile (two registers instead of twelve, so that three fit its registers).  Beside the other
+//                key set's traffic a tile takes longer to come than to multiply, so wide ones bring two ahead.  64 rows of 5 tokens behind
+//                8001 keys, 40 / 8 heads: 102 us (ROWS_MIXED 107); 48 rows of 4 behind 16000 110 us (124); 64 rows of 3 behind 4000, 14 / 2
+//                heads of 64, 18.4 us (19.7).  In the other two neither pays (ROWS_LONG with both: 1 % slower, ROWS_MIXED 2 %).
+template <int HD, int FORM>
+__global__ __launch_bounds__(256, FORM == ROWS_MIXED ? 2 : 3) void k_attn_rows(const RowsParams p)
 {
-    constexpr int ROWB = HD * 2, ND = HD / 32;
+    constexpr bool LONG = FORM == ROWS_LONG;
+    constexpr int ROWB = HD * 2, ND = HD / 32, NW = FORM == ROWS_BOTH ? 3 : 4, RING = FORM == ROWS_BOTH ? 3 : 2;
     constexpr int CH = HD / 8, PK = 1024 / ROWB;               // chunks of a key, keys of a DMA instruction
     constexpr int TILE = kKeys * ROWB;
     constexpr int JROW = HD * 4 + 16, JWAVE = 32 * JROW;        // narrow: a wave's result in LDS, rows padded by one chunk
-    constexpr int BYTES = LONG ? 4 * TILE : 8 * TILE > 4 * JWAVE + 1024 ? 8 * TILE : 4 * JWAVE + 1024;
+    constexpr int BYTES = LONG ? 2 * RING * TILE : 2 * NW * TILE > NW * (JWAVE + 256) ? 2 * NW * TILE : NW * (JWAVE + 256);
     __shared__ __attribute__((aligned(1024))) unsigned char lds[BYTES];
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l32 = lane & 31, h2 = lane >> 5;
@@ -319,7 +334,7 @@ __global__ __launch_bounds__(256, LONG ? 3 : 2) void k_attn_rows(const RowsParam
     // waits for memory (own keys), then what is left of either.
     bool second = false;
     int wg = blockIdx.x;
-    if (!LONG && p.joint) second = true;
+    if (FORM == ROWS_MIXED && p.joint) second = true;
     else if (!LONG) {
         const int blk = wg >> 8;
         if (blk < 2 * p.pairs) {
@@ -381,7 +396,7 @@ __global__ __launch_bounds__(256, LONG ? 3 : 2) void k_attn_rows(const RowsParam
     const int n = n1 - n0, w0 = row0 + (narrow ? 0 : wid * 32), row = w0 + l32, t = row / G, g = row - t * G;
     const bool ok = t < n;
     const int tok = n0 + (ok ? t : 0), head = kvh * G + (ok ? g : 0);
-    WaveRows<HD> w;
+    WaveRows<HD, FORM == ROWS_BOTH> w;
     w.load_q(p.q + (int64_t)tok * p.q_ts + (int64_t)head * HD, h2);       // in flight while the limits are looked up
     int lim, wmax, wmin, kmax;                                 // keys this lane's row sees; most and fewest of the wave's rows; most of the block's
     if (mode == ROWS_PACKED) {
@@ -430,45 +445,61 @@ __global__ __launch_bounds__(256, LONG ? 3 : 2) void k_attn_rows(const RowsParam
 #pragma unroll
         for (int j = 0; j < PIECES; j++) ro[j] = (unsigned)(drow + j * 4 * PK) * ts2;
         // piece j of K (j < PIECES) or V of tile kt; past the end of the block's keys: the last key again, masked below
-        auto piece = [&](int kt, int j) {
+        auto piece = [&](int kt, unsigned at, int j) {
             const bool v = j >= PIECES;
             const int jj = v ? j - PIECES : j;
             const unsigned end = (unsigned)min(kmax - 1 - kt * kKeys, kKeys - 1) * ts2;
-            const unsigned dst = lbase + (unsigned)(kt & 1) * (2 * TILE) + (unsigned)wid * 1024u + (unsigned)((v ? TILE : 0) + jj * 4096);
+            const unsigned dst = lbase + at + (unsigned)wid * 1024u + (unsigned)((v ? TILE : 0) + jj * 4096);
             ROWS_DMA(min(ro[jj], end) + (v ? vch : kch), (v ? vsrc : ksrc) + (int64_t)kt * kKeys * (int64_t)ts2, dst);
         };
-        if (kt0 < kt1)
+        auto whole = [&](int kt, unsigned at) {
 #pragma unroll
-            for (int j = 0; j < 2 * PIECES; j++) piece(kt0, j);
+            for (int j = 0; j < 2 * PIECES; j++) piece(kt, at, j);
+        };
+        if (kt0 < kt1) whole(kt0, 0);
+        if (RING == 3 && kt0 + 1 < kt1) whole(kt0 + 1, 2 * TILE);
         w.wait_q();
-        auto landed = [&]() {                                  // the tile has landed, and the other buffer is no longer read
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        // the tile has landed (the next one may still be on its way), and the buffer before it is no longer read
+        auto landed = [&](bool next) {
+            if (RING == 2 || !next) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            else if (PIECES == 2) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+            else asm volatile("s_waitcnt vmcnt(2)" ::: "memory");
             __syncthreads();
         };
+        unsigned at = 0, far = (RING - 1) * 2 * TILE;          // buffers of this tile and of the one that is brought meanwhile
+        auto on = [&]() {
+            at = at == (RING - 1) * 2 * TILE ? 0 : at + 2 * TILE;
+            far = far == (RING - 1) * 2 * TILE ? 0 : far + 2 * TILE;
+        };
         auto tile = [&](int kt, auto more) {
-            landed();
             const int kbase = kt * kKeys;
-            const unsigned char *buf = lds + (kt & 1) * (2 * TILE);
             f32x16 s;
-            w.scores(buf, s, [&](int i) {
+            w.scores(lds, at, s, [&](int i) {
                 if constexpr (decltype(more)::value)
-                    if (i % 2 == 0) piece(kt + 1, i / 2);
+                    if (i % 2 == 0) piece(kt + RING - 1, far, i / 2);
             });
             bf16x8_t v[ND];
-            w.values(buf + TILE, 0, v);
+            w.values(lds, at + TILE, 0, v);
             w.softmax(s, kbase + kKeys > wmin, lim - kbase - 4 * h2, kt == kt0);
-            w.accumulate(buf + TILE, s, v);
+            w.accumulate(lds, at + TILE, s, v);
+            on();
         };
         if (wmax == 0)                                         // a wave without rows, or whose rows see nothing: brings its pieces only
             for (int kt = kt0; kt < kt1; kt++) {
-                landed();
-                if (kt + 1 < kt1)
-#pragma unroll
-                    for (int j = 0; j < 2 * PIECES; j++) piece(kt + 1, j);
+                landed(kt + 1 < kt1);
+                if (kt + RING - 1 < kt1) whole(kt + RING - 1, far);
+                on();
             }
-        else if (kt0 < kt1) {
-            for (int kt = kt0; kt + 1 < kt1; kt++) tile(kt, std::true_type{});
-            tile(kt1 - 1, std::false_type{});
+        else {
+            int kt = kt0;
+            for (; kt + RING - 1 < kt1; kt++) {
+                landed(true);
+                tile(kt, std::true_type{});
+            }
+            for (; kt < kt1; kt++) {
+                landed(kt + 1 < kt1);
+                tile(kt, std::false_type{});
+            }
         }
         w.finish();
         if (p.part_o) {
@@ -509,18 +540,20 @@ __global__ __launch_bounds__(256, LONG ? 3 : 2) void k_attn_rows(const RowsParam
     auto issue = [&](int kt, const unsigned char *src, unsigned dst, bool v) {
         const int left = kmax - 1 - kt * kKeys;
         src += (int64_t)kt * kKeys * (int64_t)ts2;
+        int dr = drow;
+        if constexpr (FORM == ROWS_BOTH) asm volatile("" : "+v"(dr));
 #pragma unroll
         for (int j = 0; j < PIECES; j++) {
-            const int r = drow + j * PK;
+            const int r = dr + j * PK;
             const unsigned c = (unsigned)(dpos ^ (v ? vperm<HD>(r) : kperm<HD>(r))) * 16u;
             ROWS_DMA((unsigned)min(r, left) * ts2 + c, src, dst + j * 1024);
         }
     };
-    const unsigned char *kbuf = lds + wid * (2 * TILE), *vbuf = kbuf + TILE;
+    const unsigned kat = (unsigned)wid * (2 * TILE);
     // (a joint workgroup goes through the prefix and then through its own keys)
-    for (int pass = p.joint ? 0 : 1; pass < 2; pass++) {
+    for (int pass = FORM == ROWS_MIXED && p.joint ? 0 : 1; pass < 2; pass++) {
         const bool pre = pass == 0;
-        if (p.joint) {
+        if (FORM == ROWS_MIXED && p.joint) {
             const KeySet &k0 = p.ks[0];
             const int64_t off = (int64_t)kvh * HD;
             ts2 = (unsigned)(pre ? k0.ts : ks.ts) * 2u;
@@ -530,56 +563,58 @@ __global__ __launch_bounds__(256, LONG ? 3 : 2) void k_attn_rows(const RowsParam
             kt1 = (kmax + kKeys - 1) / kKeys;
         }
         const int plim = pre ? kmax : lim, pmin = pre ? kmax : wmin;
-        int kt = kt0 + wid;
+        int kt = wid < NW ? kt0 + wid : kt1;
         if (kt < kt1) {
             issue(kt, ksrc, kdst, false);
             issue(kt, vsrc, vdst, true);
         }
         w.wait_q();
-        for (; kt < kt1; kt += 4) {
-            const bool more = kt + 4 < kt1;
+        for (; kt < kt1; kt += NW) {
+            const bool more = kt + NW < kt1;
             const int kbase = kt * kKeys;
             f32x16 s;
             // (own DMA only, counted in order: K of this tile is behind V of this tile, which is behind K of the next)
             if (PIECES == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
             else asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
-            w.scores(kbuf, s, [](int) {});
+            w.scores(lds, kat, s, [](int) {});
             asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(s) : : "memory");       // the tile's keys have been read
-            if (more) issue(kt + 4, ksrc, kdst, false);
+            if (more) issue(kt + NW, ksrc, kdst, false);
             w.softmax(s, kbase + kKeys > pmin, plim - kbase - 4 * h2, kt == kt0 + wid);
             if (!more) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             else if (PIECES == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
             else asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
             bf16x8_t v[ND];
-            w.values(vbuf, 0, v);
-            w.accumulate(vbuf, s, v);
+            w.values(lds, kat + TILE, 0, v);
+            w.accumulate(lds, kat + TILE, s, v);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            if (more) issue(kt + 4, vsrc, vdst, true);
+            if (more) issue(kt + NW, vsrc, vdst, true);
         }
     }
     w.finish();
     __syncthreads();                                           // the tiles are no longer read
-    float *sml = reinterpret_cast<float *>(lds + 4 * JWAVE);
-    if (h2 == 0) *reinterpret_cast<float2 *>(sml + (wid * 32 + l32) * 2) = make_float2(w.ms, w.l);
+    float *sml = reinterpret_cast<float *>(lds + NW * JWAVE);
+    if (wid < NW) {
+        if (h2 == 0) *reinterpret_cast<float2 *>(sml + (wid * 32 + l32) * 2) = make_float2(w.ms, w.l);
 #pragma unroll
-    for (int d = 0; d < ND; d++)
+        for (int d = 0; d < ND; d++)
 #pragma unroll
-        for (int e = 0; e < 16; e += 4)
-            *reinterpret_cast<float4 *>(lds + wid * JWAVE + l32 * JROW + (32 * d + 2 * e + 4 * h2) * 4) =
-                make_float4(w.o[d][e], w.o[d][e + 1], w.o[d][e + 2], w.o[d][e + 3]);
+            for (int e = 0; e < 16; e += 4)
+                *reinterpret_cast<float4 *>(lds + wid * JWAVE + l32 * JROW + (32 * d + 2 * e + 4 * h2) * 4) =
+                    make_float4(w.o[d][e], w.o[d][e + 1], w.o[d][e + 2], w.o[d][e + 3]);
+    }
     __syncthreads();
     // eight threads a row, each every eighth group of four dims; neighbouring threads at neighbouring rows of a partial result's tile, or at
     // neighbouring groups of a row
     const int jr = p.part_o ? tid & 31 : tid >> 3, jq = p.part_o ? tid >> 5 : tid & 7, jt = (row0 + jr) / G, jg = row0 + jr - jt * G;
     if (jt >= n) return;
-    float mj[4], wj[4], m = -1e30f, l = 0.0f;
+    float mj[NW], wj[NW], m = -1e30f, l = 0.0f;
 #pragma unroll
-    for (int u = 0; u < 4; u++) {
+    for (int u = 0; u < NW; u++) {
         mj[u] = sml[(u * 32 + jr) * 2];
         m = fmaxf(m, mj[u]);
     }
 #pragma unroll
-    for (int u = 0; u < 4; u++) {
+    for (int u = 0; u < NW; u++) {
         wj[u] = __builtin_amdgcn_exp2f(mj[u] - m);
         l += sml[(u * 32 + jr) * 2 + 1] * wj[u];
     }
@@ -590,7 +625,7 @@ __global__ __launch_bounds__(256, LONG ? 3 : 2) void k_attn_rows(const RowsParam
     for (int q = jq; q < HD / 4; q += 8) {
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int u = 0; u < 4; u++) {
+        for (int u = 0; u < NW; u++) {
             const float4 v = *reinterpret_cast<const float4 *>(lds + u * JWAVE + jr * JROW + q * 16);
             a.x += v.x * wj[u]; a.y += v.y * wj[u]; a.z += v.z * wj[u]; a.w += v.w * wj[u];
         }
@@ -728,7 +763,7 @@ static void plan_keys(KeySet *k, int mode, int64_t seq_rows, int64_t blocks_wide
     k->blocks = (int)blocks;
     k->max_keys = max_keys;
     const int tiles = (max_keys + kKeys - 1) / kKeys, least = k->narrow ? 8 : 4;
-    const int64_t want = 2 * (int64_t)device_cu_count_physical() / (blocks * nkv > 0 ? blocks * nkv : 1);
+        const int64_t want = 2 * (int64_t)device_cu_count_physical() / (blocks * nkv > 0 ? blocks * nkv : 1);
     int parts = (int)(want < 1 ? 1 : want > 64 ? 64 : want);
     if (mode == ROWS_PACKED && !k->narrow && tiles <= 16) parts = 1;
     while (2 * (int64_t)parts * parts > 5 * (int64_t)tiles && parts > 1) parts--;
@@ -748,14 +783,18 @@ static void fewer_parts(KeySet *k)
     k->parts = (tiles + k->part_tiles - 1) / k->part_tiles;
 }
 
-static void rows_launch(const RowsParams &p, int hd, int64_t workgroups, hipStream_t st)
+static void rows_launch(const RowsParams &p, int hd, int form, int64_t workgroups, hipStream_t st)
 {
     const dim3 grid((unsigned)workgroups), block(256);
-    const bool lng = p.ks[0].mode == ROWS_PACKED && !p.ks[0].narrow;
-    if (hd == 128 && lng) hipLaunchKernelGGL((k_attn_rows<128, true>), grid, block, 0, st, p);
-    else if (hd == 128) hipLaunchKernelGGL((k_attn_rows<128, false>), grid, block, 0, st, p);
-    else if (lng) hipLaunchKernelGGL((k_attn_rows<64, true>), grid, block, 0, st, p);
-    else hipLaunchKernelGGL((k_attn_rows<64, false>), grid, block, 0, st, p);
+#define ROWS_GO(HD, FORM) hipLaunchKernelGGL((k_attn_rows<HD, FORM>), grid, block, 0, st, p)
+    if (form == ROWS_LONG) {
+        if (hd == 128) ROWS_GO(128, ROWS_LONG); else ROWS_GO(64, ROWS_LONG);
+    } else if (form == ROWS_BOTH) {
+        if (hd == 128) ROWS_GO(128, ROWS_BOTH); else ROWS_GO(64, ROWS_BOTH);
+    } else {
+        if (hd == 128) ROWS_GO(128, ROWS_MIXED); else ROWS_GO(64, ROWS_MIXED);
+    }
+#undef ROWS_GO
 }
 
 static void join_launch(const RowsParams &p, int hd, int parts, hipStream_t st)
@@ -828,7 +867,7 @@ extern "C" int ifh_attn_packed_bf16(const ifh_attn_packed_desc *d, ifh_stream_t 
     const int64_t wgs = (int64_t)k.blocks * p.nkv * k.parts;
     p.first = (int)wgs;
     hipStream_t st = as_stream(stream);
-    rows_launch(p, d->head_dim, wgs, st);
+    rows_launch(p, d->head_dim, k.narrow ? ROWS_MIXED : ROWS_LONG, wgs, st);
     IFH_LAUNCH_CHECK("attn_packed");
     if (p.part_o) {
         join_launch(p, d->head_dim, k.parts, st);
@@ -895,7 +934,7 @@ extern "C" int ifh_attn_prefix_bf16(const ifh_attn_prefix_desc *d, ifh_stream_t 
     hipStream_t st = as_stream(stream);
     if (prefix_joint((int64_t)b.blocks * p.nkv, d->prefix_keys, d->max_keys, b.narrow)) {
         p.joint = 1;
-        rows_launch(p, d->head_dim, (int64_t)b.blocks * p.nkv, st);
+        rows_launch(p, d->head_dim, ROWS_MIXED, (int64_t)b.blocks * p.nkv, st);
         IFH_LAUNCH_CHECK("attn_prefix joint");
         return IFH_OK;
     }
@@ -912,7 +951,7 @@ extern "C" int ifh_attn_prefix_bf16(const ifh_attn_prefix_desc *d, ifh_stream_t 
         b = t;
         p.first = (int)nb;
     }
-    rows_launch(p, d->head_dim, na + nb, st);
+    rows_launch(p, d->head_dim, p.pairs > 0 ? ROWS_BOTH : ROWS_MIXED, na + nb, st);
     IFH_LAUNCH_CHECK("attn_prefix");
     join_launch(p, d->head_dim, parts, st);
     IFH_LAUNCH_CHECK("attn_prefix join");
