@@ -31,6 +31,8 @@ __device__ __forceinline__ int packed_seq(const int32_t *__restrict__ cu, int n,
 }
 
 // One thread per (token, head slot, 8 pairs j .. j + 7 of the head): the arithmetic and the roundings of k_rope_append (llm.hip).
+// Bound by memory: qkv read once, q and k | v written once (64 prompts of 12 / 2 heads of 128, 87 MB: 18.3 us = 4.7 TB/s, where a large
+// copy reaches 4.9); the loads start before the sequence is looked up, whose chain would otherwise stand in front of them (+2 us).
 __global__ __launch_bounds__(256) void k_rope_packed(const uint16_t *__restrict__ qkv, int64_t qkv_ld, uint16_t *__restrict__ q_out,
                                                      int64_t q_ld, const float *__restrict__ cs, int table_len,
                                                      uint16_t *__restrict__ cache, int64_t cache_bs, int64_t cache_ts,
@@ -636,9 +638,11 @@ __global__ __launch_bounds__(256, FORM == ROWS_MIXED ? 2 : 3) void k_attn_rows(c
     }
 }
 
-// out = sum_j o_j 2^(m_j - m) / sum_j l_j 2^(m_j - m) over the parts j, a workgroup 32 DG dims of a tile of 32 rows: thread (row, q) sums DG
-// groups of four dims (512 bytes in a row for 32 neighbours), eight loads in flight, and works out the weights of every eighth part.  The
-// result goes through LDS so that a row's dims are stored in a row.  DG: whole rows where there are tiles for the device, else 32 dims.
+// out = sum_j o_j 2^(m_j - m) / sum_j l_j 2^(m_j - m) over the parts j.  Bound by the partial results' bytes where there are many rows
+// (12 800 rows of 128 in 5 parts, 33 MB: 7.5 us = 4.4 TB/s), by a few dependent loads otherwise (4 us).  A workgroup takes 32 DG dims of a
+// tile of 32 rows: thread (row, q) sums DG groups of four dims (512 bytes in a row for 32 neighbours), eight loads in flight, and works
+// out the weights of every eighth part.  The result goes through LDS so that a row's dims are stored in a row.  DG: whole rows where there
+// are tiles for the device, else 32 dims.
 constexpr int kMaxParts = 128;
 template <int HD, int DG>
 __global__ __launch_bounds__(256) void k_attn_join(const float *__restrict__ part_o, const float *__restrict__ part_ml, int row_tiles, int nkv,
@@ -945,7 +949,8 @@ extern "C" int ifh_attn_prefix_bf16(const ifh_attn_prefix_desc *d, ifh_stream_t 
     p.pairs = (int)((na < nb ? na : nb) / 256);
     if (p.pairs == 0) {
         // few of either: the own keys' workgroups (more steps each) start first.  64 rows behind 2048 keys: 14.8 us, the prefix first 15.9;
-        // where both fill the device the other order is better (64 rows of 5 tokens behind 8001 keys: 110 us against 117)
+        // where both fill the device dealing them in turn, the prefix first, is better (64 rows of 5 tokens behind 8001 keys: 110 us, own
+        // keys first 117)
         KeySet t = a;
         a = b;
         b = t;
