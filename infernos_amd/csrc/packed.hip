@@ -313,7 +313,7 @@ struct WaveRows {
 //                the vector unit in turn, at the clock that the power budget leaves (a tile of a wave: 512 clocks of products, ~400 of
 //                softmax): one prompt of 8191 tokens, 40 / 8 heads of 128, 625-655 us = 1.05-1.10 PFLOP/s.
 //   ROWS_MIXED   either form, decided at run time.  Two workgroups a CU (narrow: 68 KB, for four waves' buffers and results).  Bound by the
-//                latency of a few dependent loads: a step of 64 rows behind 2048 shared keys 11 us + 4 us for the join.
+//                latency of a few dependent loads: a step of 64 rows behind 2048 shared keys 10.5 us + 4 us for the join.
 //   ROWS_BOTH    wide and narrow ones that share a CU, where both key sets fill the device: two that multiply beside one that waits for
 //                memory.  A narrow workgroup has three waves with keys, so that three workgroups fit a CU's LDS, and fragment addresses are
 //                worked out again for every tile (two registers instead of twelve, so that three fit its registers).  Beside the other
@@ -754,26 +754,37 @@ extern "C" int ifh_rope_append_packed_bf16(const ifh_rope_packed_desc *d, ifh_st
 // Narrow workgroups where a narrow block holds a sequence's rows: with more, its keys are read once for every 32 rows.  Measured, narrow and
 // wide: 36 rows of 32 sequences behind 1000 keys 18.9 and 14.2 us, 64 rows of 4 behind 4000 16.3 and 15.3 us; with 6 rows (a decode step
 // of 64 sequences behind 1000 keys) 17.6 and 24 us.
+// A prefix is read by narrow ones as long as seven workgroups for eight CUs do and their rows are four fifths full: its keys then come to
+// four waves at once (64 rows of 12 / 2 heads behind 2048 keys 14.5 us, wide 15.3; behind 8000 21.9 and 20.1; 96 rows behind 2048 17.6 and
+// 16.5; 8 rows of 40 / 8 heads, 40 rows in two blocks, behind 4000 15.7 and 13.9).
 // Keys are split into parts until the device has two workgroups a CU, and no further than that pays for the join's launch (2.5 us) and for
 // what each part costs it: none of fewer than eight tiles (narrow: two a wave) or four (wide), wide blocks of up to 512 keys not at all
 // unless the results are joined anyway (64 sequences, 300 keys: 7.4 us, split 9.4 us; one prompt of 300 rows 9.4, split 11.9 us; of 700 keys 15.7, split 12.8 us), and at most
 // 1.6 sqrt(tiles) parts, the time of a part being tiles / parts and that of the join parts (4 sequences of 4000 keys: 31 parts 15.7 us, 16
 // parts 14.0 us, 10 parts 15.5 us; one of 8000: 63 parts 17.2 us, 25 parts 15.6 us, 15 parts 17.7 us).
-static void plan_keys(KeySet *k, int mode, int64_t seq_rows, int64_t blocks_wide, int64_t blocks_narrow, int nkv, int max_keys)
+static void split_keys(KeySet *k, bool narrow, int64_t blocks, int nkv, int max_keys)
 {
-    k->mode = mode;
-    k->narrow = seq_rows <= kNarrowRows;
-    const int64_t blocks = k->narrow ? blocks_narrow : blocks_wide;
+    k->narrow = narrow;
     k->blocks = (int)blocks;
     k->max_keys = max_keys;
-    const int tiles = (max_keys + kKeys - 1) / kKeys, least = k->narrow ? 8 : 4;
-        const int64_t want = 2 * (int64_t)device_cu_count_physical() / (blocks * nkv > 0 ? blocks * nkv : 1);
+    const int tiles = (max_keys + kKeys - 1) / kKeys, least = narrow ? 8 : 4;
+    const int64_t want = 2 * (int64_t)device_cu_count_physical() / (blocks * nkv > 0 ? blocks * nkv : 1);
     int parts = (int)(want < 1 ? 1 : want > 64 ? 64 : want);
-    if (mode == ROWS_PACKED && !k->narrow && tiles <= 16) parts = 1;
+    if (k->mode == ROWS_PACKED && !narrow && tiles <= 16) parts = 1;
     while (2 * (int64_t)parts * parts > 5 * (int64_t)tiles && parts > 1) parts--;
     if (parts > tiles / least) parts = tiles / least > 1 ? tiles / least : 1;
     k->part_tiles = (tiles + parts - 1) / parts;
     k->parts = (tiles + k->part_tiles - 1) / k->part_tiles;
+}
+static void plan_keys(KeySet *k, int mode, int64_t seq_rows, int64_t blocks_wide, int64_t blocks_narrow, int nkv, int max_keys)
+{
+    k->mode = mode;
+    const bool full = blocks_narrow * kNarrowRows * 4 <= seq_rows * 5;
+    if (seq_rows <= kNarrowRows || (mode == ROWS_PREFIX && full)) {
+        split_keys(k, true, blocks_narrow, nkv, max_keys);
+        if (seq_rows <= kNarrowRows || blocks_narrow * nkv * k->parts * 8 <= 7 * (int64_t)device_cu_count_physical()) return;
+    }
+    split_keys(k, false, blocks_wide, nkv, max_keys);
 }
 
 static int64_t part_floats(int64_t row_tiles, int nkv, int parts, int hd) { return row_tiles * nkv * parts * 32 * (hd + 2); }
