@@ -279,6 +279,16 @@ def test_attn_prefix_batches(dev, heads, B, T, P, own):
     print('attn_prefix ok', heads, B, T, P, own, 'worst share %.2f' % w)
 
 
+@pytest.mark.parametrize('heads,B,T,P,own', [((40, 8, 128), 64, 5, 1000, 300), ((8, 8, 64), 96, 6, 700, 90), ((16, 1, 128), 96, 6, 3000, 500),
+                                             ((14, 2, 64), 90, 6, 2500, 33), ((40, 8, 128), 40, 7, 97, 2000)])
+def test_attn_prefix_both_key_sets_fill_the_device(dev, heads, B, T, P, own):
+    """hundreds of workgroups of either key set; rows without an own key and rows that use none of the prefix among them"""
+    plen = [0 if b % 11 == 3 else P if b % 4 else 1 + (P * 7 * b) % P for b in range(B)]
+    c = prefix_case(dev, heads, B, T, P, [-1 if b % 13 == 5 else (b * 7919) % (own + 1) for b in range(B)], plen=plen, seed=own)
+    w = check_rows(run_prefix(c, dev).view(-1, heads[0], heads[2]), prefix_rows(c, sample=7), 'prefix')
+    print('attn_prefix ok', heads, B, T, P, own, 'worst share %.2f' % w)
+
+
 def test_attn_prefix_rows_that_see_nothing(dev):
     """no prefix and no key: zeros; no prefix, or no own key: the other alone"""
     heads = (12, 2, 128)
