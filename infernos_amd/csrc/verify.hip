@@ -5,14 +5,13 @@
 // that neither the way a sum is split nor the exponential's rounding moves a border past the number (f32 exponentials would move one in
 // every few hundred draws from a flat tail).  The f64 work (a short polynomial, ~12 operations a logit and as many in f32) stays under the
 // time the logits take to arrive.
-//   k_verify_stats   a wave a chunk of a target row: (max, sum of exp), or the arg-max for temperature 0.  Bound by memory: 320 rows of
+//   k_verify_stats   a wave or four a chunk of a target row: (max, sum of exp), or the arg-max for temperature 0.  Bound by memory: 320 rows of
 //                    151 936 logits, 194 MB, 46 us = 4.2 TB/s
-//   k_verify_mass    a wave a chunk of the refused position, where the draft has a distribution: the mass of max(p - q, 0).  64 rows of both,
+//   k_verify_mass    a wave or four a chunk of the refused position, where the draft has a distribution: the mass of max(p - q, 0).  64 rows of both,
 //                    78 MB, 15.6 us, 4 of them for the verdicts in front
 //   k_verify_draw    a workgroup a row: the chunk and then the token where the cumulated mass passes the uniform number.  A chain of
 //                    dependent loads and scans, 7 us for one row and for 64
-// A chunk is a wave's, 2048 logits: one row of 151 936 is 75 of them, so that one call's few rows still spread over the device, and a wave
-// needs no barrier.
+// A chunk is 2048 logits: one row of 151 936 is 75 of them, so that one call's few rows still spread over the device.
 // The rows' verdicts (which draft is refused) are worked out from the chunk statistics by every workgroup that asks, its waves taking the
 // row's positions in parallel: a launch of its own for them would cost more.
 #include "common.h"
@@ -67,17 +66,18 @@ struct VerifyParams {
 
 // a lane's elements of the chunk at `base`: 16 bytes at a time where the row is aligned, else every 64th
 __device__ __forceinline__ int place(int vec, int base, int lane, int e) { return base + (vec ? (e >> 2) * 256 + lane * 4 + (e & 3) : e * 64 + lane); }
-__device__ __forceinline__ void load_chunk(const float *row, int base, int lane, int vocab, int vec, float fill, float (&v)[VPL])
+template <int N>
+__device__ __forceinline__ void load_chunk(const float *row, int base, int lane, int vocab, int vec, float fill, float (&v)[N])
 {
-    if (vec && base + VC <= vocab) {
+    if (vec && base + 64 * N <= vocab) {
 #pragma unroll
-        for (int e = 0; e < VPL; e += 4) {
+        for (int e = 0; e < N; e += 4) {
             const float4 f = *reinterpret_cast<const float4 *>(row + base + e * 64 + lane * 4);
             v[e] = f.x; v[e + 1] = f.y; v[e + 2] = f.z; v[e + 3] = f.w;
         }
     } else {
 #pragma unroll
-        for (int e = 0; e < VPL; e++) {
+        for (int e = 0; e < N; e++) {
             const int j = place(vec, base, lane, e);
             v[e] = j < vocab ? row[j] : fill;
         }
@@ -128,25 +128,38 @@ __device__ __forceinline__ float wave_max_f(float v)
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
-__global__ __launch_bounds__(VT) void k_verify_stats(const VerifyParams p)
+// W waves a chunk: one (no barrier), or a workgroup's four where there are few chunks for the device, so that a lane has 8 of the f64
+// exponentials and not 32.  Four up to 32 chunks a CU: one row of 3 drafts, 151 936 tokens, 3.4 us (one wave a chunk 4.8), the whole
+// verification of 16 rows of 4 drafts 27.9 us (30.1), but of 64 rows 69.3 us (66.6).
+template <int W> __global__ __launch_bounds__(VT) void k_verify_stats(const VerifyParams p)
 {
+    constexpr int N = VPL / W;
+    __shared__ float ms[W];
+    __shared__ double ss[W];
     const int64_t pos = blockIdx.y;
-    const int lane = threadIdx.x & 63, c = blockIdx.x * 4 + (threadIdx.x >> 6), base = c * VC;
+    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+    const int c = W == 1 ? blockIdx.x * 4 + wid : blockIdx.x, base = c * VC + (W == 1 ? 0 : wid * (VC / W));
     if (c >= p.nch) return;
-    float v[VPL];
-    load_chunk(p.logits + pos * p.ld, base, lane, p.vocab, p.vec, -INFINITY, v);
+    float v[N];
+    load_chunk<N>(p.logits + pos * p.ld, base, lane, p.vocab, p.vec, -INFINITY, v);
     float m = -INFINITY;
 #pragma unroll
-    for (int e = 0; e < VPL; e++) {
+    for (int e = 0; e < N; e++) {
         v[e] = logit(v[e]);
         m = fmaxf(m, v[e]);
     }
     m = wave_max_f(m);
+    if (W > 1) {
+        if (lane == 0) ms[wid] = m;
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < W; k++) m = fmaxf(m, ms[k]);
+    }
     double s = 0.0;
     if (p.greedy) {
         int at = 0x7fffffff;                                 // the first place of the maximum
 #pragma unroll
-        for (int e = 0; e < VPL; e++)
+        for (int e = 0; e < N; e++)
             if (v[e] == m) at = min(at, place(p.vec, base, lane, e));
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) at = min(at, __shfl_xor(at, o, 64));
@@ -155,13 +168,20 @@ __global__ __launch_bounds__(VT) void k_verify_stats(const VerifyParams p)
         const double md = (double)fmaxf(m, -kFltMax);
         double s1 = 0.0;
 #pragma unroll
-        for (int e = 0; e < VPL; e += 2) {
+        for (int e = 0; e < N; e += 2) {
             s += exp_neg(((double)v[e] - md) * p.inv_temp);
             s1 += exp_neg(((double)v[e + 1] - md) * p.inv_temp);
         }
         s = wave_sum_d(s + s1);
     }
-    if (lane == 0) {
+    if (W > 1) {
+        if (lane == 0) ss[wid] = s;
+        __syncthreads();
+        s = ss[0];
+#pragma unroll
+        for (int k = 1; k < W; k++) s = p.greedy ? fmin(s, ss[k]) : s + ss[k];
+    }
+    if (W == 1 ? lane == 0 : threadIdx.x == 0) {
         p.cmax[pos * p.nch + c] = m;
         p.csum[pos * p.nch + c] = s;
     }
@@ -236,29 +256,42 @@ template <int NT> __device__ __forceinline__ Verdict verdict_of(const VerifyPara
     return w;
 }
 
-__global__ __launch_bounds__(VM) void k_verify_mass(const VerifyParams p)
+// W waves a chunk, as above: four up to 12 chunks a CU (the whole verification of one row 13.8 us, one wave a chunk 15.5; 32 rows 43.6 and
+// 44.3; 64 rows 72.7 and 70.8)
+template <int W> __global__ __launch_bounds__(VM) void k_verify_mass(const VerifyParams p)
 {
+    constexpr int N = VPL / W;
     __shared__ VerdictLds L;
-    const int r = blockIdx.y, lane = threadIdx.x & 63, c = blockIdx.x * (VM / 64) + (threadIdx.x >> 6), base = c * VC;
+    __shared__ double ss[VM / 64];
+    const int r = blockIdx.y, lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+    const int c = blockIdx.x * (VM / 64 / W) + wid / W, base = c * VC + wid % W * (VC / W);
     const Verdict w = verdict_of<VM>(p, r, L);
-    if (c >= p.nch || !w.refused || !(w.s > 0.0)) return;
-    float v[VPL], q[VPL];
-    load_chunk(p.logits + ((int64_t)r * (p.T + 1) + w.kept) * p.ld, base, lane, p.vocab, p.vec, -INFINITY, v);
-    load_chunk(p.q + ((int64_t)r * p.T + w.kept) * p.q_ld, base, lane, p.vocab, p.qvec && p.vec, 0.0f, q);
+    if (!w.refused || !(w.s > 0.0) || (W == 1 && c >= p.nch)) return;
+    const float *lrow = p.logits + ((int64_t)r * (p.T + 1) + w.kept) * p.ld, *qrow = p.q + ((int64_t)r * p.T + w.kept) * p.q_ld;
+    float v[N], q[N];
+    load_chunk<N>(lrow, base, lane, p.vocab, p.vec, -INFINITY, v);
+    load_chunk<N>(qrow, base, lane, p.vocab, p.qvec && p.vec, 0.0f, q);
     if (p.vec && !p.qvec) {                                  // (the two rows have to be read in one order)
 #pragma unroll
-        for (int e = 0; e < VPL; e++) {
+        for (int e = 0; e < N; e++) {
             const int j = place(1, base, lane, e);
-            q[e] = j < p.vocab ? p.q[((int64_t)r * p.T + w.kept) * p.q_ld + j] : 0.0f;
+            q[e] = j < p.vocab ? qrow[j] : 0.0f;
         }
     }
     const double inv_s = 1.0 / w.s;
     double s = 0.0;
 #pragma unroll
-    for (int e = 0; e < VPL; e++)
+    for (int e = 0; e < N; e++)
         s += fmax(__builtin_fma(exp_neg(((double)logit(v[e]) - (double)w.m) * p.inv_temp), inv_s, -(double)q[e]), 0.0);
     s = wave_sum_d(s);
-    if (lane == 0) p.mass[(int64_t)r * p.nch + c] = s;
+    if (W > 1) {
+        if (lane == 0) ss[wid] = s;
+        __syncthreads();
+        if (wid % W) return;
+#pragma unroll
+        for (int k = 1; k < W; k++) s += ss[wid + k];
+    }
+    if (lane == 0 && c < p.nch) p.mass[(int64_t)r * p.nch + c] = s;
 }
 
 // inclusive sums over the workgroup's threads, in thread order, and the whole
@@ -475,10 +508,16 @@ extern "C" int ifh_verify_drafts_f32(const ifh_verify_desc *d, ifh_stream_t stre
     p.mass = p.csum + positions * p.nch;
     p.cmax = (float *)(p.mass + (int64_t)d->nrows * p.nch);
     hipStream_t st = as_stream(stream);
-    hipLaunchKernelGGL(k_verify_stats, dim3((unsigned)(p.nch + 3) / 4, (unsigned)positions), dim3(VT), 0, st, p);
+    if (positions * p.nch <= 32 * (int64_t)device_cu_count_physical())
+        hipLaunchKernelGGL(k_verify_stats<4>, dim3((unsigned)p.nch, (unsigned)positions), dim3(VT), 0, st, p);
+    else
+        hipLaunchKernelGGL(k_verify_stats<1>, dim3((unsigned)(p.nch + 3) / 4, (unsigned)positions), dim3(VT), 0, st, p);
     IFH_LAUNCH_CHECK("verify stats");
     if (!p.greedy && p.q && p.T > 0) {
-        hipLaunchKernelGGL(k_verify_mass, dim3((unsigned)(p.nch + VM / 64 - 1) / (VM / 64), (unsigned)p.nrows), dim3(VM), 0, st, p);
+        if ((int64_t)p.nrows * p.nch <= 12 * (int64_t)device_cu_count_physical())
+            hipLaunchKernelGGL(k_verify_mass<4>, dim3((unsigned)(p.nch + VM / 256 - 1) / (VM / 256), (unsigned)p.nrows), dim3(VM), 0, st, p);
+        else
+            hipLaunchKernelGGL(k_verify_mass<1>, dim3((unsigned)(p.nch + VM / 64 - 1) / (VM / 64), (unsigned)p.nrows), dim3(VM), 0, st, p);
         IFH_LAUNCH_CHECK("verify mass");
     }
     hipLaunchKernelGGL(k_verify_draw, dim3((unsigned)p.nrows), dim3(VD), 0, st, p);
