@@ -23,26 +23,34 @@ constexpr int VM = 512, VD = 1024;                      // threads of the mass a
 constexpr int kVerifyMaxChunks = 256;                   // 524 288 tokens: the draw gives each chunk a thread
 constexpr float kFltMax = 3.402823466e38f;
 
-// e^x for x <= 0 in f64, relative error below 1e-10: x = k ln 2 + r, |r| <= ln 2 / 2 (k by adding and taking off 1.5 2^52), the Taylor
-// polynomial of degree 9, of which the part from r^4 on, no more than 6e-4 of the whole, is f32
-__device__ __forceinline__ double exp_neg(double x)
+// 2^(j / 32)
+__device__ const double kExp2[32] = {
+    1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237, 1.0905077326652577, 1.1143867425958924,
+    1.1387886347566916, 1.1637248587775775, 1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332,
+    1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832, 1.4142135623730951, 1.4451808069770467,
+    1.4768261459394993, 1.5091644275934228, 1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.6457554781539649,
+    1.681792830507429, 1.7186192981224779, 1.7562521603732995, 1.7947090750031072, 1.8340080864093424, 1.8741676341103,
+    1.9152065613971474, 1.9571441241754002
+};
+__device__ __forceinline__ void exp_table(double entry, double (&tab)[32])       // entry: kExp2[threadIdx.x % 32], on its way
+{
+    if (threadIdx.x < 32) tab[threadIdx.x] = entry;
+    __syncthreads();
+}
+// e^x for x <= 0 in f64, relative error below 3e-11; y = x 32 / ln 2.  y = k + u, |u| <= 1/2 (k by adding and taking off 1.5 2^52), and
+// 2^(k/32) comes from the table (LDS: its 32 entries lie in 64 different banks) and k / 32.  e^(u ln 2 / 32) is 1, the linear term in f64,
+// and the Taylor polynomial's terms 2 to 4, no more than 6e-5 of the whole, in f32.  (Without a table, a polynomial of degree 9, it was
+// 27 operations a logit instead of 19.)
+__device__ __forceinline__ double exp_neg(double y, const double (&tab)[32])
 {
     const double big = 6755399441055744.0;
-    const double kb = __builtin_fma(fmax(x, -745.0), 1.4426950408889634, big), k = kb - big;
-    const double r = __builtin_fma(k, -0.6931471805599453, fmax(x, -745.0));
-    const float f = (float)r;
-    float t = 2.7557319e-6f;                               // 1 / 9!
-    t = __builtin_fmaf(t, f, 2.4801587e-5f);
-    t = __builtin_fmaf(t, f, 1.9841270e-4f);
-    t = __builtin_fmaf(t, f, 1.3888889e-3f);
-    t = __builtin_fmaf(t, f, 8.3333333e-3f);
-    t = __builtin_fmaf(t, f, 4.1666667e-2f);
-    double e = __builtin_fma((double)t, r, 0.16666666666666666);
-    e = __builtin_fma(e, r, 0.5);
-    e = __builtin_fma(e, r, 1.0);
-    e = __builtin_fma(e, r, 1.0);
-    const double v = __builtin_ldexp(e, (int)k);
-    return x > -745.0 ? v : 0.0;
+    y = fmax(y, -40000.0);
+    const double kb = y + big, u = y - (kb - big);
+    const int k = (int)(uint32_t)__builtin_bit_cast(uint64_t, kb);
+    const float f = (float)u;
+    const float g = f * f * __builtin_fmaf(__builtin_fmaf(f, 9.1725627e-09f, 1.69385097e-06f), f, 0.000234596198f);
+    const double t = tab[k & 31];
+    return __builtin_ldexp(__builtin_fma(t, __builtin_fma(u, 0.02166084939249829, (double)g), t), k >> 5);
 }
 
 // NaN counts as -inf; +inf as the largest finite value (its differences stay finite)
@@ -57,7 +65,7 @@ struct VerifyParams {
     const float *uniform;
     int32_t *out_tokens, *out_count;
     int vocab, nrows, T, nch;
-    double inv_temp;
+    double rate;                 // 32 / (ln 2 temperature)
     int greedy, vec, qvec;
     double *csum;                // [rows * (T+1)][nch] chunk sums of exp((l - cmax) / temperature); greedy: the place of the chunk's maximum
     double *mass;                // [rows][nch]
@@ -135,13 +143,15 @@ template <int W> __global__ __launch_bounds__(VT) void k_verify_stats(const Veri
 {
     constexpr int N = VPL / W;
     __shared__ float ms[W];
-    __shared__ double ss[W];
+    __shared__ double ss[W], tab[32];
     const int64_t pos = blockIdx.y;
     const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
     const int c = W == 1 ? blockIdx.x * 4 + wid : blockIdx.x, base = c * VC + (W == 1 ? 0 : wid * (VC / W));
-    if (c >= p.nch) return;
+    const double entry = kExp2[threadIdx.x & 31];
     float v[N];
     load_chunk<N>(p.logits + pos * p.ld, base, lane, p.vocab, p.vec, -INFINITY, v);
+    exp_table(entry, tab);
+    if (c >= p.nch) return;
     float m = -INFINITY;
 #pragma unroll
     for (int e = 0; e < N; e++) {
@@ -169,8 +179,8 @@ template <int W> __global__ __launch_bounds__(VT) void k_verify_stats(const Veri
         double s1 = 0.0;
 #pragma unroll
         for (int e = 0; e < N; e += 2) {
-            s += exp_neg(((double)v[e] - md) * p.inv_temp);
-            s1 += exp_neg(((double)v[e + 1] - md) * p.inv_temp);
+            s += exp_neg(((double)v[e] - md) * p.rate, tab);
+            s1 += exp_neg(((double)v[e + 1] - md) * p.rate, tab);
         }
         s = wave_sum_d(s + s1);
     }
@@ -200,7 +210,7 @@ struct VerdictLds {
     int best[64], keep[64];
 };
 
-template <int NT> __device__ __forceinline__ Verdict verdict_of(const VerifyParams &p, int r, VerdictLds &L)
+template <int NT> __device__ __forceinline__ Verdict verdict_of(const VerifyParams &p, int r, VerdictLds &L, const double (&tab)[32])
 {
     const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
     const int n = p.lens ? min(max(p.lens[r], 0), p.T) : p.T;
@@ -234,11 +244,11 @@ template <int NT> __device__ __forceinline__ Verdict verdict_of(const VerifyPara
             // (no chunk with a finite maximum: every sum is 0)
 #pragma unroll
             for (int k = 0; k < kVerifyMaxChunks / 64; k++)
-                if (k * 64 < p.nch) s += cs[k] * exp_neg(((double)fmaxf(cm[k], -kFltMax) - (double)fmaxf(m, -kFltMax)) * p.inv_temp);
+                if (k * 64 < p.nch) s += cs[k] * exp_neg(((double)fmaxf(cm[k], -kFltMax) - (double)fmaxf(m, -kFltMax)) * p.rate, tab);
             s = wave_sum_d(s);
         }
         if (lane == 0) {
-            const double px = !in || !any ? 0.0 : p.greedy ? (x == best ? 1.0 : 0.0) : exp_neg(((double)logit(lx) - (double)m) * p.inv_temp) / s;
+            const double px = !in || !any ? 0.0 : p.greedy ? (x == best ? 1.0 : 0.0) : exp_neg(((double)logit(lx) - (double)m) * p.rate, tab) / s;
             L.keep[i] = in && any && u * qx < px;
             L.m[i] = m;
             L.s[i] = s;
@@ -262,10 +272,11 @@ template <int W> __global__ __launch_bounds__(VM) void k_verify_mass(const Verif
 {
     constexpr int N = VPL / W;
     __shared__ VerdictLds L;
-    __shared__ double ss[VM / 64];
+    __shared__ double ss[VM / 64], tab[32];
     const int r = blockIdx.y, lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
     const int c = blockIdx.x * (VM / 64 / W) + wid / W, base = c * VC + wid % W * (VC / W);
-    const Verdict w = verdict_of<VM>(p, r, L);
+    exp_table(kExp2[threadIdx.x & 31], tab);
+    const Verdict w = verdict_of<VM>(p, r, L, tab);
     if (!w.refused || !(w.s > 0.0) || (W == 1 && c >= p.nch)) return;
     const float *lrow = p.logits + ((int64_t)r * (p.T + 1) + w.kept) * p.ld, *qrow = p.q + ((int64_t)r * p.T + w.kept) * p.q_ld;
     float v[N], q[N];
@@ -282,7 +293,7 @@ template <int W> __global__ __launch_bounds__(VM) void k_verify_mass(const Verif
     double s = 0.0;
 #pragma unroll
     for (int e = 0; e < N; e++)
-        s += fmax(__builtin_fma(exp_neg(((double)logit(v[e]) - (double)w.m) * p.inv_temp), inv_s, -(double)q[e]), 0.0);
+        s += fmax(__builtin_fma(exp_neg(((double)logit(v[e]) - (double)w.m) * p.rate, tab), inv_s, -(double)q[e]), 0.0);
     s = wave_sum_d(s);
     if (W > 1) {
         if (lane == 0) ss[wid] = s;
@@ -314,14 +325,15 @@ __device__ __forceinline__ double block_scan(double v, double (&part)[VD / 64], 
 __global__ __launch_bounds__(VD) void k_verify_draw(const VerifyParams p)
 {
     __shared__ VerdictLds L;
-    __shared__ double part[4][VD / 64], cut;
+    __shared__ double part[4][VD / 64], cut, tab[32];
     __shared__ int first[2], last[2];
     const int r = blockIdx.x, tid = threadIdx.x;
     constexpr int E = VC / VD;
     if (tid < 2) first[tid] = 0x7fffffff;
     if (tid < 2) last[tid] = -1;
     const double u = (double)p.uniform[(int64_t)r * (p.T + 1) + p.T];
-    const Verdict w = verdict_of<VD>(p, r, L);
+    exp_table(kExp2[threadIdx.x & 31], tab);
+    const Verdict w = verdict_of<VD>(p, r, L, tab);
     int token = -1;
     if (p.greedy) token = w.best;
     else if (w.s > 0.0) {
@@ -343,12 +355,12 @@ __global__ __launch_bounds__(VD) void k_verify_draw(const VerifyParams p)
                 xv[e] = j < p.vocab && j != x ? row[j] : -INFINITY;
             }
         }
-        const double pm = csm * exp_neg(((double)fmaxf(cmx, -kFltMax) - md) * p.inv_temp);
+        const double pm = csm * exp_neg(((double)fmaxf(cmx, -kFltMax) - md) * p.rate, tab);
         double cm = qrow ? left : pm, total;
         if (x >= 0) {
             double s = 0.0, without;
 #pragma unroll
-            for (int e = 0; e < E; e++) s += exp_neg(((double)logit(xv[e]) - md) * p.inv_temp);
+            for (int e = 0; e < E; e++) s += exp_neg(((double)logit(xv[e]) - md) * p.rate, tab);
             block_scan(s, part[3], &without);
             if (tid == x / VC) cm = without;
         }
@@ -380,7 +392,7 @@ __global__ __launch_bounds__(VD) void k_verify_draw(const VerifyParams p)
         double mass[E], sum = 0.0, all;
 #pragma unroll
         for (int e = 0; e < E; e++) {
-            const double v = exp_neg(((double)logit(lv[e]) - md) * p.inv_temp);
+            const double v = exp_neg(((double)logit(lv[e]) - md) * p.rate, tab);
             mass[e] = rest && qrow ? fmax(__builtin_fma(v, inv_s, -(double)qv[e]), 0.0) : rest && j0 + e == x ? 0.0 : v;
             sum += mass[e];
         }
@@ -501,7 +513,7 @@ extern "C" int ifh_verify_drafts_f32(const ifh_verify_desc *d, ifh_stream_t stre
     p.out_tokens = d->out_tokens; p.out_count = d->out_count;
     p.vocab = d->vocab; p.nrows = d->nrows; p.T = d->ndraft; p.nch = (int)verify_chunks(d->vocab);
     p.greedy = d->temperature == 0.0f;
-    p.inv_temp = p.greedy ? 1.0 : 1.0 / (double)d->temperature;
+    p.rate = 46.166241308446828 / (p.greedy ? 1.0 : (double)d->temperature);
     p.vec = (((uintptr_t)d->logits) & 15) == 0 && d->ld % 4 == 0;
     p.qvec = (((uintptr_t)d->draft_probs) & 15) == 0 && d->q_ld % 4 == 0;
     p.csum = (double *)d->ws;
