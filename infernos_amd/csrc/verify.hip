@@ -3,17 +3,15 @@
 //
 // The draw compares a cumulated mass with a given number, and a vocabulary of 150 000 tokens has borders 1e-6 apart: masses are f64, so
 // that neither the way a sum is split nor the exponential's rounding moves a border past the number (f32 exponentials would move one in
-// every few hundred draws from a flat tail).  The f64 work (a short polynomial, ~12 operations a logit and as many in f32) stays under the
-// time the logits take to arrive.
+// every few hundred draws from a flat tail).  The f64 work (~19 operations a logit with the f32 ones) stays under the time the logits take to
+// arrive.
 //   k_verify_stats   a wave or four a chunk of a target row: (max, sum of exp), or the arg-max for temperature 0.  Bound by memory: 320 rows of
-//                    151 936 logits, 194 MB, 46 us = 4.2 TB/s
+//                    151 936 logits, 194 MB, 41 us = 4.7 TB/s
 //   k_verify_mass    a wave or four a chunk of the refused position, where the draft has a distribution: the mass of max(p - q, 0).  64 rows of both,
-//                    78 MB, 15.6 us, 4 of them for the verdicts in front
+//                    78 MB, 15 us, 4 of them for the verdicts in front
 //   k_verify_draw    a workgroup a row: the chunk and then the token where the cumulated mass passes the uniform number.  A chain of
 //                    dependent loads and scans, 7 us for one row and for 64
 // A chunk is 2048 logits: one row of 151 936 is 75 of them, so that one call's few rows still spread over the device.
-// The rows' verdicts (which draft is refused) are worked out from the chunk statistics by every workgroup that asks, its waves taking the
-// row's positions in parallel: a launch of its own for them would cost more.
 #include "common.h"
 
 namespace ifh {
@@ -56,6 +54,12 @@ __device__ __forceinline__ double exp_neg(double y, const double (&tab)[32])
 // NaN counts as -inf; +inf as the largest finite value (its differences stay finite)
 __device__ __forceinline__ float logit(float l) { return l == l ? fminf(l, kFltMax) : -INFINITY; }
 
+// which drafts a row keeps, and the statistics of the position that is drawn from
+struct Verdict {
+    int kept, refused, best;
+    float m;
+    double s;
+};
 struct VerifyParams {
     const float *logits;
     int64_t ld;
@@ -70,6 +74,7 @@ struct VerifyParams {
     double *csum;                // [rows * (T+1)][nch] chunk sums of exp((l - cmax) / temperature); greedy: the place of the chunk's maximum
     double *mass;                // [rows][nch]
     float *cmax;                 // [rows * (T+1)][nch] chunk maxima
+    Verdict *verdicts;           // [rows], written by the mass launch, or NULL: there is none
 };
 
 // a lane's elements of the chunk at `base`: 16 bytes at a time where the row is aligned, else every 64th
@@ -197,13 +202,9 @@ template <int W> __global__ __launch_bounds__(VT) void k_verify_stats(const Veri
     }
 }
 
-// What a row's chunk statistics say: the drafts it keeps, whether the next one is refused, and the statistics of the drawn position.
-// The workgroup's waves take the positions in turn; the same sums in the same order wherever it is asked.
-struct Verdict {
-    int kept, refused, best;
-    float m;
-    double s;
-};
+// A row's verdict from its chunk statistics.
+// The workgroup's waves take the positions in turn; the same sums in the same order wherever it is asked.  (Worked out again by every
+// workgroup of the mass launch, which leaves it for the draw: a launch of its own for it would cost more.)
 struct VerdictLds {
     double s[64];
     float m[64];
@@ -277,6 +278,7 @@ template <int W> __global__ __launch_bounds__(VM) void k_verify_mass(const Verif
     const int c = blockIdx.x * (VM / 64 / W) + wid / W, base = c * VC + wid % W * (VC / W);
     exp_table(kExp2[threadIdx.x & 31], tab);
     const Verdict w = verdict_of<VM>(p, r, L, tab);
+    if (blockIdx.x == 0 && threadIdx.x == 0) p.verdicts[r] = w;          // (for the draw)
     if (!w.refused || !(w.s > 0.0) || (W == 1 && c >= p.nch)) return;
     const float *lrow = p.logits + ((int64_t)r * (p.T + 1) + w.kept) * p.ld, *qrow = p.q + ((int64_t)r * p.T + w.kept) * p.q_ld;
     float v[N], q[N];
@@ -333,7 +335,7 @@ __global__ __launch_bounds__(VD) void k_verify_draw(const VerifyParams p)
     if (tid < 2) last[tid] = -1;
     const double u = (double)p.uniform[(int64_t)r * (p.T + 1) + p.T];
     exp_table(kExp2[threadIdx.x & 31], tab);
-    const Verdict w = verdict_of<VD>(p, r, L, tab);
+    const Verdict w = p.verdicts ? p.verdicts[r] : verdict_of<VD>(p, r, L, tab);
     int token = -1;
     if (p.greedy) token = w.best;
     else if (w.s > 0.0) {
@@ -493,7 +495,7 @@ static int64_t verify_chunks(int vocab) { return ((int64_t)vocab + VC - 1) / VC;
 extern "C" int64_t ifh_verify_drafts_ws_bytes(int nrows, int ndraft)
 {
     if (nrows <= 0 || ndraft < 0) return 0;
-    return (int64_t)nrows * kVerifyMaxChunks * ((ndraft + 1) * 12 + 8);
+    return (int64_t)nrows * (kVerifyMaxChunks * ((ndraft + 1) * 12 + 8) + (int64_t)sizeof(Verdict));
 }
 
 extern "C" int ifh_verify_drafts_f32(const ifh_verify_desc *d, ifh_stream_t stream)
@@ -516,7 +518,9 @@ extern "C" int ifh_verify_drafts_f32(const ifh_verify_desc *d, ifh_stream_t stre
     p.rate = 46.166241308446828 / (p.greedy ? 1.0 : (double)d->temperature);
     p.vec = (((uintptr_t)d->logits) & 15) == 0 && d->ld % 4 == 0;
     p.qvec = (((uintptr_t)d->draft_probs) & 15) == 0 && d->q_ld % 4 == 0;
-    p.csum = (double *)d->ws;
+    const bool mass = !p.greedy && p.q && p.T > 0;
+    p.verdicts = mass ? (Verdict *)d->ws : nullptr;
+    p.csum = (double *)((Verdict *)d->ws + d->nrows);
     p.mass = p.csum + positions * p.nch;
     p.cmax = (float *)(p.mass + (int64_t)d->nrows * p.nch);
     hipStream_t st = as_stream(stream);
@@ -525,7 +529,7 @@ extern "C" int ifh_verify_drafts_f32(const ifh_verify_desc *d, ifh_stream_t stre
     else
         hipLaunchKernelGGL(k_verify_stats<1>, dim3((unsigned)(p.nch + 3) / 4, (unsigned)positions), dim3(VT), 0, st, p);
     IFH_LAUNCH_CHECK("verify stats");
-    if (!p.greedy && p.q && p.T > 0) {
+    if (mass) {
         if ((int64_t)p.nrows * p.nch <= 12 * (int64_t)device_cu_count_physical())
             hipLaunchKernelGGL(k_verify_mass<4>, dim3((unsigned)(p.nch + VM / 256 - 1) / (VM / 256), (unsigned)p.nrows), dim3(VM), 0, st, p);
         else
