@@ -494,7 +494,7 @@ static int64_t verify_chunks(int vocab) { return ((int64_t)vocab + VC - 1) / VC;
 
 extern "C" int64_t ifh_verify_drafts_ws_bytes(int nrows, int ndraft)
 {
-    if (nrows <= 0 || ndraft < 0) return 0;
+    if (nrows <= 0 || ndraft < 0 || ndraft > 63) return 0;
     return (int64_t)nrows * (kVerifyMaxChunks * ((ndraft + 1) * 12 + 8) + (int64_t)sizeof(Verdict));
 }
 
