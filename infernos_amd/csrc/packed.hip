@@ -757,11 +757,14 @@ extern "C" int ifh_rope_append_packed_bf16(const ifh_rope_packed_desc *d, ifh_st
 // A prefix is read by narrow ones as long as seven workgroups for eight CUs do and their rows are four fifths full: its keys then come to
 // four waves at once (64 rows of 12 / 2 heads behind 2048 keys 14.5 us, wide 15.3; behind 8000 21.9 and 20.1; 96 rows behind 2048 17.6 and
 // 16.5; 8 rows of 40 / 8 heads, 40 rows in two blocks, behind 4000 15.7 and 13.9).
-// Keys are split into parts until the device has two workgroups a CU, and no further than that pays for the join's launch (2.5 us) and for
-// what each part costs it: none of fewer than eight tiles (narrow: two a wave) or four (wide), wide blocks of up to 512 keys not at all
-// unless the results are joined anyway (64 sequences, 300 keys: 7.4 us, split 9.4 us; one prompt of 300 rows 9.4, split 11.9 us; of 700 keys 15.7, split 12.8 us), and at most
-// 1.6 sqrt(tiles) parts, the time of a part being tiles / parts and that of the join parts (4 sequences of 4000 keys: 31 parts 15.7 us, 16
-// parts 14.0 us, 10 parts 15.5 us; one of 8000: 63 parts 17.2 us, 25 parts 15.6 us, 15 parts 17.7 us).
+// Keys are split into parts until the device has two workgroups a CU, and no further than that pays for the join's launch and for what
+// each part costs it: none of fewer than eight tiles (narrow: two a wave) or four (wide), and at most 1.6 sqrt(tiles) parts, the time of a
+// part being tiles / parts and that of the join parts (4 sequences of 4000 keys: 31 parts 15.7 us, 16 parts 14.0 us, 10 parts 15.5 us; one
+// of 8000: 63 parts 17.2 us, 25 parts 15.6 us, 15 parts 17.7 us).  Not at all, unless the results are joined anyway, up to 512 keys (wide)
+// or 1024 (narrow), and past them while the workgroups that there are (0 to 256) make up for it, wide up to 7 and narrow up to 20 keys a
+// workgroup (whole and split: 64 sequences of 16 tokens, 300 keys, 7.4 and 9.4 us; one prompt of 300 rows 9.4 and 11.9 us, of 700 keys 15.7
+// and 12.8; 16 of 64 tokens behind 700 keys, 12 / 2 heads, 17.6 and 19.7 us, behind 1200 24.9 and 22.7; one token of 64 sequences behind 900
+// keys 13.3 and 18.4 us, behind 2000 28.4 and 30.9; of 16 sequences behind 2000 20.4 and 14.8).
 static void split_keys(KeySet *k, bool narrow, int64_t blocks, int nkv, int max_keys)
 {
     k->narrow = narrow;
@@ -770,7 +773,7 @@ static void split_keys(KeySet *k, bool narrow, int64_t blocks, int nkv, int max_
     const int tiles = (max_keys + kKeys - 1) / kKeys, least = narrow ? 8 : 4;
     const int64_t want = 2 * (int64_t)device_cu_count_physical() / (blocks * nkv > 0 ? blocks * nkv : 1);
     int parts = (int)(want < 1 ? 1 : want > 64 ? 64 : want);
-    if (k->mode == ROWS_PACKED && !narrow && tiles <= 16) parts = 1;
+    if (k->mode == ROWS_PACKED && (tiles <= (narrow ? 32 : 16) || tiles * 32 <= blocks * nkv * (narrow ? 20 : 7))) parts = 1;
     while (2 * (int64_t)parts * parts > 5 * (int64_t)tiles && parts > 1) parts--;
     if (parts > tiles / least) parts = tiles / least > 1 ? tiles / least : 1;
     k->part_tiles = (tiles + parts - 1) / parts;

@@ -301,7 +301,7 @@ def attn_packed(q, cache, out, cu, key_len, *, ntokens, nseqs, nheads, nkv, head
     kv = nkv * head_dim
     d = _lib.AttnPackedDesc(q.data_ptr(), nheads * head_dim + 2 * kv if q_ts is None else q_ts, cache.data_ptr(), max_pos * 2 * kv, 2 * kv, kv,
                             out.data_ptr(), nheads * head_dim, cu.data_ptr(), key_len.data_ptr(), ntokens, nseqs, nheads, nkv, head_dim,
-                            max_keys, head_dim ** -0.5, _ptr(ws), 0 if ws is None else ws.numel())       # (an empty tensor's address is NULL)
+                            max_keys, head_dim ** -0.5, _ptr(ws), 0 if ws is None else ws.nbytes // 4)       # (an empty tensor's address is NULL)
     _launch('ifh_attn_packed_bf16', out, ctypes.byref(d))
     return out
 
@@ -319,7 +319,7 @@ def attn_prefix(q, prefix, cache, out, key_len, *, nrows, tokens_per_row, prefix
     kv = nkv * head_dim
     d = _lib.AttnPrefixDesc(q.data_ptr(), nheads * head_dim + 2 * kv if q_ts is None else q_ts, prefix.data_ptr(), 2 * kv, cache.data_ptr(),
                             max_pos * 2 * kv, 2 * kv, kv, out.data_ptr(), nheads * head_dim, _ptr(prefix_len), key_len.data_ptr(), nrows,
-                            tokens_per_row, prefix_keys, nheads, nkv, head_dim, max_keys, head_dim ** -0.5, ws.data_ptr(), ws.numel())
+                            tokens_per_row, prefix_keys, nheads, nkv, head_dim, max_keys, head_dim ** -0.5, ws.data_ptr(), ws.nbytes // 4)
     _launch('ifh_attn_prefix_bf16', out, ctypes.byref(d))
     return out
 

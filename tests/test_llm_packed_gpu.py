@@ -165,7 +165,9 @@ def test_attn_packed_rows_that_see_nothing_and_tokens_behind_the_last(dev):
                                                 ((4, 1, 64), [40, 0, 33, 1, 64, 9], [5000, 300, 4000, 2000, 64, 0]),
                                                 ((12, 2, 128), [2, 1, 0, 1, 1], [3001, 10, 700, 0, 1500]),
                                                 ((4, 1, 64), [1, 0, 2] * 30, [700 - 7 * s for s in range(90)]),
-                                                ((4, 1, 64), [1] * 200, [(37 * s) % 1200 for s in range(200)])])
+                                                ((4, 1, 64), [1] * 200, [(37 * s) % 1200 for s in range(200)]),
+                                                ((4, 1, 64), [1, 0, 2] * 30, [2600 - 29 * s for s in range(90)]),
+                                                ((4, 1, 64), [1] * 200, [(137 * s) % 5000 for s in range(200)])])
 def test_attn_packed_splits_ragged_sequences(dev, heads, lens, key_len):
     """few rows, long keys: sequences of every length share the workgroups, empty ones among them; tokens behind the last sequence keep
     what was there; without a workspace the same within the roundings"""
@@ -174,7 +176,7 @@ def test_attn_packed_splits_ragged_sequences(dev, heads, lens, key_len):
     N = sum(lens)
     rows = list(packed_rows(c, sample=6))
     out, ws = run_packed(c, dev)
-    assert ws.numel() > 0
+    assert ws.numel() > 0 or max(key_len) <= 1200                     # (many short sequences fill the device whole)
     check_rows(out.view(-1, nh, hd), rows, 'split')
     assert bool((out[N:] == 7.0).all())
     out, _ = run_packed(c, dev, False)
