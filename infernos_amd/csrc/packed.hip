@@ -309,7 +309,7 @@ struct WaveRows {
 //           from the end of the first product on, no barrier), and the four results are joined in LDS.  For the few rows of a decode step,
 //           whose work is bringing the keys: 128 rows would leave three waves idle.
 // and three instances of the kernel:
-//   ROWS_LONG    every workgroup is wide and its rows packed.  Three workgroups a CU (165 registers, 32 KB).  Bound by the matrix unit and
+//   ROWS_LONG    every workgroup is wide and its rows packed.  Three workgroups a CU (162 registers, 32 KB).  Bound by the matrix unit and
 //                the vector unit in turn, at the clock that the power budget leaves (a tile of a wave: 512 clocks of products, ~400 of
 //                softmax): one prompt of 8191 tokens, 40 / 8 heads of 128, 625-655 us = 1.05-1.10 PFLOP/s.
 //   ROWS_MIXED   either form, decided at run time.  Two workgroups a CU (narrow: 68 KB, for four waves' buffers and results).  Bound by the
