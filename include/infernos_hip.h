@@ -676,8 +676,9 @@ int ifh_rope_append_packed_bf16(const ifh_rope_packed_desc *desc, ifh_stream_t s
 /* Causal grouped-query attention of sequences laid end to end: sequence s has the tokens cu[s] .. cu[s+1]-1 and the first key_len[s]
  * keys of cache row s; its last token sees all of them, the one before one fewer, and so on (new tokens behind what the row already
  * holds, themselves appended before).  A token that sees no key gets zeros; tokens behind cu[nseqs] keep what out holds.  Any number of
- * query heads per kv head; head_dim 64 or 128.  softmax(scale q.k) v, f32 sums; the probabilities are rounded to bf16 for the second
- * product.  K and V from slot key_len on are not used, whatever they hold.  A K row that is not finite reaches only the tokens that see
+ * query heads per kv head; head_dim 64 or 128.  softmax(scale q.k) v, f32 sums; the probabilities go into the second
+ * product as two bf16, within 2^-16 of themselves; probs_bf16 != 0: as one, within 2^-8, like ifh_attn_gqa_bf16's for prompts (faster
+ * where the products bound: long prompts).  K and V from slot key_len on are not used, whatever they hold.  A K row that is not finite reaches only the tokens that see
  * it; V rows below key_len have to be finite, for a token multiplies those of its tiles that it does not see by zero.
  * ws: f32 workspace, with which few long rows are split along their keys: ifh_attn_packed_ws_floats() elements for the split that fills
  * the device (0: none is needed), a smaller one splits less, NULL not at all.  A workspace belongs to one stream / graph at a time. */
@@ -694,6 +695,7 @@ typedef struct ifh_attn_packed_desc {
     float scale;
     float *ws;
     int64_t ws_floats;
+    int32_t probs_bf16;
 } ifh_attn_packed_desc;
 int64_t ifh_attn_packed_ws_floats(int ntokens, int nseqs, int nheads, int nkv, int head_dim, int max_keys);
 int ifh_attn_packed_bf16(const ifh_attn_packed_desc *desc, ifh_stream_t stream);
@@ -702,7 +704,7 @@ int ifh_attn_packed_bf16(const ifh_attn_packed_desc *desc, ifh_stream_t stream);
  * key_len[i] keys of cache row b.  The prefix is read once for all rows, not once a row.  A token that sees no key gets zeros.
  * tokens_per_row > 1: drafted tokens, each with its own key_len.  V rows of the prefix, and a row's own below its largest key_len, have
  * to be finite (see above).  ws: ifh_attn_prefix_ws_floats() f32 for the split that fills the device; a smaller one splits less, down to
- * two partial results a query row.  Of one stream / graph at a time. */
+ * two partial results a query row.  Of one stream / graph at a time.  probs_bf16: as above. */
 typedef struct ifh_attn_prefix_desc {
     const void *q;
     int64_t q_ts;
@@ -718,6 +720,7 @@ typedef struct ifh_attn_prefix_desc {
     float scale;
     float *ws;
     int64_t ws_floats;
+    int32_t probs_bf16;
 } ifh_attn_prefix_desc;
 int64_t ifh_attn_prefix_ws_floats(int nrows, int tokens_per_row, int prefix_keys, int nheads, int nkv, int head_dim, int max_keys);
 int ifh_attn_prefix_bf16(const ifh_attn_prefix_desc *desc, ifh_stream_t stream);

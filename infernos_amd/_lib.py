@@ -145,7 +145,7 @@ class AttnPackedDesc(ctypes.Structure):
     _fields_ = [('q', _vp), ('q_ts', _i64), ('cache', _vp), ('cache_bs', _i64), ('cache_ts', _i64), ('v_off', ctypes.c_int32),
                 ('out', _vp), ('o_ts', _i64), ('cu', _vp), ('key_len', _vp), ('ntokens', ctypes.c_int32), ('nseqs', ctypes.c_int32),
                 ('nheads', ctypes.c_int32), ('nkv', ctypes.c_int32), ('head_dim', ctypes.c_int32), ('max_keys', ctypes.c_int32),
-                ('scale', _f), ('ws', _vp), ('ws_floats', _i64)]
+                ('scale', _f), ('ws', _vp), ('ws_floats', _i64), ('probs_bf16', ctypes.c_int32)]
 
 
 class AttnPrefixDesc(ctypes.Structure):
@@ -154,7 +154,7 @@ class AttnPrefixDesc(ctypes.Structure):
                 ('cache_ts', _i64), ('v_off', ctypes.c_int32), ('out', _vp), ('o_ts', _i64), ('prefix_len', _vp), ('key_len', _vp),
                 ('nrows', ctypes.c_int32), ('tokens_per_row', ctypes.c_int32), ('prefix_keys', ctypes.c_int32),
                 ('nheads', ctypes.c_int32), ('nkv', ctypes.c_int32), ('head_dim', ctypes.c_int32), ('max_keys', ctypes.c_int32),
-                ('scale', _f), ('ws', _vp), ('ws_floats', _i64)]
+                ('scale', _f), ('ws', _vp), ('ws_floats', _i64), ('probs_bf16', ctypes.c_int32)]
 
 
 class VerifyDesc(ctypes.Structure):

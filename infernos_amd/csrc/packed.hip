@@ -164,8 +164,12 @@ template <int HD> __device__ __forceinline__ int vperm(int r) { return HD == 128
 // A wave's 32 rows: S^T = K Q^T and O^T = V^T P^T with the 32 x 32 x 16 MFMA.  A lane holds one row's scores of 16 of every 32 keys, so the
 // softmax of a row is lane-local up to one exchange with lane ^ 32, and P goes from the accumulators of the first product into the operand
 // of the second without leaving the lane (its 8 keys are 8 half + {0..3, 8..11} + 4 (lane / 32): V^T is read in that order, transposed by
-// ds_read_b64_tr_b16).  P is rounded to bf16 for the second product, as a bf16 model does; sums and maxima are f32.
-template <int HD, bool FEW>
+// ds_read_b64_tr_b16).  Sums and maxima are f32.  The second product takes P as the sum of two bf16 (P16 false: P rounded, and what the
+// rounding left, rounded: together within 2^-16 of P), so that the result has the bits of f32 probabilities; a caller may have the first
+// alone (P16: within 2^-8, as the prompt kernel of llm.hip), which saves one of three products and the splitting.  Us a call, sum and
+// rounded: one prompt of 8191 tokens, 40 / 8 heads of 128, 850 and 625; 64 prompts of 12 / 2 heads 32.7 and 29.6; 64 rows of 5 tokens behind
+// 8001 shared keys 118 and 101, 64 single tokens behind 2048 14.9 and 14.4.
+template <int HD, bool FEW, bool P16>
 struct WaveRows {
     static constexpr int NS = HD / 16, ND = HD / 32, ROWB = HD * 2;
     bf16x8_t qf[NS];
@@ -279,6 +283,11 @@ struct WaveRows {
             v[d] = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
         }
     }
+    // the second half of two probabilities whose roundings are `hi`
+    static __device__ __forceinline__ uint32_t rest(float a, float b, uint32_t hi)
+    {
+        return f32x2_to_bf16x2(a - __uint_as_float(hi << 16), b - __uint_as_float(hi & 0xffff0000u));
+    }
     __device__ __forceinline__ void accumulate(const unsigned char *lds, unsigned at, const f32x16 &s, bf16x8_t (&v)[ND])
     {
 #pragma unroll
@@ -294,6 +303,13 @@ struct WaveRows {
             const bf16x8_t pf = __builtin_bit_cast(bf16x8_t, pb);
 #pragma unroll
             for (int d = 0; d < ND; d++) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[d], pf, o[d], 0, 0, 0);
+            if constexpr (!P16) {
+                const uint4 lo = make_uint4(rest(s[e0], s[e0 + 1], pb.x), rest(s[e0 + 2], s[e0 + 3], pb.y), rest(s[e0 + 4], s[e0 + 5], pb.z),
+                                            rest(s[e0 + 6], s[e0 + 7], pb.w));
+                const bf16x8_t pl = __builtin_bit_cast(bf16x8_t, lo);
+#pragma unroll
+                for (int d = 0; d < ND; d++) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[d], pl, o[d], 0, 0, 0);
+            }
             if (kk == 0) {
 #pragma unroll
                 for (int d = 0; d < ND; d++) v[d] = next[d];
@@ -320,7 +336,7 @@ struct WaveRows {
 //                key set's traffic a tile takes longer to come than to multiply, so wide ones bring two ahead.  64 rows of 5 tokens behind
 //                8001 keys, 40 / 8 heads: 102 us (ROWS_MIXED 107); 48 rows of 4 behind 16000 110 us (124); 64 rows of 3 behind 4000, 14 / 2
 //                heads of 64, 18.4 us (19.7).  In the other two neither pays (ROWS_LONG with both: 1 % slower, ROWS_MIXED 2 %).
-template <int HD, int FORM>
+template <int HD, int FORM, bool P16>
 __global__ __launch_bounds__(256, FORM == ROWS_MIXED ? 2 : 3) void k_attn_rows(const RowsParams p)
 {
     constexpr bool LONG = FORM == ROWS_LONG;
@@ -398,7 +414,7 @@ __global__ __launch_bounds__(256, FORM == ROWS_MIXED ? 2 : 3) void k_attn_rows(c
     const int n = n1 - n0, w0 = row0 + (narrow ? 0 : wid * 32), row = w0 + l32, t = row / G, g = row - t * G;
     const bool ok = t < n;
     const int tok = n0 + (ok ? t : 0), head = kvh * G + (ok ? g : 0);
-    WaveRows<HD, FORM == ROWS_BOTH> w;
+    WaveRows<HD, FORM == ROWS_BOTH, P16> w;
     w.load_q(p.q + (int64_t)tok * p.q_ts + (int64_t)head * HD, h2);       // in flight while the limits are looked up
     int lim, wmax, wmin, kmax;                                 // keys this lane's row sees; most and fewest of the wave's rows; most of the block's
     if (mode == ROWS_PACKED) {
@@ -801,10 +817,14 @@ static void fewer_parts(KeySet *k)
     k->parts = (tiles + k->part_tiles - 1) / k->part_tiles;
 }
 
-static void rows_launch(const RowsParams &p, int hd, int form, int64_t workgroups, hipStream_t st)
+static void rows_launch(const RowsParams &p, int hd, int form, bool p16, int64_t workgroups, hipStream_t st)
 {
     const dim3 grid((unsigned)workgroups), block(256);
-#define ROWS_GO(HD, FORM) hipLaunchKernelGGL((k_attn_rows<HD, FORM>), grid, block, 0, st, p)
+#define ROWS_GO(HD, FORM)                                                                         \
+    do {                                                                                          \
+        if (p16) hipLaunchKernelGGL((k_attn_rows<HD, FORM, true>), grid, block, 0, st, p);        \
+        else hipLaunchKernelGGL((k_attn_rows<HD, FORM, false>), grid, block, 0, st, p);           \
+    } while (0)
     if (form == ROWS_LONG) {
         if (hd == 128) ROWS_GO(128, ROWS_LONG); else ROWS_GO(64, ROWS_LONG);
     } else if (form == ROWS_BOTH) {
@@ -885,7 +905,7 @@ extern "C" int ifh_attn_packed_bf16(const ifh_attn_packed_desc *d, ifh_stream_t 
     const int64_t wgs = (int64_t)k.blocks * p.nkv * k.parts;
     p.first = (int)wgs;
     hipStream_t st = as_stream(stream);
-    rows_launch(p, d->head_dim, k.narrow ? ROWS_MIXED : ROWS_LONG, wgs, st);
+    rows_launch(p, d->head_dim, k.narrow ? ROWS_MIXED : ROWS_LONG, d->probs_bf16, wgs, st);
     IFH_LAUNCH_CHECK("attn_packed");
     if (p.part_o) {
         join_launch(p, d->head_dim, k.parts, st);
@@ -952,7 +972,7 @@ extern "C" int ifh_attn_prefix_bf16(const ifh_attn_prefix_desc *d, ifh_stream_t 
     hipStream_t st = as_stream(stream);
     if (prefix_joint((int64_t)b.blocks * p.nkv, d->prefix_keys, d->max_keys, b.narrow)) {
         p.joint = 1;
-        rows_launch(p, d->head_dim, ROWS_MIXED, (int64_t)b.blocks * p.nkv, st);
+        rows_launch(p, d->head_dim, ROWS_MIXED, d->probs_bf16, (int64_t)b.blocks * p.nkv, st);
         IFH_LAUNCH_CHECK("attn_prefix joint");
         return IFH_OK;
     }
@@ -970,7 +990,7 @@ extern "C" int ifh_attn_prefix_bf16(const ifh_attn_prefix_desc *d, ifh_stream_t 
         b = t;
         p.first = (int)nb;
     }
-    rows_launch(p, d->head_dim, p.pairs > 0 ? ROWS_BOTH : ROWS_MIXED, na + nb, st);
+    rows_launch(p, d->head_dim, p.pairs > 0 ? ROWS_BOTH : ROWS_MIXED, d->probs_bf16, na + nb, st);
     IFH_LAUNCH_CHECK("attn_prefix");
     join_launch(p, d->head_dim, parts, st);
     IFH_LAUNCH_CHECK("attn_prefix join");

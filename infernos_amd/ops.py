@@ -294,14 +294,17 @@ def attn_packed_ws(device, *, ntokens, nseqs, nheads, nkv, head_dim, max_keys):
         return _ws(_lib.lib().ifh_attn_packed_ws_floats(ntokens, nseqs, nheads, nkv, head_dim, max_keys), device)
 
 
-def attn_packed(q, cache, out, cu, key_len, *, ntokens, nseqs, nheads, nkv, head_dim, max_pos, max_keys, ws=None, q_ts=None):
+def attn_packed(q, cache, out, cu, key_len, *, ntokens, nseqs, nheads, nkv, head_dim, max_pos, max_keys, ws=None, q_ts=None,
+                probs_bf16=False):
     """causal grouped-query attention of sequences laid end to end (ifh_attn_packed_bf16): tokens cu[s] .. cu[s + 1] - 1 of sequence s
     against the first key_len[s] keys of cache row s, the last token seeing all of them.  q: the first nheads * head_dim columns of rows
-    q_ts apart (None: the fused projection's)"""
+    q_ts apart (None: the fused projection's).  probs_bf16: probabilities rounded to bf16 for the second product, as attn_gqa does on a prompt
+    (a third off a long prompt's time), instead of split in two bf16 that keep 16 bits"""
     kv = nkv * head_dim
     d = _lib.AttnPackedDesc(q.data_ptr(), nheads * head_dim + 2 * kv if q_ts is None else q_ts, cache.data_ptr(), max_pos * 2 * kv, 2 * kv, kv,
                             out.data_ptr(), nheads * head_dim, cu.data_ptr(), key_len.data_ptr(), ntokens, nseqs, nheads, nkv, head_dim,
-                            max_keys, head_dim ** -0.5, _ptr(ws), 0 if ws is None else ws.nbytes // 4)       # (an empty tensor's address is NULL)
+                            max_keys, head_dim ** -0.5, _ptr(ws), 0 if ws is None else ws.nbytes // 4,       # (an empty tensor's address is NULL)
+                            probs_bf16)
     _launch('ifh_attn_packed_bf16', out, ctypes.byref(d))
     return out
 
@@ -313,13 +316,13 @@ def attn_prefix_ws(device, *, nrows, tokens_per_row, prefix_keys, nheads, nkv, h
 
 
 def attn_prefix(q, prefix, cache, out, key_len, *, nrows, tokens_per_row, prefix_keys, nheads, nkv, head_dim, max_pos, max_keys, ws,
-                prefix_len=None, q_ts=None):
+                prefix_len=None, q_ts=None, probs_bf16=False):
     """grouped-query attention of a decode step whose rows share a prefix (ifh_attn_prefix_bf16): token i of row b sees the first
-    prefix_len[b] keys of `prefix` [prefix_keys, 2 * nkv * head_dim] (None: all) and the first key_len[i] keys of cache row b"""
+    prefix_len[b] keys of `prefix` [prefix_keys, 2 * nkv * head_dim] (None: all) and the first key_len[i] keys of cache row b.  probs_bf16: as in attn_packed"""
     kv = nkv * head_dim
     d = _lib.AttnPrefixDesc(q.data_ptr(), nheads * head_dim + 2 * kv if q_ts is None else q_ts, prefix.data_ptr(), 2 * kv, cache.data_ptr(),
                             max_pos * 2 * kv, 2 * kv, kv, out.data_ptr(), nheads * head_dim, _ptr(prefix_len), key_len.data_ptr(), nrows,
-                            tokens_per_row, prefix_keys, nheads, nkv, head_dim, max_keys, head_dim ** -0.5, ws.data_ptr(), ws.nbytes // 4)
+                            tokens_per_row, prefix_keys, nheads, nkv, head_dim, max_keys, head_dim ** -0.5, ws.data_ptr(), ws.nbytes // 4, probs_bf16)
     _launch('ifh_attn_prefix_bf16', out, ctypes.byref(d))
     return out
 

@@ -1,0 +1,115 @@
+"""GPU tests of packed.hip and verify.hip where the first ones do not reach: the bits that the probabilities keep, scores that leave the
+first tile empty, every kernel form, and draft verification at the sizes of a server's batch.  References in 64 bits."""
+import pytest
+import torch
+
+from test_llm_packed_gpu import BF, F64, dev, i32, packed_case, prefix_case        # noqa: F401  (dev is a fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+def attend_f32(q, k, v, scale):
+    """one query head -> (result in 64 bits, tolerance of a kernel whose probabilities keep 16 bits).  With A = sum_j p_j |v_j|: the
+    result's rounding to bf16, 2^-8 |o|; a probability as the sum of two bf16, each off by at most 2^-8 of what it rounds: 2^-16 A; a
+    score is an f32 sum of head_dim products, off by at most (head_dim + 4) 2^-24 sum_d |q k| scale = delta (the scaling and the
+    exponent's argument are two roundings each), which moves a normalised probability by 2 delta; the exponential 2^-21 and the
+    polynomial of its argument's range 2^-21 more; sums over n keys n 2^-24 A in numerator and denominator"""
+    if k.size(0) == 0:
+        z = torch.zeros_like(q, dtype=F64)
+        return z, z
+    q, k, v = q.double(), k.double(), v.double()
+    p = torch.softmax((k @ q) * scale, 0)
+    o, A = p @ v, p @ v.abs()
+    delta = (q.numel() + 4) * 2.0 ** -24 * float((k.abs() @ q.abs()).max()) * scale
+    return o, 2.0 ** -8 * o.abs() + 1.01 * (2.0 ** -16 + 2 * delta + 2.0 ** -20 + 2 * k.size(0) * 2.0 ** -24) * A + 1e-30
+
+
+def compare(out, rows, what, f=attend_f32):
+    """rows: (index into out [N, nh, hd], q, k, v)"""
+    worst = 0.0
+    for at, q, k, v in rows:
+        o, tol = f(q, k, v, q.numel() ** -0.5)
+        share = float(((out[at].double() - o).abs() / tol.clamp(min=1e-30)).max())
+        assert share <= 1.0, (what, at, share)
+        worst = max(worst, share)
+    return worst
+
+
+def packed_kv(c, every=1):
+    nh, nkv, hd = c['heads']
+    G, i = nh // nkv, 0
+    for s, n in enumerate(c['lens']):
+        for t in range(n):
+            if t % every and t != n - 1:
+                continue
+            m = max(0, c['klen'][s] - (n - 1 - t))
+            kv = c['cache'][s, :m].view(m, 2, nkv, hd)
+            for h in sorted({0, (5 * t) % nh, nh - 1}):
+                yield (i + t, h), c['qkv'][i + t, h * hd:(h + 1) * hd], kv[:, 0, h // G], kv[:, 1, h // G]
+        i += n
+
+
+def prefix_kv(c, every=1):
+    nh, nkv, hd = c['heads']
+    G = nh // nkv
+    for i in range(0, c['B'] * c['T'], every):
+        b, m = i // c['T'], c['klen'][i]
+        x = c['P'] if c['plen'] is None else c['plen'][b]
+        kv = torch.cat([c['prefix'][:x], c['cache'][b, :m]]).view(x + m, 2, nkv, hd)
+        for h in sorted({0, (5 * i) % nh, nh - 1}):
+            yield (i, h), c['qkv'][i, h * hd:(h + 1) * hd], kv[:, 0, h // G], kv[:, 1, h // G]
+
+
+def run_packed(c, dev, split=True, **kw):
+    from infernos_amd import ops
+    nh, nkv, hd = c['heads']
+    sizes = dict(ntokens=c['N'], nseqs=c['n'], nheads=nh, nkv=nkv, head_dim=hd, max_keys=c['max_keys'])
+    out = torch.empty(c['N'], nh * hd, dtype=BF, device=dev)
+    ops.attn_packed(c['qkv'], c['cache'], out, c['cu'], c['key_len'], max_pos=c['S'], ws=ops.attn_packed_ws(dev, **sizes) if split else None, **sizes, **kw)
+    return out.view(c['N'], nh, hd)
+
+
+def run_prefix(c, dev, **kw):
+    from infernos_amd import ops
+    nh, nkv, hd = c['heads']
+    sizes = dict(nrows=c['B'], tokens_per_row=c['T'], prefix_keys=c['P'], nheads=nh, nkv=nkv, head_dim=hd, max_keys=c['max_keys'])
+    out = torch.empty(c['B'] * c['T'], nh * hd, dtype=BF, device=dev)
+    ops.attn_prefix(c['qkv'], c['prefix'], c['cache'], out, c['key_len'], max_pos=c['S'], prefix_len=c['prefix_len'],
+                    ws=ops.attn_prefix_ws(dev, **sizes), **sizes, **kw)
+    return out.view(c['B'] * c['T'], nh, hd)
+
+
+# ---- the probabilities' bits -----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('heads,lens,past', [((4, 1, 64), [37, 1, 20], 0), ((12, 2, 128), [130, 41], 0), ((12, 2, 128), [33, 60], 1500),
+                                             ((14, 2, 64), [1, 1, 2], 3000), ((12, 2, 128), [1] * 9, 200)])
+def test_packed_probabilities_keep_16_bits(dev, heads, lens, past):
+    """wide and narrow workgroups, keys whole and split; a caller may have the probabilities rounded to bf16 instead (2^-8 A more, with A
+    of the tolerance above), which gives other bits"""
+    c = packed_case(dev, heads, lens, [n + (past + 7 * s if past else 0) for s, n in enumerate(lens)], spare=3, seed=past + len(lens))
+    rows = list(packed_kv(c, 9))
+    for split in (True, False):
+        out = run_packed(c, dev, split)
+        print('packed', heads, lens, past, split, 'worst share of the tolerance %.2f' % compare(out, rows, 'packed'))
+        rounded = run_packed(c, dev, split, probs_bf16=True)
+        assert not torch.equal(out, rounded)
+        compare(rounded, rows, 'rounded', rounded_tol)
+
+
+@pytest.mark.parametrize('heads,B,T,P,own', [((4, 1, 64), 2, 1, 333, 40), ((12, 2, 128), 64, 1, 2048, 300), ((40, 8, 128), 64, 5, 1400, 400),
+                                             ((14, 2, 64), 9, 3, 900, 300)])
+def test_prefix_probabilities_keep_16_bits(dev, heads, B, T, P, own):
+    """one launch and two, both key sets' forms"""
+    c = prefix_case(dev, heads, B, T, P, [(b * 7919) % own for b in range(B)], seed=P)
+    rows = list(prefix_kv(c, max(1, B * T // 40)))
+    out = run_prefix(c, dev)
+    print('prefix', heads, B, T, P, own, 'worst share of the tolerance %.2f' % compare(out, rows, 'prefix'))
+    rounded = run_prefix(c, dev, probs_bf16=True)
+    assert not torch.equal(out, rounded)
+    compare(rounded, rows, 'rounded', rounded_tol)
+
+
+def rounded_tol(q, k, v, scale):
+    o, tol = attend_f32(q, k, v, scale)
+    if k.size(0) == 0:
+        return o, tol
+    return o, tol + 2.0 ** -8 * (torch.softmax((k.double() @ q.double()) * scale, 0) @ v.double().abs())
