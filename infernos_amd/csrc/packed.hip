@@ -117,6 +117,7 @@ struct RowsParams {
 };
 
 enum { ROWS_MIXED, ROWS_LONG, ROWS_BOTH };
+constexpr float kNoKeys = -3.402823466e38f;     // the maximum of a row that saw nothing: no score lies below
 constexpr int kWideRows = 128, kNarrowRows = 32, kKeys = 32;
 
 // max over lanes l and l ^ 32, every lane gets it
@@ -222,12 +223,12 @@ struct WaveRows {
             if (i + AHEAD < NS) kf[i % AHEAD] = frag(i + AHEAD);
         }
     }
-    // scores -> unnormalised probabilities 2^(s c1 - ms); rel: keys of the tile this lane's row sees, minus 4 (lane / 32); first: the wave's
-    // first tile of a range of keys.  ms starts as the maximum of the first tile that a row sees anything of (what it sees of a range is
-    // its keys up to lim, so the range's first tile or none) and is raised only when a later tile exceeds it by more than 8 (a wave
-    // decides at once): p stays below 2^8, sums in f32 lose nothing by it, and the rescaling of the accumulators is skipped for almost
-    // every tile.
-    __device__ __forceinline__ void softmax(f32x16 &s, bool mask, int rel, bool first)
+    // scores -> unnormalised probabilities 2^(s c1 - ms); rel: keys of the tile this lane's row sees, minus 4 (lane / 32); first: set at the
+    // wave's first tile of a range of keys.  ms starts as the maximum of the first tile that a row sees anything of (what it sees of a range
+    // is its keys up to lim, so the range's first tile or none; first stays set while a row has seen keys, but no score above -inf) and is
+    // raised only when a later tile exceeds it by more than 8 (a wave decides at once): p stays below 2^8, sums in f32 lose nothing by it,
+    // and the rescaling of the accumulators is skipped for almost every tile.
+    __device__ __forceinline__ void softmax(f32x16 &s, bool mask, int rel, bool &first)
     {
 #pragma unroll
         for (int e = 0; e < 16; e++) s[e] = __builtin_fmaf(s[e], c1, -ms);
@@ -245,7 +246,8 @@ struct WaveRows {
         mx = max_half(fmaxf(mx, my));
         if (first || __any(mx > 8.0f)) {
             const bool unset = first && l + __shfl_xor(l, 32, 64) == 0.0f;
-            const float raise = unset ? (mx > -1e30f ? mx : 0.0f) : fmaxf(mx, 0.0f);
+            const bool none = unset && !(mx > -INFINITY);
+            const float raise = none ? 0.0f : unset ? mx : fmaxf(mx, 0.0f);
             const float alpha = unset ? 1.0f : __builtin_amdgcn_exp2f(-raise);
             ms += raise;
             l *= alpha;
@@ -255,6 +257,7 @@ struct WaveRows {
                 for (int e = 0; e < 16; e++) o[d][e] *= alpha;
 #pragma unroll
             for (int e = 0; e < 16; e++) s[e] -= raise;
+            first = __any(none && rel > 0);
         }
         float ls[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -268,7 +271,7 @@ struct WaveRows {
     __device__ __forceinline__ void finish()
     {
         l += __shfl_xor(l, 32, 64);
-        ms = l > 0.0f ? ms : -1e30f;
+        ms = l > 0.0f ? ms : kNoKeys;
     }
     // O^T += V^T P^T, V tile vt; v: the fragments of its first 16 keys, read before the softmax
     __device__ __forceinline__ void values(const unsigned char *lds, unsigned at, int kk, bf16x8_t (&v)[ND])
@@ -489,6 +492,7 @@ __global__ __launch_bounds__(256, FORM == ROWS_MIXED ? 2 : 3) void k_attn_rows(c
             at = at == (RING - 1) * 2 * TILE ? 0 : at + 2 * TILE;
             far = far == (RING - 1) * 2 * TILE ? 0 : far + 2 * TILE;
         };
+        bool first = true;
         auto tile = [&](int kt, auto more) {
             const int kbase = kt * kKeys;
             f32x16 s;
@@ -498,7 +502,7 @@ __global__ __launch_bounds__(256, FORM == ROWS_MIXED ? 2 : 3) void k_attn_rows(c
             });
             bf16x8_t v[ND];
             w.values(lds, at + TILE, 0, v);
-            w.softmax(s, kbase + kKeys > wmin, lim - kbase - 4 * h2, kt == kt0);
+            w.softmax(s, kbase + kKeys > wmin, lim - kbase - 4 * h2, first);
             w.accumulate(lds, at + TILE, s, v);
             on();
         };
@@ -582,6 +586,7 @@ __global__ __launch_bounds__(256, FORM == ROWS_MIXED ? 2 : 3) void k_attn_rows(c
         }
         const int plim = pre ? kmax : lim, pmin = pre ? kmax : wmin;
         int kt = wid < NW ? kt0 + wid : kt1;
+        bool first = true;
         if (kt < kt1) {
             issue(kt, ksrc, kdst, false);
             issue(kt, vsrc, vdst, true);
@@ -597,7 +602,7 @@ __global__ __launch_bounds__(256, FORM == ROWS_MIXED ? 2 : 3) void k_attn_rows(c
             w.scores(lds, kat, s, [](int) {});
             asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(s) : : "memory");       // the tile's keys have been read
             if (more) issue(kt + NW, ksrc, kdst, false);
-            w.softmax(s, kbase + kKeys > pmin, plim - kbase - 4 * h2, kt == kt0 + wid);
+            w.softmax(s, kbase + kKeys > pmin, plim - kbase - 4 * h2, first);
             if (!more) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             else if (PIECES == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
             else asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
@@ -625,7 +630,7 @@ __global__ __launch_bounds__(256, FORM == ROWS_MIXED ? 2 : 3) void k_attn_rows(c
     // neighbouring groups of a row
     const int jr = p.part_o ? tid & 31 : tid >> 3, jq = p.part_o ? tid >> 5 : tid & 7, jt = (row0 + jr) / G, jg = row0 + jr - jt * G;
     if (jt >= n) return;
-    float mj[NW], wj[NW], m = -1e30f, l = 0.0f;
+    float mj[NW], wj[NW], m = kNoKeys, l = 0.0f;
 #pragma unroll
     for (int u = 0; u < NW; u++) {
         mj[u] = sml[(u * 32 + jr) * 2];
@@ -681,15 +686,15 @@ __global__ __launch_bounds__(256) void k_attn_join(const float *__restrict__ par
             x[g] = ok && j < parts ? *reinterpret_cast<const float4 *>(po + j * step * (32 * HD) + g * 1024) : make_float4(0.f, 0.f, 0.f, 0.f);
     };
     auto stat = [&](int j) {
-        return ok ? *reinterpret_cast<const float2 *>(part_ml + ((j * step + tt) * 32 + row) * 2) : make_float2(-1e30f, 0.0f);
+        return ok ? *reinterpret_cast<const float2 *>(part_ml + ((j * step + tt) * 32 + row) * 2) : make_float2(kNoKeys, 0.0f);
     };
 #pragma unroll
     for (int u = 0; u < U; u++) load(u, v[u]);                 // (on their way while the weights are worked out)
     const int edge = cu && tid < 2 ? cu[tid ? nseqs : 0] : tid ? rows : 0;
-    float m = -1e30f;
+    float m = kNoKeys;
     float2 st[KS];                                             // the first 32 parts' stay in registers
 #pragma unroll
-    for (int k = 0; k < KS; k++) st[k] = q + 8 * k < parts ? stat(q + 8 * k) : make_float2(-1e30f, 0.0f);
+    for (int k = 0; k < KS; k++) st[k] = q + 8 * k < parts ? stat(q + 8 * k) : make_float2(kNoKeys, 0.0f);
 #pragma unroll
     for (int k = 0; k < KS; k++) m = fmaxf(m, st[k].x);
     for (int j = q + 8 * KS; j < parts; j += 8) m = fmaxf(m, stat(j).x);

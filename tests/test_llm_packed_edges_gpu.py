@@ -113,3 +113,66 @@ def rounded_tol(q, k, v, scale):
     if k.size(0) == 0:
         return o, tol
     return o, tol + 2.0 ** -8 * (torch.softmax((k.double() @ q.double()) * scale, 0) @ v.double().abs())
+
+
+# ---- scores at the ends of f32 ---------------------------------------------------------------------------------------------
+def far_down(c):
+    """scores of every key about -360 in front of the exponential (dimension 1), a first head_dim in which the first keys may be infinite"""
+    nh, nkv, hd = c['heads']
+    q = c['qkv'][:, :nh * hd].view(-1, nh, hd)
+    q[..., 0], q[..., 1] = -1.0, 64.0
+    q[..., 2:] *= 0.1
+
+
+@pytest.mark.parametrize('heads,lens,past,split', [((4, 2, 128), [70], 130, False), ((4, 2, 128), [3], 3000, True), ((4, 1, 64), [1, 2], 700, False),
+                                                   ((12, 2, 128), [200], 0, False)])
+def test_packed_scores_of_minus_infinity_in_the_first_keys(dev, heads, lens, past, split):
+    """keys whose score is -inf (an infinite K element against a negative q) fill more than the first tile of every wave: their weight is 0
+    and the keys behind them keep theirs, however low their scores lie"""
+    c = packed_case(dev, heads, lens, [n + past for n in lens], spare=2, seed=past)
+    nh, nkv, hd = heads
+    far_down(c)
+    k = c['cache'][:, :, :nkv * hd].view(c['n'], c['S'], nkv, hd)
+    k[..., 1] = -64.0
+    k[:, :140 if past else 40, :, 0] = float('inf')
+    skip = 140 if past else 40
+    rows = [(at, q, kk[skip:], v[skip:]) for at, q, kk, v in packed_kv(c, 7) if kk.size(0) > skip]
+    assert rows
+    print('worst share %.2f' % compare(run_packed(c, dev, split), rows, 'minus infinity'))
+
+
+def test_prefix_scores_of_minus_infinity_in_the_first_keys(dev):
+    """the same in the shared keys, read in a launch with the own keys and in workgroups of their own"""
+    for heads, B, T, P in (((4, 1, 64), 2, 1, 300), ((12, 2, 128), 24, 2, 2000)):
+        c = prefix_case(dev, heads, B, T, P, [20 + b for b in range(B)], seed=P)
+        nh, nkv, hd = heads
+        far_down(c)
+        for kv in (c['prefix'], c['cache']):
+            kv.view(-1, kv.size(-1))[:, :nkv * hd].view(-1, nkv, hd)[..., 1] = -64.0
+        c['prefix'][:140, :nkv * hd].view(140, nkv, hd)[..., 0] = float('inf')
+        rows = [(at, q, k[140:], v[140:]) for at, q, k, v in prefix_kv(c, max(1, B * T // 8))]
+        print('worst share %.2f' % compare(run_prefix(c, dev), rows, 'minus infinity'))
+
+
+@pytest.mark.parametrize('past,split', [(0, False), (3000, True)])
+def test_packed_scores_near_the_lowest_f32(dev, past, split):
+    """scores of -1e34 and, for one key, half of that: its value is the result"""
+    heads = nh, nkv, hd = (4, 1, 64)
+    c = packed_case(dev, heads, [2], [2 + past + 50], seed=1)
+    c['qkv'][:, :nh * hd] = 0.0
+    c['qkv'][:, 0:nh * hd:hd] = 2.0 ** 58
+    n = c['klen'][0]
+    k = c['cache'][0, :n, :hd]
+    k.zero_()
+    k[:, 0] = -2.0 ** 58
+    at = n // 2
+    k[at, 0] = -2.0 ** 57
+    out = run_packed(c, dev, split)
+    assert torch.equal(out, c['cache'][0, at, hd:].expand_as(out))
+    x = prefix_case(dev, heads, 2, 1, n, [40, 50], seed=2)
+    x['qkv'][:, :nh * hd] = c['qkv'][:2, :nh * hd]
+    x['prefix'] = c['cache'][0, :n].contiguous()
+    x['cache'][:, :, :hd] = 0.0
+    x['cache'][:, :, 0] = -2.0 ** 58
+    out = run_prefix(x, dev)
+    assert torch.equal(out, c['cache'][0, at, hd:].expand_as(out))
