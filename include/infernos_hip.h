@@ -744,7 +744,7 @@ typedef struct ifh_verify_desc {
     const float *uniform;
     int32_t *out_tokens, *out_count;
     int32_t vocab, nrows, ndraft;
-    float temperature;
+    double temperature;
     void *ws;
     int64_t ws_bytes;
 } ifh_verify_desc;

@@ -161,7 +161,7 @@ class VerifyDesc(ctypes.Structure):
     """ifh_verify_desc (include/infernos_hip.h)"""
     _fields_ = [('logits', _vp), ('ld', _i64), ('draft_probs', _vp), ('q_ld', _i64), ('drafts', _vp), ('lens', _vp), ('uniform', _vp),
                 ('out_tokens', _vp), ('out_count', _vp), ('vocab', ctypes.c_int32), ('nrows', ctypes.c_int32),
-                ('ndraft', ctypes.c_int32), ('temperature', _f), ('ws', _vp), ('ws_bytes', _i64)]
+                ('ndraft', ctypes.c_int32), ('temperature', ctypes.c_double), ('ws', _vp), ('ws_bytes', _i64)]
 
 
 class RtpHdr(ctypes.Structure):

@@ -505,7 +505,7 @@ extern "C" int ifh_verify_drafts_f32(const ifh_verify_desc *d, ifh_stream_t stre
     IFH_CHECK_ARG(d->ndraft >= 0 && d->ndraft <= 63 && d->vocab >= 1 && verify_chunks(d->vocab) <= kVerifyMaxChunks);
     IFH_CHECK_ARG(d->logits && d->uniform && d->out_tokens && d->out_count && d->ws && (d->drafts || d->ndraft == 0));
     IFH_CHECK_ARG(d->ld >= d->vocab && (!d->draft_probs || d->q_ld >= d->vocab));
-    IFH_CHECK_ARG(d->temperature >= 0.0f && d->temperature <= 1e6f && (d->temperature == 0.0f || d->temperature >= 1e-6f));
+    IFH_CHECK_ARG(d->temperature >= 0.0 && d->temperature <= 1e6 && (d->temperature == 0.0 || d->temperature >= 1e-6));
     const int64_t positions = (int64_t)d->nrows * (d->ndraft + 1);
     IFH_CHECK_ARG(d->nrows < 65536 && positions < 65536);
     IFH_CHECK_ARG((((uintptr_t)d->ws) & 15) == 0 && d->ws_bytes >= ifh_verify_drafts_ws_bytes(d->nrows, d->ndraft));
@@ -514,8 +514,8 @@ extern "C" int ifh_verify_drafts_f32(const ifh_verify_desc *d, ifh_stream_t stre
     p.drafts = d->drafts; p.lens = d->lens; p.uniform = d->uniform;
     p.out_tokens = d->out_tokens; p.out_count = d->out_count;
     p.vocab = d->vocab; p.nrows = d->nrows; p.T = d->ndraft; p.nch = (int)verify_chunks(d->vocab);
-    p.greedy = d->temperature == 0.0f;
-    p.rate = 46.166241308446828 / (p.greedy ? 1.0 : (double)d->temperature);
+    p.greedy = d->temperature == 0.0;
+    p.rate = 46.166241308446828 / (p.greedy ? 1.0 : d->temperature);
     p.vec = (((uintptr_t)d->logits) & 15) == 0 && d->ld % 4 == 0;
     p.qvec = (((uintptr_t)d->draft_probs) & 15) == 0 && d->q_ld % 4 == 0;
     const bool mass = !p.greedy && p.q && p.T > 0;

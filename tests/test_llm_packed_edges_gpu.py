@@ -176,3 +176,38 @@ def test_packed_scores_near_the_lowest_f32(dev, past, split):
     x['cache'][:, :, 0] = -2.0 ** 58
     out = run_prefix(x, dev)
     assert torch.equal(out, c['cache'][0, at, hd:].expand_as(out))
+
+
+# ---- draft verification: borders -------------------------------------------------------------------------------------------
+def run_verify(dev, logits, drafts, u, V, temperature, q=None, ld=None, q_ld=None):
+    from infernos_amd import ops
+    B, T1 = u.shape
+    tok, cnt = torch.full((B, T1), -7, dtype=torch.int32, device=dev), torch.full((B,), -7, dtype=torch.int32, device=dev)
+    ws = ops.verify_drafts_ws(B, T1 - 1, dev)
+    ws.fill_(255)
+    ops.verify_drafts(logits, drafts, u, tok, cnt, ws, vocab=V, ld=V if ld is None else ld, nrows=B, ndraft=T1 - 1, temperature=temperature,
+                      draft_probs=q, q_ld=q_ld)
+    return tok, cnt
+
+
+@pytest.mark.parametrize('temp', [0.7, 1.3, 0.1])
+def test_the_temperature_is_the_callers_double(dev, temp):
+    """uniform numbers that lie between a border of softmax(logits / temp) and the same border with the temperature rounded to f32 (up to
+    5e-8 away), 2e-9 or more from the first: the token is the one of the caller's temperature.  (The masses are good to 1e-10.)"""
+    V, B = 4096, 400
+    g = torch.Generator(device=dev).manual_seed(7)
+    logits = torch.randn(B, V, generator=g, device=dev) * min(2.0, 2.0 * temp)
+    # (on the CPU: the device's softmax of f64 tensors is off by 1e-8)
+    c = [torch.softmax(logits.cpu().double() / t, 1).cumsum(1).to(dev) for t in (temp, float(torch.tensor(temp, dtype=torch.float32)))]
+    mid = (c[0] + c[1]) / 2
+    u = mid.float()
+    between = (u.double() - c[0]).sign() * (u.double() - c[1]).sign() < 0
+    ok = between & ((u.double() - c[0]).abs() > 2e-9) & (u < 1)
+    rows = ok.any(1)
+    at = ok.float().argmax(1)
+    u = u.gather(1, at[:, None])[rows].contiguous()
+    logits, c = logits[rows].contiguous(), c[0][rows]
+    want = torch.searchsorted(c, u.double(), right=True)[:, 0]
+    assert want.numel() >= 50
+    tok, cnt = run_verify(dev, logits, torch.zeros(1, 1, dtype=torch.int32, device=dev), u, V, temp)
+    assert torch.equal(tok[:, 0].long(), want), int((tok[:, 0].long() != want).sum())
