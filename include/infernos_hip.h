@@ -730,7 +730,8 @@ int ifh_attn_prefix_bf16(const ifh_attn_prefix_desc *desc, ifh_stream_t stream);
  * at the first refusal the token is drawn from max(p_i - q_i, 0) (from p_i where that is zero everywhere), behind the last draft from
  * p_n: the first token, in the order of the ids (or of the candidates), whose cumulated mass exceeds uniform[r][ndraft] times the whole.
  * out_tokens int32 [nrows][ndraft+1]: the kept drafts, the drawn token, then -1; out_count int32 [nrows]: kept + 1.  uniform f32
- * [nrows][ndraft+1] in [0, 1).  Masses and sums are f64, so the token does not depend on how a sum is split.
+ * [nrows][ndraft+1] in [0, 1).  Masses and sums are f64: a cumulated mass is within 2e-14 of the whole of its exact value, and only a
+ * uniform number that near to a border between two tokens can be taken for one on the border's other side.
  * A draft outside the vocabulary is refused; a row of logits with nothing above -inf refuses its draft and draws -1; NaN counts as -inf. */
 /* p_i = softmax(logits / temperature), f32 logits [nrows*(ndraft+1)][ld]; temperature 0: p_i is 1 at the arg-max (the lowest id of
  * equals).  draft_probs f32 [nrows*ndraft][q_ld], or NULL: q_i is 1 at the draft (a draft that was looked up, not drawn).

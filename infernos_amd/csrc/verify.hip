@@ -1,10 +1,10 @@
 // Verification of drafted tokens (speculative decoding by rejection): ifh_verify_drafts_f32 on whole distributions,
 // ifh_verify_drafts_topk on the top-k sampler's candidates.
 //
-// The draw compares a cumulated mass with a given number, and a vocabulary of 150 000 tokens has borders 1e-6 apart: masses are f64, so
-// that neither the way a sum is split nor the exponential's rounding moves a border past the number (f32 exponentials would move one in
-// every few hundred draws from a flat tail).  The f64 work (~19 operations a logit with the f32 ones) stays under the time the logits take to
-// arrive.
+// The draw compares a cumulated mass with a given number, and a vocabulary of 150 000 tokens has borders 1e-6 apart: masses are f64 to
+// their last bits, so that neither the way a sum is split nor the exponential's rounding moves a border past the number (f32 exponentials
+// would move one in every few hundred draws from a flat tail).  The f64 work (17 operations a logit) stays just under the time the logits
+// take to arrive.
 //   k_verify_stats   a wave or four a chunk of a target row: (max, sum of exp), or the arg-max for temperature 0.  Bound by memory: 320 rows of
 //                    151 936 logits, 194 MB, 41 us = 4.7 TB/s
 //   k_verify_mass    a wave or four a chunk of the refused position, where the draft has a distribution: the mass of max(p - q, 0).  64 rows of both,
@@ -30,25 +30,31 @@ __device__ const double kExp2[32] = {
     1.681792830507429, 1.7186192981224779, 1.7562521603732995, 1.7947090750031072, 1.8340080864093424, 1.8741676341103,
     1.9152065613971474, 1.9571441241754002
 };
+// 32 / (ln 2 temperature), and the difference of logits below which an exponential is 0
+struct Rate {
+    double rate, least;
+};
 __device__ __forceinline__ void exp_table(double entry, double (&tab)[32])       // entry: kExp2[threadIdx.x % 32], on its way
 {
     if (threadIdx.x < 32) tab[threadIdx.x] = entry;
     __syncthreads();
 }
-// e^x for x <= 0 in f64, relative error below 3e-11; y = x 32 / ln 2.  y = k + u, |u| <= 1/2 (k by adding and taking off 1.5 2^52), and
-// 2^(k/32) comes from the table (LDS: its 32 entries lie in 64 different banks) and k / 32.  e^(u ln 2 / 32) is 1, the linear term in f64,
-// and the Taylor polynomial's terms 2 to 4, no more than 6e-5 of the whole, in f32.  (Without a table, a polynomial of degree 9, it was
-// 27 operations a logit instead of 19.)
-__device__ __forceinline__ double exp_neg(double y, const double (&tab)[32])
+// e^x for x = d / temperature <= 0 in f64; relative error below 4e-16, and what the rate's rounding makes (2.2e-16 |x|).  d rate =
+// x 32 / ln 2 = k + u, |u| <= 1/2 (k by adding and taking off 1.5 2^52, the product never rounded), and 2^(k/32) comes from the table (LDS:
+// its 32 entries lie in 64 different banks) and k / 32.  e^(u ln 2 / 32) is the Taylor polynomial of degree 6 with u^6 replaced by the
+// Chebyshev polynomial's lower terms: degree 5, within 1.5e-16.
+__device__ __forceinline__ double exp_neg(double d, const Rate &r, const double (&tab)[32])
 {
     const double big = 6755399441055744.0;
-    y = fmax(y, -40000.0);
-    const double kb = y + big, u = y - (kb - big);
+    d = fmax(d, r.least);
+    const double kb = __builtin_fma(d, r.rate, big), u = __builtin_fma(d, r.rate, big - kb);
     const int k = (int)(uint32_t)__builtin_bit_cast(uint64_t, kb);
-    const float f = (float)u;
-    const float g = f * f * __builtin_fmaf(__builtin_fmaf(f, 9.1725627e-09f, 1.69385097e-06f), f, 0.000234596198f);
+    double g = __builtin_fma(u, 3.973709984549416e-11, 9.172616498033084e-09);
+    g = __builtin_fma(u, g, 1.693850972437182e-06);
+    g = __builtin_fma(u, g, 0.0002345961981972034);
+    g = __builtin_fma(u, g, 0.02166084939249829);
     const double t = tab[k & 31];
-    return __builtin_ldexp(__builtin_fma(t, __builtin_fma(u, 0.02166084939249829, (double)g), t), k >> 5);
+    return __builtin_ldexp(__builtin_fma(t, u * g, t), k >> 5);
 }
 
 // NaN counts as -inf; +inf as the largest finite value (its differences stay finite)
@@ -69,7 +75,7 @@ struct VerifyParams {
     const float *uniform;
     int32_t *out_tokens, *out_count;
     int vocab, nrows, T, nch;
-    double rate;                 // 32 / (ln 2 temperature)
+    Rate rate;
     int greedy, vec, qvec;
     double *csum;                // [rows * (T+1)][nch] chunk sums of exp((l - cmax) / temperature); greedy: the place of the chunk's maximum
     double *mass;                // [rows][nch]
@@ -184,8 +190,8 @@ template <int W> __global__ __launch_bounds__(VT) void k_verify_stats(const Veri
         double s1 = 0.0;
 #pragma unroll
         for (int e = 0; e < N; e += 2) {
-            s += exp_neg(((double)v[e] - md) * p.rate, tab);
-            s1 += exp_neg(((double)v[e + 1] - md) * p.rate, tab);
+            s += exp_neg((double)v[e] - md, p.rate, tab);
+            s1 += exp_neg((double)v[e + 1] - md, p.rate, tab);
         }
         s = wave_sum_d(s + s1);
     }
@@ -245,11 +251,11 @@ template <int NT> __device__ __forceinline__ Verdict verdict_of(const VerifyPara
             // (no chunk with a finite maximum: every sum is 0)
 #pragma unroll
             for (int k = 0; k < kVerifyMaxChunks / 64; k++)
-                if (k * 64 < p.nch) s += cs[k] * exp_neg(((double)fmaxf(cm[k], -kFltMax) - (double)fmaxf(m, -kFltMax)) * p.rate, tab);
+                if (k * 64 < p.nch) s += cs[k] * exp_neg((double)fmaxf(cm[k], -kFltMax) - (double)fmaxf(m, -kFltMax), p.rate, tab);
             s = wave_sum_d(s);
         }
         if (lane == 0) {
-            const double px = !in || !any ? 0.0 : p.greedy ? (x == best ? 1.0 : 0.0) : exp_neg(((double)logit(lx) - (double)m) * p.rate, tab) / s;
+            const double px = !in || !any ? 0.0 : p.greedy ? (x == best ? 1.0 : 0.0) : exp_neg((double)logit(lx) - (double)m, p.rate, tab) / s;
             L.keep[i] = in && any && u * qx < px;
             L.m[i] = m;
             L.s[i] = s;
@@ -295,7 +301,7 @@ template <int W> __global__ __launch_bounds__(VM) void k_verify_mass(const Verif
     double s = 0.0;
 #pragma unroll
     for (int e = 0; e < N; e++)
-        s += fmax(__builtin_fma(exp_neg(((double)logit(v[e]) - (double)w.m) * p.rate, tab), inv_s, -(double)q[e]), 0.0);
+        s += fmax(__builtin_fma(exp_neg((double)logit(v[e]) - (double)w.m, p.rate, tab), inv_s, -(double)q[e]), 0.0);
     s = wave_sum_d(s);
     if (W > 1) {
         if (lane == 0) ss[wid] = s;
@@ -357,12 +363,12 @@ __global__ __launch_bounds__(VD) void k_verify_draw(const VerifyParams p)
                 xv[e] = j < p.vocab && j != x ? row[j] : -INFINITY;
             }
         }
-        const double pm = csm * exp_neg(((double)fmaxf(cmx, -kFltMax) - md) * p.rate, tab);
+        const double pm = csm * exp_neg((double)fmaxf(cmx, -kFltMax) - md, p.rate, tab);
         double cm = qrow ? left : pm, total;
         if (x >= 0) {
             double s = 0.0, without;
 #pragma unroll
-            for (int e = 0; e < E; e++) s += exp_neg(((double)logit(xv[e]) - md) * p.rate, tab);
+            for (int e = 0; e < E; e++) s += exp_neg((double)logit(xv[e]) - md, p.rate, tab);
             block_scan(s, part[3], &without);
             if (tid == x / VC) cm = without;
         }
@@ -394,7 +400,7 @@ __global__ __launch_bounds__(VD) void k_verify_draw(const VerifyParams p)
         double mass[E], sum = 0.0, all;
 #pragma unroll
         for (int e = 0; e < E; e++) {
-            const double v = exp_neg(((double)logit(lv[e]) - md) * p.rate, tab);
+            const double v = exp_neg((double)logit(lv[e]) - md, p.rate, tab);
             mass[e] = rest && qrow ? fmax(__builtin_fma(v, inv_s, -(double)qv[e]), 0.0) : rest && j0 + e == x ? 0.0 : v;
             sum += mass[e];
         }
@@ -515,7 +521,8 @@ extern "C" int ifh_verify_drafts_f32(const ifh_verify_desc *d, ifh_stream_t stre
     p.out_tokens = d->out_tokens; p.out_count = d->out_count;
     p.vocab = d->vocab; p.nrows = d->nrows; p.T = d->ndraft; p.nch = (int)verify_chunks(d->vocab);
     p.greedy = d->temperature == 0.0;
-    p.rate = 46.166241308446828 / (p.greedy ? 1.0 : d->temperature);
+    p.rate.rate = 46.166241308446828 / (p.greedy ? 1.0 : d->temperature);
+    p.rate.least = -40000.0 / p.rate.rate;
     p.vec = (((uintptr_t)d->logits) & 15) == 0 && d->ld % 4 == 0;
     p.qvec = (((uintptr_t)d->draft_probs) & 15) == 0 && d->q_ld % 4 == 0;
     const bool mass = !p.greedy && p.q && p.T > 0;

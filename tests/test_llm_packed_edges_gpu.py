@@ -211,3 +211,21 @@ def test_the_temperature_is_the_callers_double(dev, temp):
     assert want.numel() >= 50
     tok, cnt = run_verify(dev, logits, torch.zeros(1, 1, dtype=torch.int32, device=dev), u, V, temp)
     assert torch.equal(tok[:, 0].long(), want), int((tok[:, 0].long() != want).sum())
+
+
+def test_masses_keep_the_bits_of_f64(dev):
+    """two tokens of logits 0 and d: the first is drawn while u (1 + e^d) < 1.  Of four million d those whose f32 number nearest to the
+    border lies within 3e-12 of it, but 2e-14 or more away (80-bit exponentials; f64 masses, their sum and the product are good to
+    1e-15): an exponential that is 1e-11 off takes the other token of many"""
+    import numpy as np
+    d = -np.arange(1 << 22, dtype=np.float64) * 2.0 ** -22 - 2.0 ** -23                     # exact in f32
+    e = np.exp(d.astype(np.longdouble))
+    u = (1 / (1 + e)).astype(np.float32)
+    gap = (u.astype(np.longdouble) * (1 + e) - 1).astype(np.float64)
+    at = np.nonzero((np.abs(gap) < 3e-12) & (np.abs(gap) > 2e-14))[0]
+    assert at.size > 100 and np.finfo(np.longdouble).eps < 1e-18 and (d.astype(np.float32) == d).all()
+    logits = torch.tensor(np.stack([np.zeros(at.size), d[at]], 1), dtype=torch.float32, device=dev)
+    want = torch.tensor(gap[at] > 0, device=dev).long()
+    tok, _ = run_verify(dev, logits, torch.zeros(1, 1, dtype=torch.int32, device=dev), torch.tensor(u[at], device=dev)[:, None].contiguous(), 2, 1.0)
+    wrong = int((tok[:, 0].long() != want).sum())
+    assert wrong == 0, (wrong, at.size)
