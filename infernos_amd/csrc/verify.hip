@@ -380,9 +380,10 @@ __global__ __launch_bounds__(VD) void k_verify_draw(const VerifyParams p)
             cum = block_scan(cm, part[1], &total);
         }
         const double want = u * total;
-        // (one LDS atomic a wave: one of every thread on one word cost 7 us)
+        // (one LDS atomic a wave: one of every thread on one word cost 7 us.  A chunk without mass is never the one: the sums of neighbouring
+        // lanes are associated differently, so its cum can lie a bit above its predecessor's)
         const int lane = tid & 63;
-        const unsigned long long past = __ballot(mine && cum > want);
+        const unsigned long long past = __ballot(mine && cm > 0.0 && cum > want);
         const unsigned long long with = __ballot(mine && cm > 0.0);
         if (past && lane == __ffsll((long long)past) - 1) atomicMin(&first[0], tid);
         if (with && lane == 63 - __clzll((long long)with)) atomicMax(&last[0], tid);

@@ -229,3 +229,15 @@ def test_masses_keep_the_bits_of_f64(dev):
     tok, _ = run_verify(dev, logits, torch.zeros(1, 1, dtype=torch.int32, device=dev), torch.tensor(u[at], device=dev)[:, None].contiguous(), 2, 1.0)
     wrong = int((tok[:, 0].long() != want).sum())
     assert wrong == 0, (wrong, at.size)
+
+
+def test_a_chunk_without_mass_is_not_drawn_from(dev):
+    """one token in each of the chunks 0, 1, 2 and 4 of 2048, of masses 2^-53, 2^-53, 1 and 1 (at this temperature a logit of -53 is exactly
+    that), nothing in chunk 3.  ((0 + 1) + (2^-53 + 2^-53)) is a bit more than ((1 + 2^-53) + 2^-53), so a sum up to chunk 3 may lie
+    above the number 1 that the draw looks for and the sum up to chunk 2 not: the token comes from a chunk that has one all the same"""
+    V = 5 * 2048
+    logits = torch.full((1, V), -float('inf'), device=dev)
+    at = [5, 2048 + 700, 4096 + 1, 8192 + 2047]
+    logits[0, at] = torch.tensor([-53.0, -53.0, 0.0, 0.0], device=dev)
+    tok, cnt = run_verify(dev, logits, torch.zeros(1, 1, dtype=torch.int32, device=dev), torch.tensor([[0.5]], device=dev), V, 1.4426950408889634)
+    assert int(tok[0, 0]) in at[2:] and int(cnt[0]) == 1, tok
