@@ -405,7 +405,8 @@ __global__ __launch_bounds__(VD) void k_verify_draw(const VerifyParams p)
             mass[e] = rest && qrow ? fmax(__builtin_fma(v, inv_s, -(double)qv[e]), 0.0) : rest && j0 + e == x ? 0.0 : v;
             sum += mass[e];
         }
-        const double upto = block_scan(sum, part[2], &all) + cut;
+        double upto = block_scan(sum, part[2], &all);
+        upto += cut;                                          // (behind the scan's barrier: thread c has written it)
         int at = -1, lastj = -1;
         double a = upto - sum;
 #pragma unroll
