@@ -724,6 +724,9 @@ typedef struct ifh_attn_prefix_desc {
 } ifh_attn_prefix_desc;
 int64_t ifh_attn_prefix_ws_floats(int nrows, int tokens_per_row, int prefix_keys, int nheads, int nkv, int head_dim, int max_keys);
 int ifh_attn_prefix_bf16(const ifh_attn_prefix_desc *desc, ifh_stream_t stream);
+/* how a call of these sizes with the whole workspace runs on the current device (a test's hook): 0 one launch, 1 a launch for both key sets
+ * and the join, 2 the same with both dealt in turn; + 4 / + 8: the prefix / the own keys in workgroups of 32 rows; -1: it is refused */
+int ifh_attn_prefix_form(int nrows, int tokens_per_row, int prefix_keys, int nheads, int nkv, int max_keys);
 /* Verification of drafted tokens (speculative decoding by rejection, which keeps the target's distribution).  Row r has ndraft drafts
  * (lens int32 [nrows], optional: its own number, 0 .. ndraft) and ndraft + 1 target rows, r * (ndraft+1) + i: the distribution p_i of the
  * token at draft i's place given the drafts before it.  Draft i, drawn from q_i, is kept while uniform[r][i] * q_i(x_i) < p_i(x_i);

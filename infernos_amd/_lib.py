@@ -219,6 +219,7 @@ SIGNATURES.update({
     'ifh_attn_packed_ws_floats': (_i64, [_i, _i, _i, _i, _i, _i]),
     'ifh_attn_packed_bf16': (_i, [ctypes.POINTER(AttnPackedDesc), _vp]),
     'ifh_attn_prefix_ws_floats': (_i64, [_i, _i, _i, _i, _i, _i, _i]),
+    'ifh_attn_prefix_form': (_i, [_i, _i, _i, _i, _i, _i]),
     'ifh_attn_prefix_bf16': (_i, [ctypes.POINTER(AttnPrefixDesc), _vp]),
     'ifh_verify_drafts_ws_bytes': (_i64, [_i, _i]),
     'ifh_verify_drafts_f32': (_i, [ctypes.POINTER(VerifyDesc), _vp]),

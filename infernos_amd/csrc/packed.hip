@@ -949,6 +949,24 @@ extern "C" int64_t ifh_attn_prefix_ws_floats(int nrows, int tokens_per_row, int 
     return part_floats(row_tiles_of((int64_t)nrows * tokens_per_row, nheads / nkv), nkv, a.parts + b.parts, head_dim);
 }
 
+static int64_t key_workgroups(const KeySet &k, int nkv) { return (int64_t)k.blocks * nkv * k.parts; }
+// how many 256s of workgroups of both key sets there are: dealt in turn (ROWS_BOTH) if any
+static int prefix_pairs(const KeySet &prefix, const KeySet &own, int nkv)
+{
+    const int64_t a = key_workgroups(prefix, nkv), b = key_workgroups(own, nkv);
+    return (int)((a < b ? a : b) / 256);
+}
+
+extern "C" int ifh_attn_prefix_form(int nrows, int tokens_per_row, int prefix_keys, int nheads, int nkv, int max_keys)
+{
+    if (nrows <= 0 || tokens_per_row <= 0 || nkv <= 0 || nheads < nkv || nheads % nkv || prefix_keys <= 0 || max_keys <= 0) return -1;
+    if (!prefix_fits((int64_t)nrows * tokens_per_row, nheads, nkv)) return -1;
+    KeySet a = {}, b = {};
+    prefix_plan(nrows, tokens_per_row, prefix_keys, nheads, nkv, max_keys, &a, &b);
+    const int form = prefix_joint((int64_t)b.blocks * nkv, prefix_keys, max_keys, b.narrow) ? 0 : prefix_pairs(a, b, nkv) > 0 ? 2 : 1;
+    return form | a.narrow << 2 | b.narrow << 3;
+}
+
 extern "C" int ifh_attn_prefix_bf16(const ifh_attn_prefix_desc *d, ifh_stream_t stream)
 {
     IFH_CHECK_ARG(d && d->nrows >= 0);
@@ -983,9 +1001,9 @@ extern "C" int ifh_attn_prefix_bf16(const ifh_attn_prefix_desc *d, ifh_stream_t 
     }
     p.part_o = d->ws;
     p.part_ml = d->ws + (int64_t)p.row_tiles * p.nkv * parts * 32 * d->head_dim;
-    const int64_t na = (int64_t)a.blocks * p.nkv * a.parts, nb = (int64_t)b.blocks * p.nkv * b.parts;
+    const int64_t na = key_workgroups(a, p.nkv), nb = key_workgroups(b, p.nkv);
     p.first = (int)na;
-    p.pairs = (int)((na < nb ? na : nb) / 256);
+    p.pairs = prefix_pairs(a, b, p.nkv);
     if (p.pairs == 0) {
         // few of either: the own keys' workgroups (more steps each) start first.  64 rows behind 2048 keys: 14.8 us, the prefix first 15.9;
         // where both fill the device dealing them in turn, the prefix first, is better (64 rows of 5 tokens behind 8001 keys: 110 us, own

@@ -178,6 +178,30 @@ def test_packed_scores_near_the_lowest_f32(dev, past, split):
     assert torch.equal(out, c['cache'][0, at, hd:].expand_as(out))
 
 
+# ---- every form of the shared-prefix launch --------------------------------------------------------------------------------
+JOINT, TWO, BOTH, NARROW_PREFIX, NARROW_OWN = 0, 1, 2, 4, 8
+
+
+@pytest.mark.parametrize('heads,B,T,P,own,form', [((14, 2, 64), 64, 3, 4000, 620, BOTH + NARROW_OWN), ((14, 2, 64), 128, 6, 1500, 300, BOTH),
+                                                  ((8, 8, 64), 96, 6, 2500, 90, BOTH + NARROW_OWN), ((16, 2, 64), 70, 5, 3001, 1100, BOTH),
+                                                  ((40, 8, 128), 40, 7, 1500, 2000, BOTH), ((12, 2, 128), 160, 1, 6000, 700, BOTH + NARROW_OWN),
+                                                  ((14, 2, 64), 20, 6, 900, 300, TWO + NARROW_PREFIX), ((14, 2, 64), 9, 1, 2000, 300, TWO + NARROW_PREFIX + NARROW_OWN),
+                                                  ((12, 2, 128), 3, 7, 1500, 700, TWO + NARROW_PREFIX), ((40, 8, 128), 9, 7, 900, 200, TWO),
+                                                  ((12, 2, 128), 96, 1, 2048, 300, TWO + NARROW_OWN),
+                                                  ((4, 1, 64), 5, 2, 500, 90, JOINT + NARROW_OWN)])
+def test_prefix_forms(dev, heads, B, T, P, own, form):
+    """the form that the sizes ask for, its rows of every kind: without an own key, with a part of the prefix or none of it"""
+    from infernos_amd import _lib
+    plen = [0 if b % 11 == 3 else P if b % 4 else 1 + (P * 7 * b) % P for b in range(B)]
+    lens = [-1 if b % 13 == 5 else (b * 7919) % (own + 1) for b in range(B)]
+    lens[0] = own
+    c = prefix_case(dev, heads, B, T, P, lens, plen=plen, seed=own)
+    assert _lib.lib().ifh_attn_prefix_form(B, T, P, heads[0], heads[1], c['max_keys']) == form
+    w = compare(run_prefix(c, dev), list(prefix_kv(c, max(1, B * T // 60))), 'prefix')
+    compare(run_prefix(c, dev, probs_bf16=True), list(prefix_kv(c, max(1, B * T // 30))), 'rounded', rounded_tol)
+    print('attn_prefix ok', heads, B, T, P, own, 'form', form, 'worst share %.2f' % w)
+
+
 # ---- draft verification: borders -------------------------------------------------------------------------------------------
 def run_verify(dev, logits, drafts, u, V, temperature, q=None, ld=None, q_ld=None):
     from infernos_amd import ops
