@@ -3,7 +3,7 @@ first tile empty, every kernel form, and draft verification at the sizes of a se
 import pytest
 import torch
 
-from test_llm_packed_gpu import BF, F64, dev, i32, packed_case, prefix_case        # noqa: F401  (dev is a fixture)
+from test_llm_packed_gpu import BF, F64, check_verified, dev, i32, packed_case, prefix_case, verify64        # noqa: F401  (dev is a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -203,14 +203,14 @@ def test_prefix_forms(dev, heads, B, T, P, own, form):
 
 
 # ---- draft verification: borders -------------------------------------------------------------------------------------------
-def run_verify(dev, logits, drafts, u, V, temperature, q=None, ld=None, q_ld=None):
+def run_verify(dev, logits, drafts, u, V, temperature, q=None, ld=None, q_ld=None, lens=None):
     from infernos_amd import ops
     B, T1 = u.shape
     tok, cnt = torch.full((B, T1), -7, dtype=torch.int32, device=dev), torch.full((B,), -7, dtype=torch.int32, device=dev)
     ws = ops.verify_drafts_ws(B, T1 - 1, dev)
     ws.fill_(255)
     ops.verify_drafts(logits, drafts, u, tok, cnt, ws, vocab=V, ld=V if ld is None else ld, nrows=B, ndraft=T1 - 1, temperature=temperature,
-                      draft_probs=q, q_ld=q_ld)
+                      draft_probs=q, q_ld=q_ld, lens=lens)
     return tok, cnt
 
 
@@ -265,3 +265,56 @@ def test_a_chunk_without_mass_is_not_drawn_from(dev):
     logits[0, at] = torch.tensor([-53.0, -53.0, 0.0, 0.0], device=dev)
     tok, cnt = run_verify(dev, logits, torch.zeros(1, 1, dtype=torch.int32, device=dev), torch.tensor([[0.5]], device=dev), V, 1.4426950408889634)
     assert int(tok[0, 0]) in at[2:] and int(cnt[0]) == 1, tok
+
+
+# ---- draft verification: a server's batches --------------------------------------------------------------------------------
+# A chunk is 2048 logits.  On 256 CUs a wave takes a chunk of the statistics where rows (drafts + 1) chunks > 8192, and of the remaining
+# mass where rows chunks > 3072, else four waves do: 64 x 5 x 75 and 64 x 75, 600 x 3 x 8 and 600 x 8, 500 x 3 x 5 and 500 x 5, 1100 x 2 x 4 and
+# 1100 x 4, 2 x 4 x 75.
+@pytest.mark.parametrize('B,T,V', [(64, 4, 151936), (600, 2, 14337), (500, 2, 8193), (1100, 1, 8000), (2, 3, 151936)])
+@pytest.mark.parametrize('pad,q_pad,temp', [(0, 0, 0.7), (0, None, 1.0), (3, 3, 1.3), (3, None, 0.7), (4, 3, 0.7), (3, 4, 1.0), (0, None, 0.0), (3, 0, 0.0)])
+def test_verify_batches(dev, B, T, V, pad, q_pad, temp):
+    """both kernel forms, several chunks a row and the last one in part, rows of logits and of the draft's distribution aligned and not
+    (q_pad None: looked-up drafts), a draft count for each row; some rows in 64 bits on the CPU"""
+    g = torch.Generator(device=dev).manual_seed(B + V + pad)
+    ld = -(-V // 4) * 4 + pad
+    logits = torch.full((B * (T + 1), ld), 50.0, device=dev)                     # (columns behind the vocabulary are not used)
+    logits[:, :V] = torch.randn(B * (T + 1), V, generator=g, device=dev) * 2
+    at = torch.randint(0, V, (B * (T + 1), 6), generator=g, device=dev)
+    logits.scatter_(1, at, 9.0 + torch.rand(at.shape, generator=g, device=dev))
+    logits[:, V - 1] = 8.0
+    t = temp or 1.0
+    q = q_ld = None
+    if q_pad is not None:
+        q_ld = -(-V // 4) * 4 + q_pad
+        q = torch.full((B * T, q_ld), 0.5, device=dev)
+        near = logits.view(B, T + 1, ld)[:, :T, :V].reshape(B * T, V) + 0.3 * torch.randn(B * T, V, generator=g, device=dev)
+        q[:, :V] = torch.softmax(near / t, 1)
+        drafts = torch.multinomial(q[:, :V], 1, generator=g).view(B, T)
+        del near
+    else:
+        pick = torch.randint(0, 6, (B, T, 1), generator=g, device=dev)
+        drafts = at.view(B, T + 1, 6)[:, :T].gather(2, pick)[:, :, 0]
+    drafts = drafts.to(torch.int32).contiguous()
+    if temp == 0:
+        logits.view(B, T + 1, ld)[:, :, 77] = 11.0                              # ties: the lowest id
+        logits.view(B, T + 1, ld)[::2, :, V - 1] = 11.0
+        drafts[::3] = 77
+    u = torch.rand(B, T + 1, generator=g, device=dev)
+    lens = [T - (r % 7 == 3) for r in range(B)]
+    tok, cnt = run_verify(dev, logits, drafts, u, V, temp, q, ld, q_ld, i32(lens, dev))
+    tok, cnt = tok.cpu(), cnt.cpu()
+    seen = set()
+    for r in sorted({0, B - 1, *range(1, B, max(1, B // 9))}):
+        l = logits[r * (T + 1):(r + 1) * (T + 1), :V].cpu().double()
+        d = drafts[r].cpu()
+        if temp == 0:
+            p = torch.nn.functional.one_hot((l == l.max(1, keepdim=True).values).to(torch.int8).argmax(1), V).double()
+        else:
+            p = torch.softmax(l / temp, 1)
+        qr = q[r * T:(r + 1) * T, :V].cpu().double() if q is not None else torch.nn.functional.one_hot(d.long(), V).double()
+        kept, mass, margin = verify64(p, qr, d, u[r].cpu(), lens[r])
+        assert margin > 1e-10
+        check_verified(tok, cnt, r, kept, mass, d, float(u[r, T]))
+        seen.add(kept)
+    print('verify ok', B, T, V, pad, q_pad, temp, 'kept', sorted(seen))
