@@ -14,15 +14,15 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 namespace ifh {
 
-// Last s with cu[s] <= i, or 0 (cu non-decreasing, n + 1 entries; i the same in the whole wave): the lanes probe 64 entries at a time, one
-// round trip up to 64 sequences, two up to 4096.
-__device__ __forceinline__ int packed_seq(const int32_t *__restrict__ cu, int n, int i)
+// Last s of the n sequences with reached(s), or 0 (reached: up to some s, the same for the whole wave): the lanes probe 64 of them at a time,
+// one round trip up to 64 sequences, two up to 4096.
+template <typename F> __device__ __forceinline__ int last_reached(int n, F reached)
 {
     const int lane = threadIdx.x & 63;
     int lo = 0, range = n;
     while (range > 1) {
         const int step = (range + 63) >> 6;
-        const int cnt = __popcll(__ballot(lane * step < range && cu[lo + lane * step] <= i));
+        const int cnt = __popcll(__ballot(lane * step < range && reached(lo + lane * step)));
         const int first = (cnt > 0 ? cnt - 1 : 0) * step;
         lo += first;
         range = min(step, range - first);
@@ -47,7 +47,8 @@ __global__ __launch_bounds__(256) void k_rope_packed(const uint16_t *__restrict_
     const uint16_t *src = qkv + i * qkv_ld + (int64_t)slot * hd;
     const uint4 lo = *reinterpret_cast<const uint4 *>(src + j), hi = *reinterpret_cast<const uint4 *>(src + j + half);
     // the wave's first token's sequence; a later token's lies behind it
-    int s = packed_seq(cu, nseqs, __builtin_amdgcn_readfirstlane(i));
+    const int i0 = __builtin_amdgcn_readfirstlane(i);
+    int s = last_reached(nseqs, [&](int at) { return cu[at] <= i0; });
     if (cu[s + 1] <= i) {
         int hi_s = nseqs;
         while (s < hi_s) {
@@ -105,7 +106,7 @@ struct RowsParams {
     uint16_t *out;
     int64_t o_ts;
     const int32_t *cu;
-    int ntokens, nseqs, nh, nkv, G, T;
+    int ntokens, nseqs, nkv, G, T;
     float scale;
     KeySet ks[2];
     int first, pairs;                      // workgroups of ks[0] (the others are ks[1]'s), and how many 256s of both are dealt in turn
@@ -373,26 +374,16 @@ __global__ __launch_bounds__(256, FORM == ROWS_MIXED ? 2 : 3) void k_attn_rows(c
     // kv head, row block, part: neighbours on different XCDs, so that with 2, 4 or 8 kv heads an XCD's L2 holds its own heads' keys
     const int G = p.G, kvh = id % p.nkv, bp = id / p.nkv, part = bp / ks.blocks;
     const int rs = narrow ? 5 : 7, R = 1 << rs;                // rows of a block
-    static_assert(kNarrowRows == 32 && kWideRows == 128, "");
+    static_assert(kNarrowRows == 1 << 5 && kWideRows == 1 << 7, "rows of a block");
     int xb = bp - part * ks.blocks;
 
     // the block's sequence: tokens [n0, n1), first row of the block within it, its cache row and the keys it may read
     int n0, n1, row0, kbatch, klen;
     if (mode == ROWS_PACKED) {
         // sequence s owns the block slots floor(cu[s] G / R) + s .. : at least ceil(len G / R) of them, so no table of blocks is needed;
-        // the last blocks of a long prompt see the most keys and start first.  The lanes probe 64 sequences at a time (one round trip up
-        // to 64 sequences, two up to 4096).
+        // the last blocks of a long prompt see the most keys and start first
         xb = ks.blocks - 1 - xb;
-        int lo = 0, range = p.nseqs;
-        while (range > 1) {
-            const int step = (range + 63) >> 6, at = lo + lane * step;
-            const bool le = lane * step < range && (int)(((int64_t)p.cu[at] * G) >> rs) + at <= xb;
-            const int cnt = __popcll(__ballot(le));
-            const int first = (cnt > 0 ? cnt - 1 : 0) * step;
-            lo += first;
-            range = min(step, range - first);
-        }
-        lo = __builtin_amdgcn_readfirstlane(lo);
+        const int lo = last_reached(p.nseqs, [&](int at) { return (int)(((int64_t)p.cu[at] * G) >> rs) + at <= xb; });
         n0 = min(max(p.cu[lo], 0), p.ntokens);
         n1 = min(max(p.cu[lo + 1], n0), p.ntokens);
         const int blk = xb - ((int)(((int64_t)n0 * G) >> rs) + lo);
@@ -899,7 +890,7 @@ extern "C" int ifh_attn_packed_bf16(const ifh_attn_packed_desc *d, ifh_stream_t 
     p.q = (const uint16_t *)d->q; p.q_ts = d->q_ts; p.v_off = d->v_off;
     p.out = (uint16_t *)d->out; p.o_ts = d->o_ts;
     p.cu = d->cu;
-    p.ntokens = d->ntokens; p.nseqs = d->nseqs; p.nh = d->nheads; p.nkv = d->nkv; p.T = 1;
+    p.ntokens = d->ntokens; p.nseqs = d->nseqs; p.nkv = d->nkv; p.T = 1;
     p.scale = d->scale;
     p.row_tiles = (int)row_tiles_of(d->ntokens, p.G);
     while (k.parts > 1 && (!d->ws || part_floats(p.row_tiles, p.nkv, k.parts, d->head_dim) > d->ws_floats)) fewer_parts(&k);
@@ -985,7 +976,7 @@ extern "C" int ifh_attn_prefix_bf16(const ifh_attn_prefix_desc *d, ifh_stream_t 
     b.kv = (const uint16_t *)d->cache; b.bs = d->cache_bs; b.ts = d->cache_ts; b.lim = d->key_len;
     p.q = (const uint16_t *)d->q; p.q_ts = d->q_ts; p.v_off = d->v_off;
     p.out = (uint16_t *)d->out; p.o_ts = d->o_ts;
-    p.ntokens = (int)ntokens; p.nseqs = d->nrows; p.nh = d->nheads; p.nkv = d->nkv; p.G = d->nheads / d->nkv; p.T = d->tokens_per_row;
+    p.ntokens = (int)ntokens; p.nseqs = d->nrows; p.nkv = d->nkv; p.G = d->nheads / d->nkv; p.T = d->tokens_per_row;
     p.scale = d->scale;
     p.row_tiles = (int)row_tiles_of(ntokens, p.G);
     while (a.parts + b.parts > 2 && part_floats(p.row_tiles, p.nkv, a.parts + b.parts, d->head_dim) > d->ws_floats) fewer_parts(a.parts >= b.parts ? &a : &b);

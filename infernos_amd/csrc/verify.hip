@@ -74,7 +74,7 @@ struct VerifyParams {
     const int32_t *drafts, *lens;
     const float *uniform;
     int32_t *out_tokens, *out_count;
-    int vocab, nrows, T, nch;
+    int vocab, T, nch;
     Rate rate;
     int greedy, vec, qvec;
     double *csum;                // [rows * (T+1)][nch] chunk sums of exp((l - cmax) / temperature); greedy: the place of the chunk's maximum
@@ -389,7 +389,7 @@ __global__ __launch_bounds__(VD) void k_verify_draw(const VerifyParams p)
         if (with && lane == 63 - __clzll((long long)with)) atomicMax(&last[0], tid);
         __syncthreads();
         const int c = first[0] != 0x7fffffff ? first[0] : max(last[0], 0);     // (a number of 1 or more: the last chunk with any mass)
-        // the chunk's tokens, two consecutive ones a thread
+        // the chunk's tokens, E consecutive ones a thread
         const int j0 = c * VC + tid * E;
         float lv[E], qv[E];
 #pragma unroll
@@ -521,7 +521,7 @@ extern "C" int ifh_verify_drafts_f32(const ifh_verify_desc *d, ifh_stream_t stre
     p.logits = d->logits; p.ld = d->ld; p.q = d->draft_probs; p.q_ld = d->q_ld;
     p.drafts = d->drafts; p.lens = d->lens; p.uniform = d->uniform;
     p.out_tokens = d->out_tokens; p.out_count = d->out_count;
-    p.vocab = d->vocab; p.nrows = d->nrows; p.T = d->ndraft; p.nch = (int)verify_chunks(d->vocab);
+    p.vocab = d->vocab; p.T = d->ndraft; p.nch = (int)verify_chunks(d->vocab);
     p.greedy = d->temperature == 0.0;
     p.rate.rate = 46.166241308446828 / (p.greedy ? 1.0 : d->temperature);
     p.rate.least = -40000.0 / p.rate.rate;
@@ -539,13 +539,13 @@ extern "C" int ifh_verify_drafts_f32(const ifh_verify_desc *d, ifh_stream_t stre
         hipLaunchKernelGGL(k_verify_stats<1>, dim3((unsigned)(p.nch + 3) / 4, (unsigned)positions), dim3(VT), 0, st, p);
     IFH_LAUNCH_CHECK("verify stats");
     if (mass) {
-        if ((int64_t)p.nrows * p.nch <= 12 * (int64_t)device_cu_count_physical())
-            hipLaunchKernelGGL(k_verify_mass<4>, dim3((unsigned)(p.nch + VM / 256 - 1) / (VM / 256), (unsigned)p.nrows), dim3(VM), 0, st, p);
+        if ((int64_t)d->nrows * p.nch <= 12 * (int64_t)device_cu_count_physical())
+            hipLaunchKernelGGL(k_verify_mass<4>, dim3((unsigned)(p.nch + VM / 256 - 1) / (VM / 256), (unsigned)d->nrows), dim3(VM), 0, st, p);
         else
-            hipLaunchKernelGGL(k_verify_mass<1>, dim3((unsigned)(p.nch + VM / 64 - 1) / (VM / 64), (unsigned)p.nrows), dim3(VM), 0, st, p);
+            hipLaunchKernelGGL(k_verify_mass<1>, dim3((unsigned)(p.nch + VM / 64 - 1) / (VM / 64), (unsigned)d->nrows), dim3(VM), 0, st, p);
         IFH_LAUNCH_CHECK("verify mass");
     }
-    hipLaunchKernelGGL(k_verify_draw, dim3((unsigned)p.nrows), dim3(VD), 0, st, p);
+    hipLaunchKernelGGL(k_verify_draw, dim3((unsigned)d->nrows), dim3(VD), 0, st, p);
     IFH_LAUNCH_CHECK("verify draw");
     return IFH_OK;
 }
