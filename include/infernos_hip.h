@@ -680,6 +680,8 @@ int ifh_rope_append_packed_bf16(const ifh_rope_packed_desc *desc, ifh_stream_t s
  * product as two bf16, within 2^-16 of themselves; probs_bf16 != 0: as one, within 2^-8, like ifh_attn_gqa_bf16's for prompts (faster
  * where the products bound: long prompts).  K and V from slot key_len on are not used, whatever they hold.  A K row that is not finite reaches only the tokens that see
  * it; V rows below key_len have to be finite, for a token multiplies those of its tiles that it does not see by zero.
+ * How the keys are cut, and with it the order of a row's f32 sums, follows ntokens, nseqs, max_keys and ws_floats: a sequence's last bits
+ * are the same in every call of these sizes, not in a batch of others.
  * ws: f32 workspace, with which few long rows are split along their keys: ifh_attn_packed_ws_floats() elements for the split that fills
  * the device (0: none is needed), a smaller one splits less, NULL not at all.  A workspace belongs to one stream / graph at a time. */
 typedef struct ifh_attn_packed_desc {
@@ -704,7 +706,8 @@ int ifh_attn_packed_bf16(const ifh_attn_packed_desc *desc, ifh_stream_t stream);
  * key_len[i] keys of cache row b.  The prefix is read once for all rows, not once a row.  A token that sees no key gets zeros.
  * tokens_per_row > 1: drafted tokens, each with its own key_len.  V rows of the prefix, and a row's own below its largest key_len, have
  * to be finite (see above).  ws: ifh_attn_prefix_ws_floats() f32 for the split that fills the device; a smaller one splits less, down to
- * two partial results a query row.  Of one stream / graph at a time.  probs_bf16: as above. */
+ * two partial results a query row.  Of one stream / graph at a time.  probs_bf16 and a
+ * row's bits (nrows, tokens_per_row, prefix_keys, max_keys): as above. */
 typedef struct ifh_attn_prefix_desc {
     const void *q;
     int64_t q_ts;

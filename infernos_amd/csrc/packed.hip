@@ -169,8 +169,8 @@ template <int HD> __device__ __forceinline__ int vperm(int r) { return HD == 128
 // ds_read_b64_tr_b16).  Sums and maxima are f32.  The second product takes P as the sum of two bf16 (P16 false: P rounded, and what the
 // rounding left, rounded: together within 2^-16 of P), so that the result has the bits of f32 probabilities; a caller may have the first
 // alone (P16: within 2^-8, as the prompt kernel of llm.hip), which saves one of three products and the splitting.  Us a call, sum and
-// rounded: one prompt of 8191 tokens, 40 / 8 heads of 128, 850 and 625; 64 prompts of 12 / 2 heads 32.7 and 29.6; 64 rows of 5 tokens behind
-// 8001 shared keys 118 and 101, 64 single tokens behind 2048 14.9 and 14.4.
+// rounded: one prompt of 8191 tokens, 40 / 8 heads of 128, 860 and 627; 64 prompts of 12 / 2 heads 35 and 31; 64 rows of 5 tokens behind
+// 8001 shared keys 120 and 104, 64 single tokens behind 2048 15.0 and 14.4.
 template <int HD, bool FEW, bool P16>
 struct WaveRows {
     static constexpr int NS = HD / 16, ND = HD / 32, ROWB = HD * 2;
@@ -329,17 +329,18 @@ struct WaveRows {
 //           from the end of the first product on, no barrier), and the four results are joined in LDS.  For the few rows of a decode step,
 //           whose work is bringing the keys: 128 rows would leave three waves idle.
 // and three instances of the kernel:
-//   ROWS_LONG    every workgroup is wide and its rows packed.  Three workgroups a CU (162 registers, 32 KB).  Bound by the matrix unit and
-//                the vector unit in turn, at the clock that the power budget leaves (a tile of a wave: 512 clocks of products, ~400 of
-//                softmax): one prompt of 8191 tokens, 40 / 8 heads of 128, 625-655 us = 1.05-1.10 PFLOP/s.
+//   ROWS_LONG    every workgroup is wide and its rows packed.  Three workgroups a CU (164 registers, 32 KB).  Bound by the matrix unit and
+//                the vector unit in turn, at the clock that the power budget leaves (a tile of a wave: 768 clocks of products, ~550 of
+//                softmax and splitting; 512 and ~400 with rounded probabilities): one prompt of 8191 tokens, 40 / 8 heads of 128,
+//                850-865 us = 0.8 PFLOP/s of the formula, 1.2 of the matrix unit (rounded 625-655 us, 1.05-1.10 of both).
 //   ROWS_MIXED   either form, decided at run time.  Two workgroups a CU (narrow: 68 KB, for four waves' buffers and results).  Bound by the
-//                latency of a few dependent loads: a step of 64 rows behind 2048 shared keys 10.5 us + 4 us for the join.
+//                latency of a few dependent loads: a step of 64 rows behind 2048 shared keys 11.3 us + 4 us for the join.
 //   ROWS_BOTH    wide and narrow ones that share a CU, where both key sets fill the device: two that multiply beside one that waits for
 //                memory.  A narrow workgroup has three waves with keys, so that three workgroups fit a CU's LDS, and fragment addresses are
 //                worked out again for every tile (two registers instead of twelve, so that three fit its registers).  Beside the other
 //                key set's traffic a tile takes longer to come than to multiply, so wide ones bring two ahead.  64 rows of 5 tokens behind
-//                8001 keys, 40 / 8 heads: 102 us (ROWS_MIXED 107); 48 rows of 4 behind 16000 110 us (124); 64 rows of 3 behind 4000, 14 / 2
-//                heads of 64, 18.4 us (19.7).  In the other two neither pays (ROWS_LONG with both: 1 % slower, ROWS_MIXED 2 %).
+//                8001 keys, 40 / 8 heads: 112 us (ROWS_MIXED 129); 48 rows of 4 behind 16000 118 us (132); 64 rows of 3 behind 4000, 14 / 2
+//                heads of 64, 21.5 us (22.7).  In the other two neither pays (ROWS_LONG with both: 1 % slower, ROWS_MIXED 2 %).
 template <int HD, int FORM, bool P16>
 __global__ __launch_bounds__(256, FORM == ROWS_MIXED ? 2 : 3) void k_attn_rows(const RowsParams p)
 {
@@ -763,20 +764,23 @@ extern "C" int ifh_rope_append_packed_bf16(const ifh_rope_packed_desc *d, ifh_st
 }
 
 // Fills in a key set's split for sequences (rows of a batch) of seq_rows rows.
-// Narrow workgroups where a narrow block holds a sequence's rows: with more, its keys are read once for every 32 rows.  Measured, narrow and
-// wide: 36 rows of 32 sequences behind 1000 keys 18.9 and 14.2 us, 64 rows of 4 behind 4000 16.3 and 15.3 us; with 6 rows (a decode step
-// of 64 sequences behind 1000 keys) 17.6 and 24 us.
+// Narrow workgroups where a narrow block holds a sequence's rows, for packed tokens those of the batch's mean sequence: with more, its keys
+// are read once for every 32 rows.  Measured, narrow and wide: 36 rows of 32 sequences behind 1000 keys 15.7 and 16.0 us (with rounded
+// probabilities 15.1 and 14.7), 64 rows of 4 behind 4000 14.2 and 14.5 us (13.7 and 13.5); with 6 rows (a decode step of 64 sequences behind
+// 1000 keys) 15.6 and 16.7 us.  A batch of long and short sequences has one form for both and is still better off together than in two
+// calls: 255 single tokens behind 200-1700 keys and a prompt of 1000, narrow, 65 us, alone 55 and 23; 63 behind 1000-3000 keys and a prompt
+// of 512, wide, 50 us, alone 39 and 16.
 // A prefix is read by narrow ones as long as seven workgroups for eight CUs do and their rows are four fifths full: its keys then come to
-// four waves at once (64 rows of 12 / 2 heads behind 2048 keys 14.5 us, wide 15.3; behind 8000 21.9 and 20.1; 96 rows behind 2048 17.6 and
-// 16.5; 8 rows of 40 / 8 heads, 40 rows in two blocks, behind 4000 15.7 and 13.9).
+// four waves at once (64 rows of 12 / 2 heads behind 2048 keys 14.9 us, wide 16.3; behind 8000 22.5 and 21.8; 96 rows behind 2048 18.3 and
+// 17.3; 8 rows of 40 / 8 heads, 40 rows in two blocks, behind 4000 15.5 and 14.7).
 // Keys are split into parts until the device has two workgroups a CU, and no further than that pays for the join's launch and for what
 // each part costs it: none of fewer than eight tiles (narrow: two a wave) or four (wide), and at most 1.6 sqrt(tiles) parts, the time of a
-// part being tiles / parts and that of the join parts (4 sequences of 4000 keys: 31 parts 15.7 us, 16 parts 14.0 us, 10 parts 15.5 us; one
-// of 8000: 63 parts 17.2 us, 25 parts 15.6 us, 15 parts 17.7 us).  Not at all, unless the results are joined anyway, up to 512 keys (wide)
+// part being tiles / parts and that of the join parts (4 sequences of 4000 keys: 31 parts 15.0 us, 16 parts 13.5 us, 10 parts 14.6 us; one
+// of 8000: 63 parts 17.7 us, 25 parts 14.4 us, 15 parts 15.6 us).  Not at all, unless the results are joined anyway, up to 512 keys (wide)
 // or 1024 (narrow), and past them while the workgroups that there are (0 to 256) make up for it, wide up to 7 and narrow up to 20 keys a
-// workgroup (whole and split: 64 sequences of 16 tokens, 300 keys, 7.4 and 9.4 us; one prompt of 300 rows 9.4 and 11.9 us, of 700 keys 15.7
-// and 12.8; 16 of 64 tokens behind 700 keys, 12 / 2 heads, 17.6 and 19.7 us, behind 1200 24.9 and 22.7; one token of 64 sequences behind 900
-// keys 13.3 and 18.4 us, behind 2000 28.4 and 30.9; of 16 sequences behind 2000 20.4 and 14.8).
+// workgroup (whole and split: 64 sequences of 16 tokens, 300 keys, 8.7 and 10.4 us; one prompt of 300 rows 10.1 and 11.1 us, of 700 keys 18.8
+// and 12.9; 16 of 64 tokens behind 700 keys, 12 / 2 heads, 23.0 and 21.6 us (rounded 19.9 and 20.2), behind 1200 34.4 and 27.4; one token of
+// 64 sequences behind 900 keys 15.5 and 19.2 us, behind 2000 30.3 and 36.7; of 16 sequences behind 2000 23.8 and 14.8).
 static void split_keys(KeySet *k, bool narrow, int64_t blocks, int nkv, int max_keys)
 {
     k->narrow = narrow;
@@ -916,9 +920,9 @@ static bool prefix_fits(int64_t ntokens, int64_t nheads, int64_t nkv)
 }
 
 // A short prefix is not worth a launch to share it: up to 640 keys in all (five tiles a wave) and two workgroups a CU, the workgroup of a
-// row's own keys reads the prefix too (from L2) and writes the result.  Measured, joint and shared: 2 rows of 333 + 40 keys 6.8 and 10.3
-// us, 64 rows of 300 + 200 15.1 and 18.4 us (40 / 8 heads); the shared form gains from about 700 keys on (64 rows of 600 + 150 12.2 and
-// 11.5 us, 16 rows of 2000 + 200 35.8 and 11.7 us).
+// row's own keys reads the prefix too (from L2) and writes the result.  Measured, joint and shared: 2 rows of 333 + 40 keys 7.6 and 10.5
+// us, 64 rows of 300 + 200 17.3 and 22.3 us (40 / 8 heads); the shared form gains from about 700 keys on (64 rows of 600 + 150 14.4 and
+// 11.9 us, 16 rows of 2000 + 200 26.8 and 12.2 us).
 static bool prefix_joint(int64_t workgroups, int prefix_keys, int max_keys, bool narrow)
 {
     return narrow && (int64_t)prefix_keys + max_keys <= 640 && workgroups <= 2 * (int64_t)device_cu_count_physical();
@@ -996,9 +1000,9 @@ extern "C" int ifh_attn_prefix_bf16(const ifh_attn_prefix_desc *d, ifh_stream_t 
     p.first = (int)na;
     p.pairs = prefix_pairs(a, b, p.nkv);
     if (p.pairs == 0) {
-        // few of either: the own keys' workgroups (more steps each) start first.  64 rows behind 2048 keys: 14.8 us, the prefix first 15.9;
-        // where both fill the device dealing them in turn, the prefix first, is better (64 rows of 5 tokens behind 8001 keys: 110 us, own
-        // keys first 117)
+        // few of either: the own keys' workgroups (more steps each) start first.  64 rows behind 2048 keys, rounded probabilities: 14.8 us, the
+        // prefix first 15.9; where both fill the device dealing them in turn, the prefix first, is better (64 rows of 5 tokens behind 8001
+        // keys: 110 us, own keys first 117)
         KeySet t = a;
         a = b;
         b = t;

@@ -8,9 +8,9 @@
 //   k_verify_stats   a wave or four a chunk of a target row: (max, sum of exp), or the arg-max for temperature 0.  Bound by memory: 320 rows of
 //                    151 936 logits, 194 MB, 41 us = 4.7 TB/s
 //   k_verify_mass    a wave or four a chunk of the refused position, where the draft has a distribution: the mass of max(p - q, 0).  64 rows of both,
-//                    78 MB, 15 us, 4 of them for the verdicts in front
+//                    78 MB, 15.5 us, 4 of them for the verdicts in front
 //   k_verify_draw    a workgroup a row: the chunk and then the token where the cumulated mass passes the uniform number.  A chain of
-//                    dependent loads and scans, 7 us for one row and for 64
+//                    dependent loads and scans, 6.4 us for one row and 6.0 for 64
 // A chunk is 2048 logits: one row of 151 936 is 75 of them, so that one call's few rows still spread over the device.
 #include "common.h"
 
@@ -148,8 +148,8 @@ __device__ __forceinline__ float wave_max_f(float v)
 }
 
 // W waves a chunk: one (no barrier), or a workgroup's four where there are few chunks for the device, so that a lane has 8 of the f64
-// exponentials and not 32.  Four up to 32 chunks a CU: one row of 3 drafts, 151 936 tokens, 3.4 us (one wave a chunk 4.8), the whole
-// verification of 16 rows of 4 drafts 27.9 us (30.1), but of 64 rows 69.3 us (66.6).
+// exponentials and not 32.  Four up to 32 chunks a CU: the whole verification of one row of 3 looked-up drafts, 151 936 tokens, 9.7 us (one
+// wave a chunk 10.9), of 16 rows of 4 drafts 24.3 us (26.0), of 32 rows 41.5 (41.2), but of 64 rows 69.4 us (64.7).
 template <int W> __global__ __launch_bounds__(VT) void k_verify_stats(const VerifyParams p)
 {
     constexpr int N = VPL / W;
@@ -273,8 +273,8 @@ template <int NT> __device__ __forceinline__ Verdict verdict_of(const VerifyPara
     return w;
 }
 
-// W waves a chunk, as above: four up to 12 chunks a CU (the whole verification of one row 13.8 us, one wave a chunk 15.5; 32 rows 43.6 and
-// 44.3; 64 rows 72.7 and 70.8)
+// W waves a chunk, as above: four up to 12 chunks a CU (the whole verification of one row of 4 drafts 12.5 us, one wave a chunk 13.7; 32 rows
+// 41.6 and 41.7; 64 rows 66.2 and 64.9)
 template <int W> __global__ __launch_bounds__(VM) void k_verify_mass(const VerifyParams p)
 {
     constexpr int N = VPL / W;
