@@ -329,7 +329,7 @@ struct WaveRows {
 //           from the end of the first product on, no barrier), and the four results are joined in LDS.  For the few rows of a decode step,
 //           whose work is bringing the keys: 128 rows would leave three waves idle.
 // and three instances of the kernel:
-//   ROWS_LONG    every workgroup is wide and its rows packed.  Three workgroups a CU (164 registers, 32 KB).  Bound by the matrix unit and
+//   ROWS_LONG    every workgroup is wide and its rows packed.  Three workgroups a CU (162 registers, 32 KB).  Bound by the matrix unit and
 //                the vector unit in turn, at the clock that the power budget leaves (a tile of a wave: 768 clocks of products, ~550 of
 //                softmax and splitting; 512 and ~400 with rounded probabilities): one prompt of 8191 tokens, 40 / 8 heads of 128,
 //                850-865 us = 0.8 PFLOP/s of the formula, 1.2 of the matrix unit (rounded 625-655 us, 1.05-1.10 of both).

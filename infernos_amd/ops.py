@@ -299,7 +299,7 @@ def attn_packed(q, cache, out, cu, key_len, *, ntokens, nseqs, nheads, nkv, head
     """causal grouped-query attention of sequences laid end to end (ifh_attn_packed_bf16): tokens cu[s] .. cu[s + 1] - 1 of sequence s
     against the first key_len[s] keys of cache row s, the last token seeing all of them.  q: the first nheads * head_dim columns of rows
     q_ts apart (None: the fused projection's).  probs_bf16: probabilities rounded to bf16 for the second product, as attn_gqa does on a prompt
-    (a third off a long prompt's time), instead of split in two bf16 that keep 16 bits"""
+    (a quarter off a long prompt's time), instead of split in two bf16 that keep 16 bits"""
     kv = nkv * head_dim
     d = _lib.AttnPackedDesc(q.data_ptr(), nheads * head_dim + 2 * kv if q_ts is None else q_ts, cache.data_ptr(), max_pos * 2 * kv, 2 * kv, kv,
                             out.data_ptr(), nheads * head_dim, cu.data_ptr(), key_len.data_ptr(), ntokens, nseqs, nheads, nkv, head_dim,
