@@ -676,10 +676,10 @@ int ifh_rope_append_packed_bf16(const ifh_rope_packed_desc *desc, ifh_stream_t s
 /* Causal grouped-query attention of sequences laid end to end: sequence s has the tokens cu[s] .. cu[s+1]-1 and the first key_len[s]
  * keys of cache row s; its last token sees all of them, the one before one fewer, and so on (new tokens behind what the row already
  * holds, themselves appended before).  A token that sees no key gets zeros; tokens behind cu[nseqs] keep what out holds.  Any number of
- * query heads per kv head; head_dim 64 or 128.  softmax(scale q.k) v, f32 sums; the probabilities go into the second
- * product as two bf16, within 2^-16 of themselves; probs_bf16 != 0: as one, within 2^-8, like ifh_attn_gqa_bf16's for prompts (faster
- * where the products bound: long prompts).  K and V from slot key_len on are not used, whatever they hold.  A K row that is not finite reaches only the tokens that see
- * it; V rows below key_len have to be finite, for a token multiplies those of its tiles that it does not see by zero.
+ * query heads per kv head; head_dim 64 or 128.  softmax(scale q.k) v, f32 sums; the probabilities go into the second product as two bf16,
+ * within 2^-16 of themselves; probs_bf16 != 0: as one, within 2^-8, like ifh_attn_gqa_bf16's for prompts (faster where the products bound:
+ * long prompts).  K and V from slot key_len on are not used, whatever they hold.  A K row that is not finite reaches only the tokens that
+ * see it; V rows below key_len have to be finite, for a token multiplies those of its tiles that it does not see by zero.
  * How the keys are cut, and with it the order of a row's f32 sums, follows ntokens, nseqs, max_keys and ws_floats: a sequence's last bits
  * are the same in every call of these sizes, not in a batch of others.
  * ws: f32 workspace, with which few long rows are split along their keys: ifh_attn_packed_ws_floats() elements for the split that fills
@@ -736,8 +736,8 @@ int ifh_attn_prefix_form(int nrows, int tokens_per_row, int prefix_keys, int nhe
  * at the first refusal the token is drawn from max(p_i - q_i, 0) (from p_i where that is zero everywhere), behind the last draft from
  * p_n: the first token, in the order of the ids (or of the candidates), whose cumulated mass exceeds uniform[r][ndraft] times the whole.
  * out_tokens int32 [nrows][ndraft+1]: the kept drafts, the drawn token, then -1; out_count int32 [nrows]: kept + 1.  uniform f32
- * [nrows][ndraft+1] in [0, 1).  Masses and sums are f64: a cumulated mass is within 2e-14 of the whole of its exact value, and only a
- * uniform number that near to a border between two tokens can be taken for one on the border's other side.
+ * [nrows][ndraft+1] in [0, 1).  Masses and sums are f64: a cumulated mass is within 2e-14 of its exact value (all of p being 1), and only
+ * a uniform number that near to a border between two tokens can be taken for one on the border's other side.
  * A draft outside the vocabulary is refused; a row of logits with nothing above -inf refuses its draft and draws -1; NaN counts as -inf. */
 /* p_i = softmax(logits / temperature), f32 logits [nrows*(ndraft+1)][ld]; temperature 0: p_i is 1 at the arg-max (the lowest id of
  * equals).  draft_probs f32 [nrows*ndraft][q_ld], or NULL: q_i is 1 at the draft (a draft that was looked up, not drawn).

@@ -318,7 +318,8 @@ def attn_prefix_ws(device, *, nrows, tokens_per_row, prefix_keys, nheads, nkv, h
 def attn_prefix(q, prefix, cache, out, key_len, *, nrows, tokens_per_row, prefix_keys, nheads, nkv, head_dim, max_pos, max_keys, ws,
                 prefix_len=None, q_ts=None, probs_bf16=False):
     """grouped-query attention of a decode step whose rows share a prefix (ifh_attn_prefix_bf16): token i of row b sees the first
-    prefix_len[b] keys of `prefix` [prefix_keys, 2 * nkv * head_dim] (None: all) and the first key_len[i] keys of cache row b.  probs_bf16: as in attn_packed"""
+    prefix_len[b] keys of `prefix` [prefix_keys, 2 * nkv * head_dim] (None: all) and the first key_len[i] keys of cache row b.
+    probs_bf16: as in attn_packed"""
     kv = nkv * head_dim
     d = _lib.AttnPrefixDesc(q.data_ptr(), nheads * head_dim + 2 * kv if q_ts is None else q_ts, prefix.data_ptr(), 2 * kv, cache.data_ptr(),
                             max_pos * 2 * kv, 2 * kv, kv, out.data_ptr(), nheads * head_dim, _ptr(prefix_len), key_len.data_ptr(), nrows,

@@ -268,9 +268,9 @@ def test_a_chunk_without_mass_is_not_drawn_from(dev):
 
 
 # ---- draft verification: a server's batches --------------------------------------------------------------------------------
-# A chunk is 2048 logits.  On 256 CUs a wave takes a chunk of the statistics where rows (drafts + 1) chunks > 8192, and of the remaining
-# mass where rows chunks > 3072, else four waves do: 64 x 5 x 75 and 64 x 75, 600 x 3 x 8 and 600 x 8, 500 x 3 x 5 and 500 x 5, 1100 x 2 x 4 and
-# 1100 x 4, 2 x 4 x 75.
+# A chunk is 2048 logits.  A wave takes a chunk of the statistics where there are more than 32 chunks a CU, and of the remaining mass where
+# more than 12, else four waves do; on 256 CUs: (64, 4, 151936) 94 and 19, (600, 2, 14337) 56 and 19, (500, 2, 8193) 29 and 10, (1100, 1,
+# 8000) 34 and 17, (2, 3, 151936) 2 and 1.
 @pytest.mark.parametrize('B,T,V', [(64, 4, 151936), (600, 2, 14337), (500, 2, 8193), (1100, 1, 8000), (2, 3, 151936)])
 @pytest.mark.parametrize('pad,q_pad,temp', [(0, 0, 0.7), (0, None, 1.0), (3, 3, 1.3), (3, None, 0.7), (4, 3, 0.7), (3, 4, 1.0), (0, None, 0.0), (3, 0, 0.0)])
 def test_verify_batches(dev, B, T, V, pad, q_pad, temp):
